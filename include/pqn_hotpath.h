@@ -647,6 +647,101 @@ int pqn_bigmlp_gemm(int32_t m, int32_t n, int32_t k, const float *a, int64_t lda
                     int64_t ldb, int32_t trans_b, const float *bias, float *c, int64_t ldc, int32_t nsplit,
                     int64_t split_stride, int32_t tile_rows, float *scratch, void *stream);
 
+/* ---- operators of sequence-memory networks ----------------------------------------------------------------------------- */
+/* What a Q-network with a memory needs between its Dense layers, for acting one step at a time and for learning on [T][M] windows:
+ * linear attention with a decay per head (the memory), the norms around a residual block, the log probabilities of taken actions.
+ * Tensors are f32, bf16 or f16 as `dtype` says; sums, states, statistics and parameters are f32, and a 16-bit output is rounded once,
+ * to nearest even.  Strides count elements; the last index of every tensor is contiguous, outputs are contiguous.  Outputs must not
+ * overlap inputs unless an entry says so.  Workspaces are scratch of one call: two calls that may run at the same time need two. */
+enum { PQN_DTYPE_F32 = 0, PQN_DTYPE_BF16 = 1, PQN_DTYPE_F16 = 2 };
+
+/* Linear attention with a decay per head, cut at episode ends (the role of ScannedRNN, pqn_rnn_gymnax.py:26-54: resets come BEFORE
+ * the step they are given for):
+ *   S_t = decay[h] (1 - reset[t][m]) S_{t-1} + k_t v_t^T       o_t = scale S_t^T q_t       per row m and head h, S_{-1} = state_in
+ * reset chooses: what it drops may be NaN or uninitialised.  decay in [0, 1] is a constant of the head, as gamma and lambda are of
+ * pqn_q_lambda: it has no gradient.  A window of one step is the recurrent form (acting); state_out may equal state_in.
+ * pqn_decay_attn      reads q, k, v, decay, state_in, reset; writes out, state_out
+ * pqn_decay_attn_grad reads those but out / state_out, and dout, dstate_out (the gradient of state_out); writes dq, dk, dv and, where
+ *                     wanted, dstate_in.  dstate_in may equal dstate_out.  Bit-identical in every run. */
+#define PQN_ATTN_MAX_D 128
+typedef struct {
+  int32_t t_len, m, heads, dk, dv; /* dk, dv <= PQN_ATTN_MAX_D */
+  int32_t dtype;                   /* PQN_DTYPE_F32 or PQN_DTYPE_BF16 */
+  float scale;
+  const void *q, *k;               /* [t_len][m][heads][dk] */
+  const void *v;                   /* [t_len][m][heads][dv] */
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* over (time, row, head) */
+  const float *decay;              /* [heads] */
+  const float *state_in;           /* [m][heads][dk][dv], NULL = zeros */
+  const uint8_t *reset;            /* [t_len][m], NULL = none */
+  void *out;                       /* [t_len][m][heads][dv] */
+  float *state_out;                /* [m][heads][dk][dv], NULL = not wanted */
+  const void *dout;                /* [t_len][m][heads][dv] */
+  int64_t dout_stride[3];
+  const float *dstate_out;         /* [m][heads][dk][dv], NULL = zeros */
+  void *dq, *dk_out, *dv_out;
+  float *dstate_in;                /* NULL = not wanted */
+  void *workspace;                 /* pqn_decay_attn_workspace_bytes, 16-byte aligned; NULL where that is 0 */
+} pqn_decay_attn_t;
+int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *args /* host */, int32_t grad);
+int pqn_decay_attn(const pqn_decay_attn_t *args /* host */, void *stream);
+int pqn_decay_attn_grad(const pqn_decay_attn_t *args /* host */, void *stream);
+
+/* The norms around a residual block, with the block's gate and residual scale, over the rows of [n][d]:
+ *   z = Norm(f) * post_scale + post_bias      y = x + res_scale * act(gate) * z      h = Norm(y) * pre_scale + pre_bias
+ * x: the residual stream, f: the block's output; Norm: LayerNorm (flax's eps of 1e-6 is the caller's) or RMSNorm.  post = 0: z = f;
+ * pre = 0: no h.  Every parameter is f32 [d], NULL = 1 (scales) or 0 (biases).  h is the norm of y before y's rounding to its type.
+ * pqn_residual_norm_grad reads dy, dh (one may be NULL = zeros) and writes dx, df, dgate and those of the parameter gradients that
+ * are not NULL; it recomputes what it needs from x, f, gate.  Bit-identical in every run.  d <= 8192. */
+enum { PQN_NORM_LAYER = 0, PQN_NORM_RMS = 1 };
+enum { PQN_GATE_NONE = 0, PQN_GATE_SIGMOID = 1, PQN_GATE_SILU = 2 };
+typedef struct {
+  int64_t n;
+  int32_t d, dtype, norm, gate_act, post, pre;
+  float eps;
+  const void *x, *f, *gate;                  /* [n][d]; gate NULL with PQN_GATE_NONE */
+  int64_t x_stride, f_stride, gate_stride;   /* between rows */
+  const float *res_scale, *post_scale, *post_bias, *pre_scale, *pre_bias;
+  void *y, *h;
+  const void *dy, *dh;
+  int64_t dy_stride, dh_stride;
+  void *dx, *df, *dgate;
+  float *dres_scale, *dpost_scale, *dpost_bias, *dpre_scale, *dpre_bias;
+  float *workspace;                          /* gradient only: pqn_residual_norm_workspace_floats */
+} pqn_residual_norm_t;
+int64_t pqn_residual_norm_workspace_floats(int64_t n, int32_t d);
+int pqn_residual_norm(const pqn_residual_norm_t *args /* host */, void *stream);
+int pqn_residual_norm_grad(const pqn_residual_norm_t *args /* host */, void *stream);
+
+/* Log probabilities of taken actions under softmax(logits / temperature) over the allowed columns (a Boltzmann policy over q, or a
+ * policy head), with the entropy, the logsumexp (temperature * lse = the soft value of q) and the top alternatives:
+ *   lse = log sum_j e^(x_j)   logp = x_action - lse   entropy = -sum_j p_j log p_j       x = logits / temperature where allowed
+ * mask (u8, 0 = not allowed, never looked at); a logit of -inf is not allowed either.  top_action / top_logp [n][top]: the largest
+ * allowed logits, ties to the lowest index, -1 / -inf where fewer are allowed.  An action outside 0 .. a-1 is none: logp 0, no
+ * gradient; one that is not allowed: logp -inf, no gradient.  A row that allows nothing: lse -inf, entropy 0, gradient 0.  NaN or +inf
+ * among the allowed logits: lse, logp, entropy NaN.
+ * pqn_action_logprobs_grad reads logits, action, mask, lse, entropy and the gradients of logp, entropy, lse (NULL = zeros, not all) and
+ * writes dlogits, 0 where not allowed. */
+#define PQN_LOGPROB_MAX_TOP 16
+typedef struct {
+  int32_t n, a, top, dtype;
+  float temperature;
+  const void *logits;              /* [n][a] */
+  int64_t logits_stride;           /* between rows */
+  const uint8_t *mask;             /* [n][a], NULL = all allowed */
+  int64_t mask_stride;
+  const int32_t *action;           /* [n] */
+  float *logp, *entropy, *lse;     /* [n] */
+  float *top_logp;                 /* [n][top] */
+  int32_t *top_action;             /* [n][top] */
+  const float *dlogp, *dentropy, *dlse; /* [n] */
+  void *dlogits;                   /* [n][a] */
+  void *workspace;                 /* forward only: pqn_action_logprobs_workspace_bytes, 8-byte aligned; NULL where that is 0 */
+} pqn_action_logprobs_t;
+int64_t pqn_action_logprobs_workspace_bytes(int32_t n, int32_t a);
+int pqn_action_logprobs(const pqn_action_logprobs_t *args /* host */, void *stream);
+int pqn_action_logprobs_grad(const pqn_action_logprobs_t *args /* host */, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

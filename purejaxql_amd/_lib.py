@@ -30,6 +30,40 @@ class StepOut(C.Structure):
                 ("returned_episode_lengths", c_void_p), ("timestep", c_void_p), ("achievements", c_void_p)]
 
 
+# element types of the sequence-memory operators
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+ATTN_MAX_D, LOGPROB_MAX_TOP = 128, 16
+
+
+class DecayAttnArgs(C.Structure):
+    """pqn_decay_attn_t"""
+    _fields_ = [("t_len", c_int32), ("m", c_int32), ("heads", c_int32), ("dk", c_int32), ("dv", c_int32), ("dtype", c_int32),
+                ("scale", c_float), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_stride", c_int64 * 3),
+                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("decay", c_void_p), ("state_in", c_void_p),
+                ("reset", c_void_p), ("out", c_void_p), ("state_out", c_void_p), ("dout", c_void_p), ("dout_stride", c_int64 * 3),
+                ("dstate_out", c_void_p), ("dq", c_void_p), ("dk_out", c_void_p), ("dv_out", c_void_p), ("dstate_in", c_void_p),
+                ("workspace", c_void_p)]
+
+
+class ResidualNormArgs(C.Structure):
+    """pqn_residual_norm_t"""
+    _fields_ = [("n", c_int64), ("d", c_int32), ("dtype", c_int32), ("norm", c_int32), ("gate_act", c_int32), ("post", c_int32),
+                ("pre", c_int32), ("eps", c_float), ("x", c_void_p), ("f", c_void_p), ("gate", c_void_p), ("x_stride", c_int64),
+                ("f_stride", c_int64), ("gate_stride", c_int64), ("res_scale", c_void_p), ("post_scale", c_void_p),
+                ("post_bias", c_void_p), ("pre_scale", c_void_p), ("pre_bias", c_void_p), ("y", c_void_p), ("h", c_void_p),
+                ("dy", c_void_p), ("dh", c_void_p), ("dy_stride", c_int64), ("dh_stride", c_int64), ("dx", c_void_p),
+                ("df", c_void_p), ("dgate", c_void_p), ("dres_scale", c_void_p), ("dpost_scale", c_void_p), ("dpost_bias", c_void_p),
+                ("dpre_scale", c_void_p), ("dpre_bias", c_void_p), ("workspace", c_void_p)]
+
+
+class ActionLogprobsArgs(C.Structure):
+    """pqn_action_logprobs_t"""
+    _fields_ = [("n", c_int32), ("a", c_int32), ("top", c_int32), ("dtype", c_int32), ("temperature", c_float), ("logits", c_void_p),
+                ("logits_stride", c_int64), ("mask", c_void_p), ("mask_stride", c_int64), ("action", c_void_p), ("logp", c_void_p),
+                ("entropy", c_void_p), ("lse", c_void_p), ("top_logp", c_void_p), ("top_action", c_void_p), ("dlogp", c_void_p),
+                ("dentropy", c_void_p), ("dlse", c_void_p), ("dlogits", c_void_p), ("workspace", c_void_p)]
+
+
 # name -> (restype, argtypes).  Every symbol include/pqn_hotpath.h declares.
 SIGNATURES = {
     "pqn_last_error": (C.c_char_p, []),
@@ -117,6 +151,15 @@ SIGNATURES = {
     "pqn_bigmlp_gemm_scratch_floats": (c_int64, [c_int32, c_int32, c_int32]),
     "pqn_bigmlp_gemm": (c_int, [c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_void_p,
                                 c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p]),
+    "pqn_decay_attn_workspace_bytes": (c_int64, [C.POINTER(DecayAttnArgs), c_int32]),
+    "pqn_decay_attn": (c_int, [C.POINTER(DecayAttnArgs), c_void_p]),
+    "pqn_decay_attn_grad": (c_int, [C.POINTER(DecayAttnArgs), c_void_p]),
+    "pqn_residual_norm_workspace_floats": (c_int64, [c_int64, c_int32]),
+    "pqn_residual_norm": (c_int, [C.POINTER(ResidualNormArgs), c_void_p]),
+    "pqn_residual_norm_grad": (c_int, [C.POINTER(ResidualNormArgs), c_void_p]),
+    "pqn_action_logprobs_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pqn_action_logprobs": (c_int, [C.POINTER(ActionLogprobsArgs), c_void_p]),
+    "pqn_action_logprobs_grad": (c_int, [C.POINTER(ActionLogprobsArgs), c_void_p]),
 }
 
 _lib = None

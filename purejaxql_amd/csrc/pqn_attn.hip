@@ -1,0 +1,243 @@
+// pqn_attn.hip -- linear attention with a decay per head over time-major windows, cut at episode ends, forward and gradient
+// (pqn_decay_attn, pqn_decay_attn_grad in include/pqn_hotpath.h).
+//
+//   S_t = decay_h (1 - reset_t) S_{t-1} + k_t v_t^T          o_t = scale S_t^T q_t            (S_-1 = the state that came in)
+//
+// The gradient is three scans of the same form.  With R_t = scale q_t do_t^T + decay_h (1 - reset_{t+1}) R_{t+1}, R_T-1 also holding
+// the gradient of the state that went out:
+//   dq_t = scale S_t do_t                 a forward scan with (do, v, k) for (q, k, v) and S transposed
+//   dk_t = R_t v_t                        a backward scan with (v, do, q) and R transposed
+//   dv_t = R_t^T k_t                      a backward scan with (k, q, do)
+//   d(state that came in) = decay_h (1 - reset_0) R_0
+// so one kernel serves the forward and, over three argument sets in one launch, the gradient; a backward scan is a forward one over
+// negative time strides.
+#include "pqn_vec.h"
+
+struct da_pass {
+  const void *q, *k, *v;
+  void *o;
+  long long qs[3], ks[3], vs[3], os[3];   // strides over (time, row, head) in elements
+  const float *s_in;
+  float *s_out;
+  int s_rs, s_cs;                         // element strides of the state's first (q, k) and second (v, o) index
+  const uint8_t *reset;                   // flag of the border before step i at reset[i * reset_ts + row]
+  long long reset_ts;
+  float o_scale, s_scale;                 // on the outputs; on what a step adds to the state
+  int a, b;                               // width of q, k; width of v, o
+  int late;                               // 0: a border (decay, reset) lies before every step.  1 (backward scans): before every step
+                                          // but the first, and one more behind the last step, before the state goes out
+};
+struct da_args {
+  da_pass pass[3];
+  int t_len, m, heads;
+  const float *decay;
+};
+
+// ---- the recurrence, step by step ------------------------------------------------------------------------------------------
+// A wave owns 32 columns of one (row, head)'s state in registers for the whole scan: 8 lanes x 4 columns across, 8 lane groups down
+// the rows, RPT rows per lane.  A step reads q, k, v once and reduces o over the lane groups by shuffles; no shared memory.
+template <int RPT, bool VEC>
+PQN_D void da_state_io(float (&s)[RPT][4], float *mem, const da_pass &P, int r0, int c0, bool write) {
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = r0 + 8 * i;
+    if (r >= P.a) continue;
+    float *p = mem + (long long)r * P.s_rs + (long long)c0 * P.s_cs;
+    if constexpr (VEC) {
+      if (c0 < P.b) {
+        if (write) pqn_store<float, 4>(p, s[i]);
+        else pqn_load<float, 4>(s[i], p);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + j < P.b) {
+          if (write) p[(long long)j * P.s_cs] = s[i][j];
+          else s[i][j] = p[(long long)j * P.s_cs];
+        }
+    }
+  }
+}
+
+template <typename T, int RPT, bool VEC>
+__global__ __launch_bounds__(256) void da_recur_kernel(da_args A) {
+  const da_pass &P = A.pass[blockIdx.y];
+  const int cb = (P.b + 31) >> 5;
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= (long long)A.m * A.heads * cb) return;             // whole waves
+  const int lane = threadIdx.x & 63;
+  const long long mh = unit / cb;
+  const int h = (int)(mh % A.heads), row = (int)(mh / A.heads);
+  const int c0 = (int)(unit % cb) * 32 + (lane & 7) * 4, r0 = lane >> 3;
+  const float decay = A.decay[h];
+  const T *q = (const T *)P.q + row * P.qs[1] + h * P.qs[2];
+  const T *k = (const T *)P.k + row * P.ks[1] + h * P.ks[2];
+  const T *v = (const T *)P.v + row * P.vs[1] + h * P.vs[2];
+  T *o = (T *)P.o + row * P.os[1] + h * P.os[2];
+  const long long so = mh * ((long long)P.a * P.b);
+  float s[RPT][4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+  if (P.s_in) da_state_io<RPT, VEC>(s, const_cast<float *>(P.s_in) + so, P, r0, c0, false);
+  for (int t = 0; t < A.t_len; ++t) {
+    float kr[RPT], qr[RPT], vc[4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = r0 + 8 * i;
+      kr[i] = r < P.a ? pqn_to_f32(k[t * P.ks[0] + r]) : 0.f;
+      qr[i] = r < P.a ? pqn_to_f32(q[t * P.qs[0] + r]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vc[j] = c0 + j < P.b ? pqn_to_f32(v[t * P.vs[0] + c0 + j]) * P.s_scale : 0.f;
+    if (t > 0 || !P.late) {
+      const bool cut = P.reset && P.reset[t * P.reset_ts + row];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = cut ? 0.f : s[i][j] * decay;   // a choice, not a product: what a reset drops may be NaN
+    }
+    float out[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(kr[i], vc[j], s[i][j]);
+        out[j] = fmaf(qr[i], s[i][j], out[j]);
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int d = 8; d < 64; d <<= 1) out[j] += __shfl_xor(out[j], d, 64);
+      if (r0 == 0 && c0 + j < P.b) o[t * P.os[0] + c0 + j] = (T)(out[j] * P.o_scale);
+    }
+  }
+  if (P.s_out) {
+    if (P.late && A.t_len > 0) {
+      const bool cut = P.reset && P.reset[A.t_len * P.reset_ts + row];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = cut ? 0.f : s[i][j] * decay;
+    }
+    da_state_io<RPT, VEC>(s, P.s_out + so, P, r0, c0, true);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+template <typename T>
+static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
+  int amax = 0, cbmax = 0;
+  bool vec = true;
+  for (int p = 0; p < passes; ++p) {
+    const da_pass &P = A.pass[p];
+    amax = P.a > amax ? P.a : amax;
+    cbmax = (P.b + 31) / 32 > cbmax ? (P.b + 31) / 32 : cbmax;
+    vec = vec && P.s_cs == 1 && P.b % 4 == 0 && (((uintptr_t)P.s_in | (uintptr_t)P.s_out) & 15) == 0;
+  }
+  const long long units = (long long)A.m * A.heads * cbmax, blocks = (units + 3) / 4;
+  const dim3 grid((unsigned)blocks, passes);
+#define DA_GO(RPT)                                                          \
+  do {                                                                      \
+    if (vec) da_recur_kernel<T, RPT, true><<<grid, 256, 0, st>>>(A);        \
+    else da_recur_kernel<T, RPT, false><<<grid, 256, 0, st>>>(A);           \
+    return pqn_check_launch("pqn_decay_attn");                              \
+  } while (0)
+  if (amax <= 32) DA_GO(4);
+  if (amax <= 64) DA_GO(8);
+  DA_GO(16);
+#undef DA_GO
+}
+
+static int da_check(const pqn_decay_attn_t *a, const char *who) {
+  PQN_REQUIRE(a, "%s: NULL argument block", who);
+  PQN_REQUIRE(a->dtype == PQN_DTYPE_F32 || a->dtype == PQN_DTYPE_BF16, "%s: dtype %d is neither f32 nor bf16", who, a->dtype);
+  PQN_REQUIRE(a->t_len >= 0 && a->m >= 0 && a->heads > 0, "%s: t_len, m must be >= 0 and heads > 0 (%d, %d, %d)", who, a->t_len, a->m, a->heads);
+  PQN_REQUIRE(a->dk > 0 && a->dk <= PQN_ATTN_MAX_D && a->dv > 0 && a->dv <= PQN_ATTN_MAX_D, "%s: head widths of 1 .. %d (dk=%d dv=%d)", who,
+              PQN_ATTN_MAX_D, a->dk, a->dv);
+  PQN_REQUIRE((long long)a->m * a->heads <= (1ll << 28), "%s: up to 2^28 (row, head) pairs (m=%d heads=%d)", who, a->m, a->heads);
+  PQN_REQUIRE(a->decay || a->m == 0, "%s: NULL decay", who);
+  PQN_REQUIRE((a->q && a->k && a->v) || a->t_len == 0 || a->m == 0, "%s: NULL q, k or v", who);
+  return PQN_OK;
+}
+
+static void da_strides(long long (&to)[3], const int64_t *from, bool reverse) {
+  to[0] = reverse ? -from[0] : from[0];
+  to[1] = from[1];
+  to[2] = from[2];
+}
+// a tensor over (time, row, head): its first element in scan order and its strides
+static const void *da_first(const void *p, const int64_t *s, int t_len, int es, bool reverse) {
+  return (reverse && t_len > 0) ? (const char *)p + (long long)(t_len - 1) * s[0] * es : p;
+}
+
+static da_pass da_make(const pqn_decay_attn_t *a, const void *q, const int64_t *qs, const void *k, const int64_t *ks, const void *v,
+                       const int64_t *vs, void *o, int wq, int wv, bool reverse) {
+  const int es = pqn_dtype_size(a->dtype);
+  da_pass P = {};
+  const int64_t os[3] = {(int64_t)a->m * a->heads * wv, (int64_t)a->heads * wv, wv};
+  P.q = da_first(q, qs, a->t_len, es, reverse);
+  P.k = da_first(k, ks, a->t_len, es, reverse);
+  P.v = da_first(v, vs, a->t_len, es, reverse);
+  P.o = const_cast<void *>(da_first(o, os, a->t_len, es, reverse));
+  da_strides(P.qs, qs, reverse);
+  da_strides(P.ks, ks, reverse);
+  da_strides(P.vs, vs, reverse);
+  da_strides(P.os, os, reverse);
+  P.a = wq;
+  P.b = wv;
+  // backward scans meet the border between steps t and t + 1 in front of their step T - 1 - t: flag t + 1 = T - i
+  P.reset = a->reset ? a->reset + (reverse ? (long long)a->t_len * a->m : 0) : nullptr;
+  P.reset_ts = reverse ? -(long long)a->m : a->m;
+  P.late = reverse;
+  P.o_scale = reverse ? 1.f : a->scale;
+  P.s_scale = reverse ? a->scale : 1.f;
+  return P;
+}
+
+extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
+  const int rc = da_check(a, "pqn_decay_attn");
+  if (rc != PQN_OK) return rc;
+  if (a->m == 0 || (a->t_len == 0 && !a->state_out)) return PQN_OK;
+  PQN_REQUIRE(a->out || a->t_len == 0, "pqn_decay_attn: NULL out");
+  da_args A = {};
+  A.t_len = a->t_len; A.m = a->m; A.heads = a->heads; A.decay = a->decay;
+  da_pass &P = A.pass[0];
+  P = da_make(a, a->q, a->q_stride, a->k, a->k_stride, a->v, a->v_stride, a->out, a->dk, a->dv, false);
+  P.s_in = a->state_in;
+  P.s_out = a->state_out;
+  P.s_rs = a->dv;
+  P.s_cs = 1;
+  return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 1, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 1, (hipStream_t)stream);
+}
+
+extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
+  const int rc = da_check(a, "pqn_decay_attn_grad");
+  if (rc != PQN_OK) return rc;
+  if (a->m == 0 || (a->t_len == 0 && !a->dstate_in)) return PQN_OK;
+  PQN_REQUIRE((a->dout && a->dq && a->dk_out && a->dv_out) || a->t_len == 0, "pqn_decay_attn_grad: NULL dout, dq, dk or dv");
+  da_args A = {};
+  A.t_len = a->t_len; A.m = a->m; A.heads = a->heads; A.decay = a->decay;
+  da_pass &Q = A.pass[0], &K = A.pass[1], &V = A.pass[2];
+  Q = da_make(a, a->dout, a->dout_stride, a->v, a->v_stride, a->k, a->k_stride, a->dq, a->dv, a->dk, false);
+  Q.s_in = a->state_in;
+  Q.s_rs = 1;
+  Q.s_cs = a->dv;
+  K = da_make(a, a->v, a->v_stride, a->dout, a->dout_stride, a->q, a->q_stride, a->dk_out, a->dv, a->dk, true);
+  K.s_in = a->dstate_out;
+  K.s_rs = 1;
+  K.s_cs = a->dv;
+  V = da_make(a, a->k, a->k_stride, a->q, a->q_stride, a->dout, a->dout_stride, a->dv_out, a->dk, a->dv, true);
+  V.s_in = a->dstate_out;
+  V.s_out = a->dstate_in;
+  V.s_rs = a->dv;
+  V.s_cs = 1;
+  return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 3, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 3, (hipStream_t)stream);
+}
+
+extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
+  (void)a;
+  (void)grad;
+  return 0;
+}

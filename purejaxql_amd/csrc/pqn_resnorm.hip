@@ -1,0 +1,432 @@
+// pqn_resnorm.hip -- the norms around a residual block with the block's gate and residual scale, forward and gradient, one pass over
+// the rows each (pqn_residual_norm, pqn_residual_norm_grad in include/pqn_hotpath.h).
+//
+//   z = Norm(f)      n = z * post_scale + post_bias      y = x + res_scale * act(g) * n      u = Norm(y)      h = u * pre_scale + pre_bias
+//
+// A row lives in the registers of one wave (up to 1024 columns) or of one workgroup (up to 8192) from its load to its store, so the
+// forward reads x, f, g once and writes y, h once, and the gradient reads x, f, g, dy, dh once and writes dx, df, dg once; both norms'
+// statistics are taken twice over the registers (mean, then the centred sum of squares), in f32.  The gradient recomputes y in f32
+// from x, f, g instead of reading a stored y: the same bytes, and no rounding between the two halves.
+#include "pqn_vec.h"
+
+static constexpr int RN_MAX = 16;         // columns per thread: five row tensors and five column sums stay in registers
+static constexpr int RN_MAX_D = 512 * RN_MAX;
+
+struct rn_args {
+  long long n;
+  int d;
+  int rms, gate_act, has_post, has_pre;
+  float eps;
+  const void *x, *f, *g;
+  long long xs, fs, gs;                   // row strides in elements
+  const float *res_scale, *post_scale, *post_bias, *pre_scale, *pre_bias;
+  void *y, *h;
+  const void *dy, *dh;
+  long long dys, dhs;
+  void *dx, *df, *dg;
+  float *partials;                        // [gridDim.x][RN_PARAMS][d]
+};
+enum { RN_RES = 0, RN_POST_SCALE, RN_POST_BIAS, RN_PRE_SCALE, RN_PRE_BIAS, RN_PARAMS };
+
+// sum of NV values at once over the NT threads that hold a row
+template <int NT, int K>
+PQN_D void rn_row_sum(float (&v)[K], float *lds) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = pqn_group_sum<64>(v[k]);
+  if constexpr (NT > 64) {
+    constexpr int NW = NT / 64;
+    __syncthreads();                      // the values of the previous sum have been read
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) lds[k * NW + (threadIdx.x >> 6)] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) s += lds[k * NW + w];
+      v[k] = s;
+    }
+  }
+}
+
+template <typename T, int NT, int VW, int NV>
+struct RnRow {
+  static constexpr int E = VW * NV;
+  PQN_D static int col(int lane, int i) { return (i * NT + lane) * VW; }
+  // columns behind d hold zeros, which no sum notices
+  PQN_D static void load(float (&r)[E], const void *base, long long off, int d, int lane) {
+    const T *p = (const T *)base + off;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(lane, i);
+      if (c < d) pqn_load<T, VW>(r + i * VW, p + c);
+      else
+#pragma unroll
+        for (int j = 0; j < VW; ++j) r[i * VW + j] = 0.f;
+    }
+  }
+  PQN_D static void store(void *base, long long off, const float (&r)[E], int d, int lane) {
+    T *p = (T *)base + off;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(lane, i);
+      if (c < d) pqn_store<T, VW>(p + c, r + i * VW);
+    }
+  }
+  PQN_D static void param(float (&r)[E], const float *p, float absent, int d, int lane) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(lane, i);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) r[i * VW + j] = (p && c < d) ? p[c + j] : absent;
+    }
+  }
+  // r -> (r - mean) * inv in place; returns inv = 1 / sqrt(var + eps).  rms: mean = 0
+  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds) {
+    if (!rms) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[0] += r[e];
+      rn_row_sum<NT>(s, lds);
+      const float mean = s[0] / (float)d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = col(lane, i) < d;
+#pragma unroll
+        for (int j = 0; j < VW; ++j) r[i * VW + j] = in ? r[i * VW + j] - mean : 0.f;
+      }
+    }
+    float q[1] = {0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[0] = fmaf(r[e], r[e], q[0]);
+    rn_row_sum<NT>(q, lds);
+    const float inv = 1.0f / sqrtf(q[0] / (float)d + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] *= inv;
+    return inv;
+  }
+  // gradient of the normalisation: dz -> d(input), z = the normalised row
+  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds) {
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s[0] = fmaf(dz[e], z[e], s[0]);
+      s[1] += dz[e];
+    }
+    rn_row_sum<NT>(s, lds);
+    const float a = s[0] / (float)d, b = rms ? 0.f : s[1] / (float)d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool in = col(lane, i) < d;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) dz[i * VW + j] = in ? (dz[i * VW + j] - z[i * VW + j] * a - b) * inv : 0.f;
+    }
+  }
+};
+
+// act(g) and its slope
+PQN_D void rn_act(int kind, float g, float &act, float &slope) {
+  act = 1.f;
+  slope = 0.f;
+  if (kind == PQN_GATE_NONE) return;
+  const float s = 1.0f / (1.0f + expf(-g));
+  if (kind == PQN_GATE_SIGMOID) {
+    act = s;
+    slope = s * (1.0f - s);
+  } else {
+    act = g * s;
+    slope = s * (1.0f + g * (1.0f - s));
+  }
+}
+
+// WPB waves (NT = 64) or one row (NT > 64) per workgroup
+template <typename T, int NT, int VW, int NV>
+__global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
+  using Row = RnRow<T, NT, VW, NV>;
+  constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
+  __shared__ float lds[2 * 16];
+  const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63;
+  const int d = A.d;
+  const long long row = (long long)blockIdx.x * RPB + (NT > 64 ? 0 : threadIdx.x >> 6);
+  if (row >= A.n) return;                 // whole waves / workgroups
+  float z[E], y[E], p[E];
+  Row::load(z, A.f, row * A.fs, d, lane);
+  Row::load(y, A.x, row * A.xs, d, lane);
+  if (A.has_post) {
+    Row::normalise(z, A.rms, A.eps, d, lane, lds);
+    Row::param(p, A.post_scale, 1.f, d, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] *= p[e];
+    if (A.post_bias) {
+      Row::param(p, A.post_bias, 0.f, d, lane);
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] += p[e];
+    }
+  }
+  if (A.gate_act != PQN_GATE_NONE) {
+    Row::load(p, A.g, row * A.gs, d, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float act, slope;
+      rn_act(A.gate_act, p[e], act, slope);
+      z[e] *= act;
+    }
+  }
+  Row::param(p, A.res_scale, 1.f, d, lane);
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = fmaf(p[e], z[e], y[e]);
+  Row::store(A.y, row * d, y, d, lane);
+  if (A.has_pre) {
+    Row::normalise(y, A.rms, A.eps, d, lane, lds);
+    Row::param(p, A.pre_scale, 1.f, d, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] *= p[e];
+    if (A.pre_bias) {
+      Row::param(p, A.pre_bias, 0.f, d, lane);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] += p[e];
+    }
+    Row::store(A.h, row * d, y, d, lane);
+  }
+}
+
+// Rows blockIdx, blockIdx + gridDim, ... : the parameter gradients are summed over a thread's rows in registers and leave the
+// workgroup as one partial row per parameter, summed in a fixed order by rn_param_kernel (the same result in every run).
+template <typename T, int NT, int VW, int NV>
+__global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
+  using Row = RnRow<T, NT, VW, NV>;
+  constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
+  __shared__ float lds[2 * 16];
+  __shared__ float fold[NT > 64 ? 1 : 3 * 64 * E];
+  const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63, wave = NT > 64 ? 0 : threadIdx.x >> 6;
+  const int d = A.d;
+  float sum[RN_PARAMS][E];
+#pragma unroll
+  for (int k = 0; k < RN_PARAMS; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[k][e] = 0.f;
+  for (long long row = (long long)blockIdx.x * RPB + wave; row < A.n; row += (long long)gridDim.x * RPB) {
+    float z[E], y[E], e_[E], p[E], g[E];
+    Row::load(z, A.f, row * A.fs, d, lane);
+    Row::load(y, A.x, row * A.xs, d, lane);
+    if (A.gate_act != PQN_GATE_NONE) Row::load(g, A.g, row * A.gs, d, lane);
+    if (A.dy) Row::load(e_, A.dy, row * A.dys, d, lane);
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) e_[e] = 0.f;
+    float inv_f = 1.f;
+    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds);
+    float ps[E], pb[E], rs[E];
+    Row::param(ps, A.post_scale, 1.f, d, lane);
+    Row::param(pb, A.post_bias, 0.f, d, lane);
+    Row::param(rs, A.res_scale, 1.f, d, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float act, slope;
+      rn_act(A.gate_act, g[e], act, slope);
+      y[e] = fmaf(rs[e], act * fmaf(z[e], ps[e], pb[e]), y[e]);
+    }
+    if (A.dh) {
+      float dh[E];
+      Row::load(dh, A.dh, row * A.dhs, d, lane);
+      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds);
+      Row::param(p, A.pre_scale, 1.f, d, lane);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        sum[RN_PRE_SCALE][e] = fmaf(dh[e], y[e], sum[RN_PRE_SCALE][e]);
+        sum[RN_PRE_BIAS][e] += dh[e];
+        dh[e] *= p[e];
+      }
+      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds);
+#pragma unroll
+      for (int e = 0; e < E; ++e) e_[e] += dh[e];
+    }
+    Row::store(A.dx, row * d, e_, d, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float act, slope;
+      rn_act(A.gate_act, g[e], act, slope);
+      const float n = fmaf(z[e], ps[e], pb[e]);
+      sum[RN_RES][e] = fmaf(e_[e], act * n, sum[RN_RES][e]);
+      const float da = e_[e] * rs[e];
+      g[e] = da * n * slope;               // dg
+      const float dn = da * act;
+      sum[RN_POST_SCALE][e] = fmaf(dn, z[e], sum[RN_POST_SCALE][e]);
+      sum[RN_POST_BIAS][e] += dn;
+      p[e] = dn * ps[e];
+    }
+    if (A.gate_act != PQN_GATE_NONE) Row::store(A.dg, row * d, g, d, lane);
+    if (A.has_post) Row::normalise_back(p, z, inv_f, A.rms, d, lane, lds);
+    Row::store(A.df, row * d, p, d, lane);
+  }
+  float *out = A.partials + (size_t)blockIdx.x * RN_PARAMS * d;
+#pragma unroll
+  for (int k = 0; k < RN_PARAMS; ++k) {
+    if constexpr (NT == 64) {              // waves 1 .. 3 hand their sums to wave 0
+      __syncthreads();
+      if (wave > 0)
+#pragma unroll
+        for (int e = 0; e < E; ++e) fold[((wave - 1) * E + e) * 64 + lane] = sum[k][e];
+      __syncthreads();
+      if (wave == 0)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          sum[k][e] = ((sum[k][e] + fold[e * 64 + lane]) + fold[(E + e) * 64 + lane]) + fold[(2 * E + e) * 64 + lane];
+    }
+    if (wave == 0)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = Row::col(lane, i);
+        if (c < d)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) out[(size_t)k * d + c + j] = sum[k][i * VW + j];
+      }
+  }
+}
+
+// column sums of the partials: 64 columns x 16 row groups per workgroup, fixed order
+struct rn_param_out {
+  float *p[RN_PARAMS];
+};
+__global__ __launch_bounds__(1024) void rn_param_kernel(const float *__restrict__ partials, int parts, int d, rn_param_out out) {
+  __shared__ float s[16][64];
+  const int k = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+  if (!out.p[k]) return;
+  float a = 0.f;
+  if (c < d)
+    for (int i = r; i < parts; i += 16) a += partials[((size_t)i * RN_PARAMS + k) * d + c];
+  s[r][threadIdx.x & 63] = a;
+  __syncthreads();
+  if (r == 0 && c < d) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) a += s[i][threadIdx.x];
+    out.p[k][c] = a;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Threads per row: a wave while 16 columns per lane hold it (no barrier then), else the smallest workgroup that does.  Vector
+// accesses of 16 B where width, strides and pointers allow them, else one element per lane and access.
+static int rn_threads(int d) { return d <= 64 * RN_MAX ? 64 : d <= 256 * RN_MAX ? 256 : 512; }
+// workgroups of the gradient: enough waves to fill the chip at its register use, few enough that the partial rows stay small
+static int rn_bwd_blocks(long long n, int d) {
+  const int nt = rn_threads(d);
+  const long long want = nt == 64 ? (n + 3) / 4 : n, cap = 512;
+  return (int)(want < cap ? want : cap);
+}
+
+template <typename T, bool BWD>
+static int rn_launch(const rn_args &A, bool vec, hipStream_t st) {
+  constexpr int VW = 16 / (int)sizeof(T);
+  const int nt = rn_threads(A.d);
+  const dim3 grid(BWD ? rn_bwd_blocks(A.n, A.d) : (unsigned)(nt == 64 ? (A.n + 3) / 4 : A.n));
+  const int per = (A.d + nt - 1) / nt;
+#define RN_GO(NT, W, NVV)                                                                                         \
+  do {                                                                                                            \
+    if constexpr (BWD) rn_bwd_kernel<T, NT, W, NVV><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                      \
+    else rn_fwd_kernel<T, NT, W, NVV><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                                    \
+    return pqn_check_launch(BWD ? "pqn_residual_norm_grad" : "pqn_residual_norm");                                \
+  } while (0)
+  if (vec) {
+    if (nt == 64) {
+      if (per <= VW) RN_GO(64, VW, 1);
+      if (per <= 2 * VW) RN_GO(64, VW, 2);
+      RN_GO(64, VW, RN_MAX / VW);
+    }
+    if (nt == 256) {
+      if (per <= 2 * VW) RN_GO(256, VW, 2);
+      RN_GO(256, VW, RN_MAX / VW);
+    }
+    RN_GO(512, VW, RN_MAX / VW);
+  }
+  if (nt == 64) {
+    if (per <= 4) RN_GO(64, 1, 4);
+    RN_GO(64, 1, RN_MAX);
+  }
+  if (nt == 256) RN_GO(256, 1, RN_MAX);
+  RN_GO(512, 1, RN_MAX);
+#undef RN_GO
+}
+
+static bool rn_vec_ok(const pqn_residual_norm_t *a, const void *const *ptrs, int np, const int64_t *strides, int ns) {
+  const int es = pqn_dtype_size(a->dtype), vw = 16 / es;
+  if (a->d % vw) return false;
+  for (int i = 0; i < np; ++i)
+    if ((uintptr_t)ptrs[i] & 15) return false;
+  for (int i = 0; i < ns; ++i)
+    if (strides[i] % vw) return false;
+  return true;
+}
+
+static int rn_check(const pqn_residual_norm_t *a, const char *who) {
+  PQN_REQUIRE(a, "%s: NULL argument block", who);
+  PQN_REQUIRE(pqn_dtype_known(a->dtype), "%s: unknown dtype %d", who, a->dtype);
+  PQN_REQUIRE(a->n >= 0 && a->d > 0, "%s: n must be >= 0 and d > 0 (n=%lld d=%d)", who, (long long)a->n, a->d);
+  PQN_REQUIRE(a->d <= RN_MAX_D, "%s: rows of up to %d columns (d=%d)", who, RN_MAX_D, a->d);
+  PQN_REQUIRE(a->n <= 0x7fffffffll, "%s: up to 2^31 - 1 rows (n=%lld)", who, (long long)a->n);
+  PQN_REQUIRE(a->norm == PQN_NORM_LAYER || a->norm == PQN_NORM_RMS, "%s: unknown norm %d", who, a->norm);
+  PQN_REQUIRE(a->gate_act == PQN_GATE_NONE || a->gate_act == PQN_GATE_SIGMOID || a->gate_act == PQN_GATE_SILU,
+              "%s: unknown gate activation %d", who, a->gate_act);
+  PQN_REQUIRE(a->eps >= 0.f, "%s: eps must be >= 0", who);
+  PQN_REQUIRE(a->post || (!a->post_scale && !a->post_bias), "%s: post_scale / post_bias without the norm after the block", who);
+  PQN_REQUIRE(a->pre || (!a->pre_scale && !a->pre_bias), "%s: pre_scale / pre_bias without the norm before the next block", who);
+  if (a->n > 0) {
+    PQN_REQUIRE(a->x && a->f, "%s: NULL x or f", who);
+    PQN_REQUIRE((a->gate != nullptr) == (a->gate_act != PQN_GATE_NONE), "%s: gate and gate_act go together", who);
+  }
+  return PQN_OK;
+}
+
+static rn_args rn_fill(const pqn_residual_norm_t *a) {
+  rn_args A = {};
+  A.n = a->n; A.d = a->d; A.rms = a->norm == PQN_NORM_RMS; A.gate_act = a->gate_act;
+  A.has_post = a->post; A.has_pre = a->pre; A.eps = a->eps;
+  A.x = a->x; A.f = a->f; A.g = a->gate; A.xs = a->x_stride; A.fs = a->f_stride; A.gs = a->gate_stride;
+  A.res_scale = a->res_scale; A.post_scale = a->post_scale; A.post_bias = a->post_bias;
+  A.pre_scale = a->pre_scale; A.pre_bias = a->pre_bias;
+  A.y = a->y; A.h = a->h;
+  A.dy = a->dy; A.dh = a->dh; A.dys = a->dy_stride; A.dhs = a->dh_stride;
+  A.dx = a->dx; A.df = a->df; A.dg = a->dgate;
+  A.partials = a->workspace;
+  return A;
+}
+
+extern "C" int pqn_residual_norm(const pqn_residual_norm_t *a, void *stream) {
+  const int rc = rn_check(a, "pqn_residual_norm");
+  if (rc != PQN_OK) return rc;
+  if (a->n == 0) return PQN_OK;
+  PQN_REQUIRE(a->y && (a->h != nullptr) == (a->pre != 0), "pqn_residual_norm: y is an output, and h is one exactly where pre is set");
+  const void *ptrs[] = {a->x, a->f, a->gate, a->y, a->h};
+  const int64_t strides[] = {a->x_stride, a->f_stride, a->gate ? a->gate_stride : 0};
+  const bool vec = rn_vec_ok(a, ptrs, 5, strides, 3);
+  return pqn_with_dtype(a->dtype, [&](auto t) { return rn_launch<decltype(t), false>(rn_fill(a), vec, (hipStream_t)stream); });
+}
+
+extern "C" int64_t pqn_residual_norm_workspace_floats(int64_t n, int32_t d) {
+  if (n <= 0 || d <= 0 || d > RN_MAX_D) return 0;
+  return (int64_t)rn_bwd_blocks(n, d) * RN_PARAMS * d;
+}
+
+extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream) {
+  const int rc = rn_check(a, "pqn_residual_norm_grad");
+  if (rc != PQN_OK) return rc;
+  rn_param_out out = {{a->dres_scale, a->dpost_scale, a->dpost_bias, a->dpre_scale, a->dpre_bias}};
+  bool any = false;
+  for (int k = 0; k < RN_PARAMS; ++k) any = any || out.p[k];
+  if (a->n > 0) {
+    PQN_REQUIRE(a->dx && a->df && (a->dgate != nullptr) == (a->gate != nullptr), "pqn_residual_norm_grad: dx, df (and dgate with a gate) are outputs");
+    PQN_REQUIRE(a->workspace, "pqn_residual_norm_grad: NULL workspace");
+    PQN_REQUIRE(a->dy || a->dh, "pqn_residual_norm_grad: dy and dh are both NULL");
+    PQN_REQUIRE(!a->dh || a->pre, "pqn_residual_norm_grad: dh without the norm before the next block");
+    const void *ptrs[] = {a->x, a->f, a->gate, a->dy, a->dh, a->dx, a->df, a->dgate};
+    const int64_t strides[] = {a->x_stride, a->f_stride, a->gate ? a->gate_stride : 0, a->dy ? a->dy_stride : 0, a->dh ? a->dh_stride : 0};
+    const bool vec = rn_vec_ok(a, ptrs, 8, strides, 5);
+    const int r = pqn_with_dtype(a->dtype, [&](auto t) { return rn_launch<decltype(t), true>(rn_fill(a), vec, (hipStream_t)stream); });
+    if (r != PQN_OK) return r;
+  }
+  if (!any) return PQN_OK;
+  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_bwd_blocks(a->n, a->d) : 0,
+                                                                                      a->d, out);
+  return pqn_check_launch("pqn_residual_norm_grad");
+}

@@ -1,0 +1,47 @@
+// pqn_vec.h -- typed loads and stores and wave reductions shared by the operators on f32 / bf16 / f16 tensors
+// (pqn_attn.hip, pqn_resnorm.hip, pqn_logprob.hip).  Arithmetic is f32; a 16-bit value is rounded once, to nearest even, when stored.
+#pragma once
+#include "pqn_common.h"
+
+typedef __bf16 pqn_bf16;
+typedef _Float16 pqn_f16;
+
+PQN_D float pqn_to_f32(float x) { return x; }
+PQN_D float pqn_to_f32(pqn_bf16 x) { return (float)x; }
+PQN_D float pqn_to_f32(pqn_f16 x) { return (float)x; }
+
+// W consecutive elements in one access (the caller has checked the alignment of W * sizeof(T) bytes)
+template <typename T, int W>
+struct pqn_pack {
+  T v[W];
+} __attribute__((aligned(W * sizeof(T) > 16 ? 16 : W * sizeof(T))));
+
+template <typename T, int W>
+PQN_D void pqn_load(float *dst, const T *src) {
+  const pqn_pack<T, W> p = *(const pqn_pack<T, W> *)src;
+#pragma unroll
+  for (int i = 0; i < W; ++i) dst[i] = pqn_to_f32(p.v[i]);
+}
+template <typename T, int W>
+PQN_D void pqn_store(T *dst, const float *src) {
+  pqn_pack<T, W> p;
+#pragma unroll
+  for (int i = 0; i < W; ++i) p.v[i] = (T)src[i];
+  *(pqn_pack<T, W> *)dst = p;
+}
+
+// sum over the lanes of an aligned group of G lanes (G a power of two), the same in every lane
+template <int G = 64>
+PQN_D float pqn_group_sum(float x) {
+#pragma unroll
+  for (int d = G / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+
+inline int pqn_dtype_size(int dtype) { return dtype == PQN_DTYPE_F32 ? 4 : 2; }
+inline bool pqn_dtype_known(int dtype) { return dtype == PQN_DTYPE_F32 || dtype == PQN_DTYPE_BF16 || dtype == PQN_DTYPE_F16; }
+// f(T{}) with the element type of `dtype` (checked before)
+template <typename F>
+inline auto pqn_with_dtype(int dtype, F f) {
+  return dtype == PQN_DTYPE_F32 ? f(float{}) : dtype == PQN_DTYPE_BF16 ? f(pqn_bf16{}) : f(pqn_f16{});
+}
