@@ -659,10 +659,11 @@ enum { PQN_DTYPE_F32 = 0, PQN_DTYPE_BF16 = 1, PQN_DTYPE_F16 = 2 };
  * the step they are given for):
  *   S_t = decay[h] (1 - reset[t][m]) S_{t-1} + k_t v_t^T       o_t = scale S_t^T q_t       per row m and head h, S_{-1} = state_in
  * reset chooses: what it drops may be NaN or uninitialised.  decay in [0, 1] is a constant of the head, as gamma and lambda are of
- * pqn_q_lambda: it has no gradient.  A window of one step is the recurrent form (acting); state_out may equal state_in.
+ * pqn_q_lambda: it has no gradient.  A window of one step is the recurrent form (acting); state_out may equal state_in there, and only there.
  * pqn_decay_attn      reads q, k, v, decay, state_in, reset; writes out, state_out
  * pqn_decay_attn_grad reads those but out / state_out, and dout, dstate_out (the gradient of state_out); writes dq, dk, dv and, where
- *                     wanted, dstate_in.  dstate_in may equal dstate_out.  Bit-identical in every run. */
+ *                     wanted, dstate_in.
+ * Bit-identical in every run.  A NaN or infinity in q, k, v reaches the steps behind it in its episode and no others. */
 #define PQN_ATTN_MAX_D 128
 typedef struct {
   int32_t t_len, m, heads, dk, dv; /* dk, dv <= PQN_ATTN_MAX_D */

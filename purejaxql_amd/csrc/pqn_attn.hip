@@ -11,27 +11,7 @@
 //   d(state that came in) = decay_h (1 - reset_0) R_0
 // so one kernel serves the forward and, over three argument sets in one launch, the gradient; a backward scan is a forward one over
 // negative time strides.
-#include "pqn_vec.h"
-
-struct da_pass {
-  const void *q, *k, *v;
-  void *o;
-  long long qs[3], ks[3], vs[3], os[3];   // strides over (time, row, head) in elements
-  const float *s_in;
-  float *s_out;
-  int s_rs, s_cs;                         // element strides of the state's first (q, k) and second (v, o) index
-  const uint8_t *reset;                   // flag of the border before step i at reset[i * reset_ts + row]
-  long long reset_ts;
-  float o_scale, s_scale;                 // on the outputs; on what a step adds to the state
-  int a, b;                               // width of q, k; width of v, o
-  int late;                               // 0: a border (decay, reset) lies before every step.  1 (backward scans): before every step
-                                          // but the first, and one more behind the last step, before the state goes out
-};
-struct da_args {
-  da_pass pass[3];
-  int t_len, m, heads;
-  const float *decay;
-};
+#include "pqn_attn_chunk.h"
 
 // ---- the recurrence, step by step ------------------------------------------------------------------------------------------
 // A wave owns 32 columns of one (row, head)'s state in registers for the whole scan: 8 lanes x 4 columns across, 8 lane groups down
@@ -125,6 +105,26 @@ __global__ __launch_bounds__(256) void da_recur_kernel(da_args A) {
   }
 }
 
+// the parts' states in order: part p's own, from zero, becomes the state behind it, S_p = decay^len S_{p-1} + own unless it was cut
+__global__ __launch_bounds__(256) void da_join_kernel(da_args A, da_split X, int size) {
+  const long long block = blockIdx.x, per = (size + 1023) / 1024;
+  const long long mh = block / per;
+  const int e = (int)(block % per) * 1024 + threadIdx.x * 4, pass = blockIdx.y;
+  if (e >= size) return;
+  float *p = X.state + pass * X.pass_stride + mh * (X.parts - 1) * (long long)size + e;
+  const int *cut = X.cut + pass * X.cut_stride + mh * (X.parts - 1);
+  const float fade = (float)pqn_powi((double)A.decay[mh % A.heads], X.len);
+  f32x4_t s = *(const f32x4_t *)p;
+  for (int i = 1; i < X.parts - 1; ++i) {
+    const f32x4_t own = *(const f32x4_t *)(p + (long long)i * size);
+    if (cut[i]) s = own;
+    else
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = fmaf(s[j], fade, own[j]);
+    *(f32x4_t *)(p + (long long)i * size) = s;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------
 template <typename T>
 static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
@@ -148,6 +148,64 @@ static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
   if (amax <= 64) DA_GO(8);
   DA_GO(16);
 #undef DA_GO
+}
+
+// One step at a time up to this length, chunks beyond.
+static constexpr int DA_RECUR_MAX = 4;
+// The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
+// reading of k and v and a state written and read), as many as make DA_FILL waves.
+static constexpr int DA_MIN_PART = 256, DA_FILL = 2048;
+
+static da_split da_cut(int t_len, long long rows, int passes, int a, int b) {
+  da_split X = {};
+  const long long waves = rows * passes * da_nw(a, b);
+  long long want = (DA_FILL + waves - 1) / (waves > 0 ? waves : 1);
+  const long long most = t_len / DA_MIN_PART;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  X.len = (int)(((t_len + want - 1) / want + 63) / 64 * 64);      // whole chunks
+  X.parts = X.len > 0 ? (t_len + X.len - 1) / X.len : 1;
+  if (X.parts < 1) X.parts = 1;
+  return X;
+}
+// workspace of one launch of `passes` scans: the parts' states, then their cut flags
+static long long da_state_floats(const da_split &X, long long rows, int a, int b) {
+  return rows * (X.parts - 1) * (long long)(da_ap(a) * 32 * da_nw(a, b));
+}
+static long long da_ws_bytes(const da_split &X, long long rows, int passes, int a, int b) {
+  if (X.parts <= 1) return 0;
+  return passes * (da_state_floats(X, rows, a, b) * 4 + (rows * (X.parts - 1) * 4 + 15) / 16 * 16);
+}
+
+// passes of equal widths, chunked, in one launch each of: the parts' states, their join, the scan
+static int da_run_chunks(da_args &A, int passes, int dtype, void *workspace, hipStream_t st) {
+  const long long rows = (long long)A.m * A.heads;
+  const int a = A.pass[0].a, b = A.pass[0].b, ev = 16 / pqn_dtype_size(dtype);
+  da_split X = da_cut(A.t_len, rows, passes, a, b);
+  X.vec = a % ev == 0 && b % ev == 0;
+  for (int p = 0; p < passes; ++p) {
+    const da_pass &P = A.pass[p];
+    X.vec = X.vec && (((uintptr_t)P.q | (uintptr_t)P.k | (uintptr_t)P.v | (uintptr_t)P.o) & 15) == 0;
+    for (int i = 0; i < 3; ++i) X.vec = X.vec && P.qs[i] % ev == 0 && P.ks[i] % ev == 0 && P.vs[i] % ev == 0;
+  }
+  X.pass_stride = da_state_floats(X, rows, a, b);
+  X.cut_stride = (rows * (X.parts - 1) * 4 + 15) / 16 * 4;
+  X.state = (float *)workspace;
+  X.cut = (int *)(X.state + passes * X.pass_stride);
+  auto go = [&](bool state) {
+    return dtype == PQN_DTYPE_F32 ? da_launch_chunk_f32(A, X, passes, state, st) : da_launch_chunk_bf16(A, X, passes, state, st);
+  };
+  if (X.parts > 1) {
+    int rc = go(true);
+    if (rc != PQN_OK) return rc;
+    if (X.parts > 2) {
+      const int size = da_ap(a) * 32 * da_nw(a, b);
+      da_join_kernel<<<dim3((unsigned)(rows * ((size + 1023) / 1024)), passes), 256, 0, st>>>(A, X, size);
+      rc = pqn_check_launch("pqn_decay_attn");
+      if (rc != PQN_OK) return rc;
+    }
+  }
+  return go(false);
 }
 
 static int da_check(const pqn_decay_attn_t *a, const char *who) {
@@ -196,11 +254,23 @@ static da_pass da_make(const pqn_decay_attn_t *a, const void *q, const int64_t *
   return P;
 }
 
+extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
+  if (da_check(a, "pqn_decay_attn_workspace_bytes") != PQN_OK || a->t_len <= DA_RECUR_MAX || a->m == 0) return 0;
+  const long long rows = (long long)a->m * a->heads;
+  auto need = [&](int passes, int wa, int wb) { return da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb), rows, passes, wa, wb); };
+  if (!grad) return need(1, a->dk, a->dv);
+  if (a->dk == a->dv) return need(3, a->dk, a->dv);
+  const long long one = need(2, a->dv, a->dk), two = need(1, a->dk, a->dv);         // one after the other
+  return one > two ? one : two;
+}
+
 extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
   const int rc = da_check(a, "pqn_decay_attn");
   if (rc != PQN_OK) return rc;
   if (a->m == 0 || (a->t_len == 0 && !a->state_out)) return PQN_OK;
   PQN_REQUIRE(a->out || a->t_len == 0, "pqn_decay_attn: NULL out");
+  PQN_REQUIRE(((uintptr_t)a->workspace & 15) == 0, "pqn_decay_attn: the workspace must be 16-byte aligned");
+  PQN_REQUIRE(!a->state_out || a->state_out != a->state_in || a->t_len <= 1, "pqn_decay_attn: in place only for a window of one step");
   da_args A = {};
   A.t_len = a->t_len; A.m = a->m; A.heads = a->heads; A.decay = a->decay;
   da_pass &P = A.pass[0];
@@ -209,6 +279,10 @@ extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
   P.s_out = a->state_out;
   P.s_rs = a->dv;
   P.s_cs = 1;
+  if (a->t_len > DA_RECUR_MAX) {
+    PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 0) == 0, "pqn_decay_attn: NULL workspace");
+    return da_run_chunks(A, 1, a->dtype, a->workspace, (hipStream_t)stream);
+  }
   return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 1, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 1, (hipStream_t)stream);
 }
 
@@ -217,6 +291,8 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   if (rc != PQN_OK) return rc;
   if (a->m == 0 || (a->t_len == 0 && !a->dstate_in)) return PQN_OK;
   PQN_REQUIRE((a->dout && a->dq && a->dk_out && a->dv_out) || a->t_len == 0, "pqn_decay_attn_grad: NULL dout, dq, dk or dv");
+  PQN_REQUIRE(((uintptr_t)a->workspace & 15) == 0, "pqn_decay_attn_grad: the workspace must be 16-byte aligned");
+  PQN_REQUIRE(!a->dstate_in || a->dstate_in != a->dstate_out, "pqn_decay_attn_grad: dstate_in must not be dstate_out");
   da_args A = {};
   A.t_len = a->t_len; A.m = a->m; A.heads = a->heads; A.decay = a->decay;
   da_pass &Q = A.pass[0], &K = A.pass[1], &V = A.pass[2];
@@ -233,11 +309,13 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   V.s_out = a->dstate_in;
   V.s_rs = a->dv;
   V.s_cs = 1;
+  if (a->t_len > DA_RECUR_MAX) {
+    PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
+    if (a->dk == a->dv) return da_run_chunks(A, 3, a->dtype, a->workspace, (hipStream_t)stream);
+    int rc = da_run_chunks(A, 2, a->dtype, a->workspace, (hipStream_t)stream);      // dq, dk: states of [dv][dk]
+    if (rc != PQN_OK) return rc;
+    A.pass[0] = A.pass[2];                                                          // dv: [dk][dv]
+    return da_run_chunks(A, 1, a->dtype, a->workspace, (hipStream_t)stream);
+  }
   return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 3, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 3, (hipStream_t)stream);
-}
-
-extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
-  (void)a;
-  (void)grad;
-  return 0;
 }
