@@ -154,11 +154,11 @@ static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
 static constexpr int DA_RECUR_MAX = 4;
 // The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
 // reading of k and v and a state written and read), as many as make DA_FILL waves.
-static constexpr int DA_MIN_PART = 256, DA_FILL = 2048;
+static constexpr int DA_MIN_PART = 64, DA_FILL = 2048;
 
-static da_split da_cut(int t_len, long long rows, int passes, int a, int b) {
+static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int vec) {
   da_split X = {};
-  const long long waves = rows * passes * da_nw(a, b);
+  const long long waves = rows * passes * da_nw(a, b, vec);
   long long want = (DA_FILL + waves - 1) / (waves > 0 ? waves : 1);
   const long long most = t_len / DA_MIN_PART;
   if (want > most) want = most;
@@ -166,29 +166,31 @@ static da_split da_cut(int t_len, long long rows, int passes, int a, int b) {
   X.len = (int)(((t_len + want - 1) / want + 63) / 64 * 64);      // whole chunks
   X.parts = X.len > 0 ? (t_len + X.len - 1) / X.len : 1;
   if (X.parts < 1) X.parts = 1;
+  X.vec = vec;
   return X;
 }
-// workspace of one launch of `passes` scans: the parts' states, then their cut flags
-static long long da_state_floats(const da_split &X, long long rows, int a, int b) {
-  return rows * (X.parts - 1) * (long long)(da_ap(a) * 32 * da_nw(a, b));
+static bool da_vec(const pqn_decay_attn_t *a, int grad) {
+  const int ev = 16 / pqn_dtype_size(a->dtype);
+  uintptr_t at = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (grad ? (uintptr_t)a->dout | (uintptr_t)a->dq | (uintptr_t)a->dk_out | (uintptr_t)a->dv_out : (uintptr_t)a->out);
+  bool vec = a->dk % ev == 0 && a->dv % ev == 0 && (at & 15) == 0;
+  for (int i = 0; i < 3; ++i)
+    vec = vec && a->q_stride[i] % ev == 0 && a->k_stride[i] % ev == 0 && a->v_stride[i] % ev == 0 && (!grad || a->dout_stride[i] % ev == 0);
+  return vec;
 }
+// workspace of one launch of `passes` scans: the parts' states, then their cut flags
+static int da_state_size(const da_split &X, int a, int b) { return da_ap(a, X.vec) * 32 * da_nw(a, b, X.vec); }
 static long long da_ws_bytes(const da_split &X, long long rows, int passes, int a, int b) {
   if (X.parts <= 1) return 0;
-  return passes * (da_state_floats(X, rows, a, b) * 4 + (rows * (X.parts - 1) * 4 + 15) / 16 * 16);
+  return passes * (rows * (X.parts - 1) * 4ll * da_state_size(X, a, b) + (rows * (X.parts - 1) * 4 + 15) / 16 * 16);
 }
 
 // passes of equal widths, chunked, in one launch each of: the parts' states, their join, the scan
-static int da_run_chunks(da_args &A, int passes, int dtype, void *workspace, hipStream_t st) {
+static int da_run_chunks(da_args &A, int passes, int dtype, int vec, void *workspace, hipStream_t st) {
   const long long rows = (long long)A.m * A.heads;
-  const int a = A.pass[0].a, b = A.pass[0].b, ev = 16 / pqn_dtype_size(dtype);
-  da_split X = da_cut(A.t_len, rows, passes, a, b);
-  X.vec = a % ev == 0 && b % ev == 0;
-  for (int p = 0; p < passes; ++p) {
-    const da_pass &P = A.pass[p];
-    X.vec = X.vec && (((uintptr_t)P.q | (uintptr_t)P.k | (uintptr_t)P.v | (uintptr_t)P.o) & 15) == 0;
-    for (int i = 0; i < 3; ++i) X.vec = X.vec && P.qs[i] % ev == 0 && P.ks[i] % ev == 0 && P.vs[i] % ev == 0;
-  }
-  X.pass_stride = da_state_floats(X, rows, a, b);
+  const int a = A.pass[0].a, b = A.pass[0].b;
+  da_split X = da_cut(A.t_len, rows, passes, a, b, vec);
+  const int size = da_state_size(X, a, b);
+  X.pass_stride = rows * (X.parts - 1) * size;
   X.cut_stride = (rows * (X.parts - 1) * 4 + 15) / 16 * 4;
   X.state = (float *)workspace;
   X.cut = (int *)(X.state + passes * X.pass_stride);
@@ -199,7 +201,6 @@ static int da_run_chunks(da_args &A, int passes, int dtype, void *workspace, hip
     int rc = go(true);
     if (rc != PQN_OK) return rc;
     if (X.parts > 2) {
-      const int size = da_ap(a) * 32 * da_nw(a, b);
       da_join_kernel<<<dim3((unsigned)(rows * ((size + 1023) / 1024)), passes), 256, 0, st>>>(A, X, size);
       rc = pqn_check_launch("pqn_decay_attn");
       if (rc != PQN_OK) return rc;
@@ -257,7 +258,8 @@ static da_pass da_make(const pqn_decay_attn_t *a, const void *q, const int64_t *
 extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
   if (da_check(a, "pqn_decay_attn_workspace_bytes") != PQN_OK || a->t_len <= DA_RECUR_MAX || a->m == 0) return 0;
   const long long rows = (long long)a->m * a->heads;
-  auto need = [&](int passes, int wa, int wb) { return da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb), rows, passes, wa, wb); };
+  const int vec = da_vec(a, grad);
+  auto need = [&](int passes, int wa, int wb) { return da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb, vec), rows, passes, wa, wb); };
   if (!grad) return need(1, a->dk, a->dv);
   if (a->dk == a->dv) return need(3, a->dk, a->dv);
   const long long one = need(2, a->dv, a->dk), two = need(1, a->dk, a->dv);         // one after the other
@@ -280,8 +282,9 @@ extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
   P.s_rs = a->dv;
   P.s_cs = 1;
   if (a->t_len > DA_RECUR_MAX) {
+    const int vec = da_vec(a, 0);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 0) == 0, "pqn_decay_attn: NULL workspace");
-    return da_run_chunks(A, 1, a->dtype, a->workspace, (hipStream_t)stream);
+    return da_run_chunks(A, 1, a->dtype, vec, a->workspace, (hipStream_t)stream);
   }
   return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 1, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 1, (hipStream_t)stream);
 }
@@ -310,12 +313,13 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   V.s_rs = a->dv;
   V.s_cs = 1;
   if (a->t_len > DA_RECUR_MAX) {
+    const int vec = da_vec(a, 1);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
-    if (a->dk == a->dv) return da_run_chunks(A, 3, a->dtype, a->workspace, (hipStream_t)stream);
-    int rc = da_run_chunks(A, 2, a->dtype, a->workspace, (hipStream_t)stream);      // dq, dk: states of [dv][dk]
+    if (a->dk == a->dv) return da_run_chunks(A, 3, a->dtype, vec, a->workspace, (hipStream_t)stream);
+    int rc = da_run_chunks(A, 2, a->dtype, vec, a->workspace, (hipStream_t)stream);      // dq, dk: states of [dv][dk]
     if (rc != PQN_OK) return rc;
     A.pass[0] = A.pass[2];                                                          // dv: [dk][dv]
-    return da_run_chunks(A, 1, a->dtype, a->workspace, (hipStream_t)stream);
+    return da_run_chunks(A, 1, a->dtype, vec, a->workspace, (hipStream_t)stream);
   }
   return a->dtype == PQN_DTYPE_F32 ? da_launch_recur<float>(A, 3, (hipStream_t)stream) : da_launch_recur<pqn_bf16>(A, 3, (hipStream_t)stream);
 }

@@ -3,5 +3,5 @@
 #include "pqn_attn_chunk.h"
 
 int da_launch_chunk_bf16(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st) {
-  return da_launch_chunk<pqn_bf16, 64>(A, X, passes, state, st);
+  return da_launch_chunk<pqn_bf16, 32>(A, X, passes, state, st);
 }

@@ -73,15 +73,16 @@ struct DaTile {
     const int lane = threadIdx.x & 63;
     return *(const F *)(m + at(row0 + (lane & 15), col0 + (lane >> 4) * EV));
   }
-  // operand with the column index on the lanes (columns da_col(tile, lane & 15) behind col0), k down the rows from row0
+  // operand with the column index on the lanes (columns da_col(tile, lane & 15) behind col0), k down the rows from row0.  bf16: a
+  // lane's 8 values are rows 4 g + e and 16 + 4 g + e (e < 4), the order in which two 16 x 16 accumulators lie in a lane
   template <typename F>
   PQN_D static F cols(const T *m, int row0, int col0, int tile) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     F f;
     if constexpr (sizeof(T) == 2) {
-      const int c = col0 + 32 * (tile >> 1) + 8 * (i & 3) + 4 * (tile & 1), r = row0 + 8 * g + (i >> 2);
+      const int c = col0 + 32 * (tile >> 1) + 8 * (i & 3) + 4 * (tile & 1), r = row0 + 4 * g + (i >> 2);
       const da_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r, c)));
-      const da_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r + 4, c)));
+      const da_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r + 16, c)));
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       f = __builtin_bit_cast(F, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
@@ -99,42 +100,72 @@ PQN_D f32x4_t da_mfma(f32x4_t a, f32x4_t b, f32x4_t c) {   // k = 4 (lane >> 4) 
   return c;
 }
 
-// rows first + r (r < n) of one (row, head)'s tensor, on their way to a DaTile<T, W> of L rows
-template <typename T, int W, int L, int NTHR>
+// Rows of one (row, head)'s tensor on their way to a DaTile<T, W> of L rows.  load() only requests: every lane reads some row and column
+// that exists, without a branch, so that all requests are in flight together; store() puts zeros into the rows from n on.  Columns
+// from `width` on are never written: the tile starts out as zeros.
+template <typename T, int W, int L, int NTHR, bool VEC>
 struct DaLoad {
-  static constexpr int EV = 16 / (int)sizeof(T), VPR = W / EV, N = L * VPR / NTHR, STEP = NTHR / VPR;
-  static_assert(NTHR % VPR == 0 && L % STEP == 0, "whole rows per pass");
+  static constexpr int EV = 16 / (int)sizeof(T), VPR = W / EV, STEP = NTHR / VPR, N = (L + STEP - 1) / STEP;
+  static_assert(NTHR % VPR == 0, "whole rows per pass");
   u32x4_t r[N];
-  PQN_D void load(const T *p, long long stride, int n, int width, bool vec) {
-    const int row0 = threadIdx.x / VPR, c = (threadIdx.x % VPR) * EV;
+  const T *p;                       // this lane's first row and column of the chunk
+  long long stride;
+  int width;
+  PQN_D static int row0() { return threadIdx.x / VPR; }
+  PQN_D static int col() { return threadIdx.x % VPR * EV; }
+  PQN_D static bool inside(int row) { return L % STEP == 0 || row < L; }
+  PQN_D void start(const T *first, long long stride_, int width_) {
+    stride = stride_;
+    width = width_;
+    p = first + row0() * stride + (col() < width ? col() : 0);
+  }
+  PQN_D void advance(int n) { p += n * stride; }
+  PQN_D void fetch(int i, const T *src) {
+    if constexpr (VEC) r[i] = *(const u32x4_t *)src;
+    else {
+      const int c = col() < width ? col() : 0;
+      pqn_pack<T, EV> v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int row = row0 + i * STEP;
-      r[i] = u32x4_t{0u, 0u, 0u, 0u};
-      if (row < n && c < width) {
-        const T *src = p + row * stride + c;
-        if (vec) r[i] = *(const u32x4_t *)src;
-        else {
-          pqn_pack<T, EV> v;
-#pragma unroll
-          for (int e = 0; e < EV; ++e) v.v[e] = c + e < width ? src[e] : (T)0.f;
-          r[i] = __builtin_bit_cast(u32x4_t, v);
-        }
-      }
+      for (int e = 0; e < EV; ++e) v.v[e] = src[min(c + e, width - 1) - c];
+      r[i] = __builtin_bit_cast(u32x4_t, v);
     }
   }
-  PQN_D void store(T *lds) const {
-    const int row0 = threadIdx.x / VPR, c = (threadIdx.x % VPR) * EV;
+  PQN_D void load(int n) {          // n >= 1
+    if (n == L && L % STEP == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *(u32x4_t *)(lds + DaTile<T, W>::at(row0 + i * STEP, c)) = r[i];
+      for (int i = 0; i < N; ++i) fetch(i, p + i * STEP * stride);
+    } else
+#pragma unroll
+      for (int i = 0; i < N; ++i) fetch(i, p + (min(row0() + i * STEP, n - 1) - row0()) * stride);
+  }
+  PQN_D void store(T *lds, int n) {
+    const int c = col();
+    if (c >= width) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = u32x4_t{0u, 0u, 0u, 0u};          // not_finite() looks at these too
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = row0() + i * STEP;
+      if constexpr (!VEC) {
+        pqn_pack<T, EV> v = __builtin_bit_cast(pqn_pack<T, EV>, r[i]);
+#pragma unroll
+        for (int e = 0; e < EV; ++e) v.v[e] = c + e < width ? v.v[e] : (T)0.f;
+        r[i] = __builtin_bit_cast(u32x4_t, v);
+      }
+      if (n < L && row >= n) r[i] = u32x4_t{0u, 0u, 0u, 0u};
+      if (inside(row)) *(u32x4_t *)(lds + DaTile<T, W>::at(row, c)) = r[i];
+    }
   }
   PQN_D static void zero_behind(T *lds, int n) {
-    const int row0 = threadIdx.x / VPR, c = (threadIdx.x % VPR) * EV;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (row0 + i * STEP >= n) *(u32x4_t *)(lds + DaTile<T, W>::at(row0 + i * STEP, c)) = u32x4_t{0u, 0u, 0u, 0u};
+    for (int i = 0; i < N; ++i) {
+      const int row = row0() + i * STEP;
+      if (row >= n && inside(row)) *(u32x4_t *)(lds + DaTile<T, W>::at(row, col())) = u32x4_t{0u, 0u, 0u, 0u};
+    }
   }
-  PQN_D bool not_finite() const {
+  PQN_D bool not_finite() const {                                          // of what store() has put down
     if constexpr (sizeof(T) == 2) {
       typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
       u16x2 m = {0, 0};
@@ -154,44 +185,65 @@ struct DaLoad {
   }
 };
 
+// two floats to bf16, one instruction; the value of a bf16 pair's halves
+typedef pqn_bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+PQN_D uint32_t da_pair(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), bf16x2_t)); }
+PQN_D float da_low(uint32_t p) { return __uint_as_float(p << 16); }
+PQN_D float da_high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+static constexpr int DA_WAVES = 2;   // waves per SIMD at least
+
 struct da_split {       // the time axis in `parts` parts of `len` steps, one workgroup each; parts = 1: not cut
-  int parts, len, vec;  // vec: every row of every tensor of the launch starts on 16 bytes and is whole 16-byte accesses
+  int parts, len;
+  int vec;              // every row of every tensor of the launch starts on 16 bytes and is whole 16-byte accesses
   float *state;         // [pass][row, head][parts - 1][a_pad * b_pad], in the order of the accumulators: the state behind part p ...
   int *cut;             // ... and whether an episode ends inside it
   long long pass_stride, cut_stride;
 };
 
 // STATE: only what the part adds to the state (its first step onwards from zero, the first part from the state that came in)
-template <typename T, int AP, int NW, int L, bool STATE>
-__global__ __launch_bounds__(64 * NW) void da_chunk_kernel(da_args A, da_split X, int passes) {
-  constexpr int NTHR = 64 * NW, BP = 32 * NW, KB = sizeof(T) == 2 ? 32 : 16, NF = AP / KB, NS = AP / 16, NJ = L / KB, NT = L / 16;
-  typedef typename std::conditional<sizeof(T) == 2, bf16x8_t, f32x4_t>::type F;
+template <typename T, int AP, int NW, int L, bool VEC, bool STATE>
+__global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, da_split X, int passes) {
+  constexpr bool B16 = sizeof(T) == 2;
+  constexpr int NTHR = 64 * NW, BP = 32 * NW, KB = B16 ? 32 : 16, NF = AP / KB, NS = AP / 16, NJ = L / KB, NT = L / 16;
+  constexpr int EV = 16 / (int)sizeof(T), PER = KB / 16, OUT = B16 ? 1 : 2;
+  // The weights between the steps of a chunk: the waves share the tiles out and exchange them through LDS.  A wave alone keeps them in
+  // its registers, where they lie as the next product's operand already.
+  constexpr bool SHARE = NW > 1 && !STATE;
+  typedef typename std::conditional<B16, bf16x8_t, f32x4_t>::type F;
   typedef DaTile<T, AP> TA;
   typedef DaTile<T, BP> TB;
   typedef DaTile<T, L> TP;
-  __shared__ __attribute__((aligned(16))) T Qs[STATE ? 8 : L * TA::LD], Ks[L * TA::LD], Vs[L * TB::LD], Ps[STATE ? 8 : L * TP::LD];
-  __shared__ __attribute__((aligned(16))) float pw[L + 4], wv[L];
+  __shared__ __attribute__((aligned(16))) T Qs[STATE ? 8 : L * TA::LD], Ks[L * TA::LD], Vs[L * TB::LD], Ps[SHARE ? L * TP::LD : 8];
+  __shared__ __attribute__((aligned(16))) float pw[L + 4];
   __shared__ int bad[NW];
   // the passes of one (row, head) meet in one XCD's L2: workgroups go round the 8 XCDs
-  const long long nunits = (long long)A.m * A.heads * (STATE ? X.parts - 1 : X.parts);
+  const int parts = STATE ? X.parts - 1 : X.parts;
+  const long long nunits = (long long)A.m * A.heads * parts;
   const long long block = blockIdx.x, unit = block / (8 * passes) * 8 + block % 8;
   const int pass = (int)(block / 8 % passes);
   if (unit >= nunits) return;
   const da_pass &P = A.pass[pass];
-  const int parts = STATE ? X.parts - 1 : X.parts;
   const long long mh = unit / parts;
   const int part = (int)(unit % parts);
   const int h = (int)(mh % A.heads), row = (int)(mh / A.heads);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, ln = lane & 15;
   const int t_first = part * X.len, t_end = min(A.t_len, t_first + X.len);
-  const double decay = (double)A.decay[h];
-  for (int i = threadIdx.x; i <= L; i += NTHR) pw[i] = (float)pqn_powi(decay, i);   // every power rounded once
-  if constexpr (!STATE)
-    for (int i = threadIdx.x; i < L * TP::LD; i += NTHR) Ps[i] = (T)0.f;             // tiles above the diagonal stay zero
-  const T *qp = (const T *)P.q + row * P.qs[1] + h * P.qs[2];
-  const T *kp = (const T *)P.k + row * P.ks[1] + h * P.ks[2];
-  const T *vp = (const T *)P.v + row * P.vs[1] + h * P.vs[2];
-  T *op = (T *)P.o + row * P.os[1] + h * P.os[2];
+  DaLoad<T, AP, L, NTHR, VEC> rq, rk;
+  DaLoad<T, BP, L, NTHR, VEC> rv;
+  if constexpr (!STATE) rq.start((const T *)P.q + t_first * P.qs[0] + row * P.qs[1] + h * P.qs[2], P.qs[0], P.a);
+  rk.start((const T *)P.k + t_first * P.ks[0] + row * P.ks[1] + h * P.ks[2], P.ks[0], P.a);
+  rv.start((const T *)P.v + t_first * P.vs[0] + row * P.vs[1] + h * P.vs[2], P.vs[0], P.b);
+  int flag = 0;
+  auto fetch = [&](int t) {
+    const int n = min(L, t_end - t);
+    rk.load(n);
+    rv.load(n);
+    if constexpr (!STATE) rq.load(n);
+    if (P.reset) flag = P.reset[max(t + min(lane, n - 1), P.late) * P.reset_ts + row];
+  };
+  if (t_first < t_end) fetch(t_first);
   f32x4_t s[NS][2];
 #pragma unroll
   for (int i = 0; i < NS; ++i)
@@ -217,28 +269,77 @@ __global__ __launch_bounds__(64 * NW) void da_chunk_kernel(da_args A, da_split X
 #pragma unroll
       for (int c = 0; c < 2; ++c) s[i][c] = *(const f32x4_t *)(xs + (long long)(part - 1) * (AP * BP) + (i * 2 + c) * 256);
   }
-  DaLoad<T, AP, L, NTHR> rq, rk;
-  DaLoad<T, BP, L, NTHR> rv;
-  int flag = 0;
-  auto fetch = [&](int t) {
-    const int n = min(L, t_end - t);
-    if constexpr (!STATE) rq.load(qp + t * P.qs[0], P.qs[0], n, P.a, X.vec);
-    rk.load(kp + t * P.ks[0], P.ks[0], n, P.a, X.vec);
-    rv.load(vp + t * P.vs[0], P.vs[0], n, P.b, X.vec);
-    flag = 0;
-    if (P.reset && lane < n && (t + lane > 0 || !P.late)) flag = P.reset[(t + lane) * P.reset_ts + row];
+  const double decay = (double)A.decay[h];
+  for (int i = threadIdx.x; i <= L; i += NTHR) pw[i] = (float)pqn_powi(decay, i);   // every power rounded once
+  if (P.a < AP || P.b < BP) {
+    for (int i = threadIdx.x; i < L * TA::LD; i += NTHR) {
+      if constexpr (!STATE) Qs[i] = (T)0.f;
+      Ks[i] = (T)0.f;
+    }
+    for (int i = threadIdx.x; i < L * TB::LD; i += NTHR) Vs[i] = (T)0.f;
+  }
+  T *op = STATE ? nullptr : (T *)P.o + t_first * P.os[0] + row * P.os[1] + h * P.os[2] + ln * P.os[0] + dv0 + (B16 ? 8 : 4) * g;
+  typedef pqn_pack<T, EV> Out;
+  Out held[NT][OUT];                   // a chunk's outputs, step 16 tt + ln: 8 columns from 8 g, or 4 from 16 c + 4 g
+  int n_held = 0;
+  auto write_out = [&]() {
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+      if (16 * tt + ln >= n_held) continue;
+#pragma unroll
+      for (int c = 0; c < OUT; ++c) {
+        T *dst = op + 16 * tt * P.os[0] + 16 * c;
+        const int col = dv0 + (B16 ? 8 * g : 16 * c + 4 * g);
+        if constexpr (VEC) {
+          if (col < P.b) *(pqn_pack<T, EV> *)dst = held[tt][c];
+        } else
+#pragma unroll
+          for (int e = 0; e < EV; ++e)
+            if (col + e < P.b) dst[e] = held[tt][c].v[e];
+      }
+    }
+    op += n_held * P.os[0];
   };
-  if (t_first < t_end) fetch(t_first);
-  bool any_cut = false;
+  // What depends on the decay alone for a whole chunk without an episode's end is made once: the weights between steps, of the state
+  // on the outputs and of the steps on the state behind them.  `usual` says that they are those.
+  float wt[NT][NT][4], wc[NT], wu[NJ][EV];
+  bool usual = false, any_cut = false;
+  auto make_weights = [&](int n, unsigned long long cuts, int first) {
+    const int last_cut = cuts ? 63 - __clzll(cuts) : 0;
+    if constexpr (!STATE)
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt) {
+        const int t = 16 * tt + ln;
+        const unsigned long long upto = cuts & ((2ull << t) - 1ull);
+        const int from = upto ? 63 - __clzll(upto) : 0;      // first step of t's episode in this chunk
+        wc[tt] = pw[t + first] * P.o_scale;
+#pragma unroll
+        for (int jt = 0; jt <= tt; ++jt) {
+          if (SHARE && (tt * (tt + 1) / 2 + jt) % NW != wave) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = 16 * jt + 4 * g + e;
+            wt[tt][jt][e] = j <= t && j >= from ? pw[max(t - j, 0)] * (P.s_scale * P.o_scale) : 0.f;
+          }
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const int at = j * KB + 4 * g + (e & 3) + 16 * (e >> 2);
+        wu[j][e] = at < n && at >= last_cut ? pw[max(n - 1 - at, 0)] * P.s_scale : 0.f;
+      }
+  };
+  __syncthreads();                                     // pw
   for (int t0 = t_first; t0 < t_end;) {
     int n = min(L, t_end - t0);
-    __syncthreads();                                   // the chunk before has been read
-    if constexpr (!STATE) rq.store(Qs);
-    rk.store(Ks);
-    rv.store(Vs);
+    rk.store(Ks, n);
+    rv.store(Vs, n);
+    if constexpr (!STATE) rq.store(Qs, n);
     const bool nf = __any(rk.not_finite() || rv.not_finite());
     if (lane == 0) bad[wave] = nf;
-    const unsigned long long cuts_all = __ballot(flag != 0);
+    const unsigned long long cuts_all = __ballot(flag != 0 && lane < n && (t0 + lane > 0 || !P.late));
     __syncthreads();
     int off = 0;
 #pragma unroll
@@ -250,34 +351,52 @@ __global__ __launch_bounds__(64 * NW) void da_chunk_kernel(da_args A, da_split X
       decltype(rv)::zero_behind(Vs, 1);
       __syncthreads();
     }
-    const unsigned long long cuts = cuts_all & (n == 64 ? ~0ull : (1ull << n) - 1ull);
-    if (t0 + n < t_end) fetch(t0 + n);
-    const int first = (t0 == 0 && P.late) ? 0 : 1;     // borders up to and including step 0 of this chunk
-    const int last_cut = cuts ? 63 - __clzll(cuts) : -1;
-    if (wave == 0 && lane < L) wv[lane] = lane < n && lane >= last_cut ? pw[n - 1 - lane] * P.s_scale : 0.f;
-    if constexpr (!STATE) {
-      // P^T tiles on and below the diagonal, dealt to the waves
-#pragma unroll
-      for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-        for (int jt = 0; jt <= tt; ++jt) {
-          if ((tt * (tt + 1) / 2 + jt) % NW != wave || 16 * tt >= n) continue;
-          f32x4_t p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int f = 0; f < NF; ++f) p = da_mfma(TA::template rows<F>(Ks, 16 * jt, f * KB), TA::template rows<F>(Qs, 16 * tt, f * KB), p);
-          const int t = 16 * tt + ln;
-          const unsigned long long upto = cuts & ((2ull << t) - 1ull);
-          const int from = upto ? 63 - __clzll(upto) : 0;      // first step of t's episode in this chunk
-          float o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 16 * jt + 4 * g + e;
-            o[e] = j <= t && j >= from ? p[e] * (pw[max(t - j, 0)] * P.s_scale) : 0.f;
-          }
-          pqn_store<T, 4>(Ps + TP::at(t, 16 * jt + 4 * g), o);
-        }
+    const unsigned long long cuts = cuts_all & ((1ull << n) - 1ull);
+    // Outputs leave one chunk late, in front of the next requests: memory operations end in order, so the wait for a chunk's inputs
+    // would otherwise be one for the stores behind them as well.
+    if constexpr (!STATE) write_out();
+    if (t0 + n < t_end) {
+      rk.advance(n);
+      rv.advance(n);
+      if constexpr (!STATE) rq.advance(n);
+      fetch(t0 + n);
     }
-    __syncthreads();
+    const int first = (t0 == 0 && P.late) ? 0 : 1;     // borders up to and including step 0 of this chunk
+    const bool plain = n == L && !cuts && first;
+    if (!(plain && usual)) make_weights(n, cuts, first);
+    usual = plain;
+    // the weights of steps 16 jt + 4 g + e on step 16 tt + ln
+    auto weights = [&](int tt, int jt, const F (&qf)[NF]) {
+      f32x4_t p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < NF; ++f) p = da_mfma(TA::template rows<F>(Ks, 16 * jt, f * KB), qf[f], p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] *= wt[tt][jt][e];
+      return p;
+    };
+    if constexpr (SHARE) {
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt) {
+        if (16 * tt >= n) continue;
+#pragma unroll
+        for (int jt = 0; jt < (tt / PER + 1) * PER; ++jt) {      // whole operands: with zeros above the diagonal
+          if ((tt * (tt + 1) / 2 + min(jt, tt)) % NW != wave) continue;
+          f32x4_t p = {0.f, 0.f, 0.f, 0.f};
+          if (jt <= tt) {
+            F qf[NF];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Qs, 16 * tt, f * KB);
+            p = weights(tt, jt, qf);
+          }
+          if constexpr (B16) {                                   // in the order of DaTile::cols
+            uint32_t *dst = (uint32_t *)(Ps + TP::at(16 * tt + ln, 32 * (jt >> 1) + 8 * g + 4 * (jt & 1)));
+            dst[0] = da_pair(p[0], p[1]);
+            dst[1] = da_pair(p[2], p[3]);
+          } else *(f32x4_t *)(Ps + TP::at(16 * tt + ln, 16 * jt + 4 * g)) = p;
+        }
+      }
+      __syncthreads();
+    }
     F vf[2][NJ];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -289,108 +408,115 @@ __global__ __launch_bounds__(64 * NW) void da_chunk_kernel(da_args A, da_split X
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sf[f][c][e] = (T)s[2 * f][c][e];
-              sf[f][c][4 + e] = (T)s[2 * f + 1][c][e];
-            }
+          if constexpr (B16) {
+            const f32x4_t a = s[2 * f][c], b = s[2 * f + 1][c];
+            sf[f][c] = __builtin_bit_cast(F, (u32x4_t{da_pair(a[0], a[1]), da_pair(a[2], a[3]), da_pair(b[0], b[1]), da_pair(b[2], b[3])}));
           } else sf[f][c] = s[f][c];
 #pragma unroll
       for (int tt = 0; tt < NT; ++tt) {
         if (16 * tt >= n) continue;
+        F qf[NF];
+#pragma unroll
+        for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Qs, 16 * tt, f * KB);
         f32x4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const F qf = TA::template rows<F>(Qs, 16 * tt, f * KB);
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) o[c] = da_mfma(sf[f][c], qf, o[c]);
+          for (int c = 0; c < 2; ++c) o[c] = da_mfma(sf[f][c], qf[f], o[c]);
+        if (cuts) {                                              // a choice, not a product: the state may be NaN
+          const bool carried = (cuts & ((2ull << (16 * tt + ln)) - 1ull)) == 0;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][e] = carried ? o[c][e] : 0.f;
         }
-        const int t = 16 * tt + ln;
-        const bool carried = (cuts & ((2ull << t) - 1ull)) == 0;
-        const float w = pw[t + first];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][e] = carried ? o[c][e] * w : 0.f;
+          for (int e = 0; e < 4; ++e) o[c][e] *= wc[tt];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if (j * KB >= 16 * (tt + 1)) continue;
-          const F pf = TP::template rows<F>(Ps, 16 * tt, j * KB);
+          F pf;
+          if constexpr (SHARE) pf = TP::template rows<F>(Ps, 16 * tt, j * KB);
+          else if constexpr (B16) {
+            u32x4_t u = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (2 * j + half > tt) continue;
+              const f32x4_t p = weights(tt, 2 * j + half, qf);
+              u[2 * half] = da_pair(p[0], p[1]);
+              u[2 * half + 1] = da_pair(p[2], p[3]);
+            }
+            pf = __builtin_bit_cast(F, u);
+          } else pf = weights(tt, j, qf);
 #pragma unroll
           for (int c = 0; c < 2; ++c) o[c] = da_mfma(vf[c][j], pf, o[c]);
         }
-        if (t < n) {
-          T *dst = op + (t0 + t) * P.os[0];
-          if constexpr (sizeof(T) == 2) {
-            const int col = dv0 + 8 * g;
-            float v8[8];
+        if constexpr (B16)
+          held[tt][0] = __builtin_bit_cast(Out, (u32x4_t{da_pair(o[0][0], o[0][1]), da_pair(o[0][2], o[0][3]),
+                                                                        da_pair(o[1][0], o[1][1]), da_pair(o[1][2], o[1][3])}));
+        else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v8[e] = o[e >> 2][e & 3] * P.o_scale;
-            if (X.vec) {
-              if (col < P.b) pqn_store<T, 8>(dst + col, v8);
-            } else
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (col + e < P.b) dst[col + e] = (T)v8[e];
-          } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = dv0 + 16 * c + 4 * g;
-              float v4[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v4[e] = o[c][e] * P.o_scale;
-              if (X.vec) {
-                if (col < P.b) pqn_store<T, 4>(dst + col, v4);
-              } else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (col + e < P.b) dst[col + e] = (T)v4[e];
-            }
-          }
-        }
+          for (int c = 0; c < OUT; ++c) held[tt][c] = __builtin_bit_cast(Out, o[c]);
       }
+      n_held = n;
     }
     // the state behind the chunk
-    const float fade = cuts ? 0.f : pw[n - 1 + first];
+    const float fade = pw[n - 1 + first];
     any_cut = any_cut || cuts != 0;
+    if (cuts) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) s[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][c][e] = cuts ? 0.f : s[i][c][e] * fade;
-    F lo[2][NJ];
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      constexpr int EV = 16 / (int)sizeof(T);
-      float w[EV];
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int e = 0; e < EV; e += 4) *(f32x4_t *)(w + e) = *(const f32x4_t *)(wv + j * KB + g * EV + e);
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < EV; ++e) {
-          const float x = w[e] == 0.f ? 0.f : pqn_to_f32((T)vf[c][j][e]) * w[e];
-          vf[c][j][e] = (T)x;
-          if constexpr (sizeof(T) == 2) lo[c][j][e] = (T)(x - pqn_to_f32((T)vf[c][j][e]));
-        }
+          for (int e = 0; e < 4; ++e) s[i][c][e] *= fade;
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if (j * KB >= n) continue;
+      constexpr int PIECES = B16 ? 3 : 1;
+      F x[2][PIECES];                                  // w v is its pieces' sum exactly
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if constexpr (B16) {
+          const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[c][j]);
+          u32x4_t u[3];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float lo = da_low(v[e]) * wu[j][2 * e], hi = da_high(v[e]) * wu[j][2 * e + 1];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              u[k][e] = da_pair(lo, hi);
+              lo -= da_low(u[k][e]);
+              hi -= da_high(u[k][e]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) x[c][k] = __builtin_bit_cast(F, u[k]);
+        } else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[c][0][e] = vf[c][j][e] * wu[j][e];
+      }
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const F kf = TA::template cols<F>(Ks, j * KB, 0, i);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          s[i][c] = da_mfma(kf, vf[c][j], s[i][c]);
-          if constexpr (sizeof(T) == 2) s[i][c] = da_mfma(kf, lo[c][j], s[i][c]);
-        }
+        for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) s[i][c] = da_mfma(kf, x[c][k], s[i][c]);
       }
     }
     t0 += n;
+    __syncthreads();                                   // the chunk has been read
   }
+  if constexpr (!STATE) write_out();
   if constexpr (STATE) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
@@ -412,35 +538,36 @@ __global__ __launch_bounds__(64 * NW) void da_chunk_kernel(da_args A, da_split X
   }
 }
 
-
-// widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave
-inline int da_ap(int a) { return a <= 32 ? 32 : a <= 64 ? 64 : 128; }
-inline int da_nw(int a, int b) {
+// widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave.  Tensors whose rows are not whole 16-byte
+// accesses take the widest kernel, whose loads go element by element.
+inline int da_ap(int a, int vec) { return !vec ? 128 : a <= 32 ? 32 : a <= 64 ? 64 : 128; }
+inline int da_nw(int a, int b, int vec) {
   const int nw = b <= 32 ? 1 : b <= 64 ? 2 : 4;
-  return a > 64 && nw < 2 ? 2 : nw;               // a wave alone would hold 128 registers of loads in flight
+  return !vec ? 4 : a > 64 && nw < 2 ? 2 : nw;    // a wave alone would hold 128 registers of loads in flight
 }
 int da_launch_chunk_f32(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st);
 int da_launch_chunk_bf16(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st);
 
 template <typename T, int L>
 static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st) {
-  const int ap = da_ap(A.pass[0].a), nw = da_nw(A.pass[0].a, A.pass[0].b);
+  const int ap = da_ap(A.pass[0].a, X.vec), nw = da_nw(A.pass[0].a, A.pass[0].b, X.vec);
   const long long units = (long long)A.m * A.heads * (state ? X.parts - 1 : X.parts), grid = (units + 7) / 8 * 8 * passes;
   PQN_REQUIRE(grid < (1ll << 31), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
-#define DA_GO(AP, NW)                                                                               \
-  if (ap == AP && nw == NW) {                                                                       \
-    if (state) da_chunk_kernel<T, AP, NW, L, true><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);  \
-    else da_chunk_kernel<T, AP, NW, L, false><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);       \
-    return pqn_check_launch("pqn_decay_attn");                                                      \
+#define DA_GO(AP, NW, VEC)                                                                               \
+  if (ap == AP && nw == NW && (X.vec != 0) == VEC) {                                                     \
+    if (state) da_chunk_kernel<T, AP, NW, L, VEC, true><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);  \
+    else da_chunk_kernel<T, AP, NW, L, VEC, false><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);       \
+    return pqn_check_launch("pqn_decay_attn");                                                           \
   }
-  DA_GO(32, 1)
-  DA_GO(32, 2)
-  DA_GO(32, 4)
-  DA_GO(64, 1)
-  DA_GO(64, 2)
-  DA_GO(64, 4)
-  DA_GO(128, 2)
-  DA_GO(128, 4)
+  DA_GO(32, 1, true)
+  DA_GO(32, 2, true)
+  DA_GO(32, 4, true)
+  DA_GO(64, 1, true)
+  DA_GO(64, 2, true)
+  DA_GO(64, 4, true)
+  DA_GO(128, 2, true)
+  DA_GO(128, 4, true)
+  DA_GO(128, 4, false)
 #undef DA_GO
   pqn_set_error("pqn_decay_attn: no kernel for widths %d, %d", A.pass[0].a, A.pass[0].b);
   return PQN_E_UNSUPPORTED;
