@@ -3,14 +3,16 @@
 //
 //   z = Norm(f)      n = z * post_scale + post_bias      y = x + res_scale * act(g) * n      u = Norm(y)      h = u * pre_scale + pre_bias
 //
-// A row lives in the registers of one wave (up to 1024 columns) or of one workgroup (up to 8192) from its load to its store, so the
-// forward reads x, f, g once and writes y, h once, and the gradient reads x, f, g, dy, dh once and writes dx, df, dg once; both norms'
-// statistics are taken twice over the registers (mean, then the centred sum of squares), in f32.  The gradient recomputes y in f32
-// from x, f, g instead of reading a stored y: the same bytes, and no rounding between the two halves.
+// A row lives in the registers of one wave (up to 512 columns) or of one workgroup from its load to its store, so the forward reads
+// x, f, g once and writes y, h once, and the gradient reads x, f, g, dy, dh once and writes dx, df, dg once; both norms' statistics are
+// taken twice over the registers (mean, then the centred sum of squares), in f32.  The gradient recomputes y in f32 from x, f, g
+// instead of reading a stored y: the same bytes, and no rounding between the two halves.
+//
+// Bound: HBM.  Waves walk over rows with the parameters in registers and the next row's loads in flight; 8 columns per thread keep
+// the gradient's row tensors, parameters and five column sums within the registers of three waves per SIMD.
 #include "pqn_vec.h"
 
-static constexpr int RN_MAX = 16;         // columns per thread: five row tensors and five column sums stay in registers
-static constexpr int RN_MAX_D = 512 * RN_MAX;
+static constexpr int RN_MAX_D = 8192;
 
 struct rn_args {
   long long n;
@@ -28,23 +30,25 @@ struct rn_args {
 };
 enum { RN_RES = 0, RN_POST_SCALE, RN_POST_BIAS, RN_PRE_SCALE, RN_PRE_BIAS, RN_PARAMS };
 
-// sum of NV values at once over the NT threads that hold a row
+// K sums at once over the NT threads that hold a row, the same in every thread.  `turn` alternates between two places in LDS, so
+// that one barrier per sum is enough: a place is written again behind the barrier of the sum in between.
 template <int NT, int K>
-PQN_D void rn_row_sum(float (&v)[K], float *lds) {
+PQN_D void rn_row_sum(float (&v)[K], float *lds, int &turn) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = pqn_group_sum<64>(v[k]);
+  for (int k = 0; k < K; ++k) v[k] = pqn_wave_sum(v[k]);
   if constexpr (NT > 64) {
     constexpr int NW = NT / 64;
-    __syncthreads();                      // the values of the previous sum have been read
+    float *at = lds + turn * 2 * NW;
+    turn ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int k = 0; k < K; ++k) lds[k * NW + (threadIdx.x >> 6)] = v[k];
+      for (int k = 0; k < K; ++k) at[k * NW + (threadIdx.x >> 6)] = v[k];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float s = 0.f;
+      float s = at[k * NW];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) s += lds[k * NW + w];
+      for (int w = 1; w < NW; ++w) s += at[k * NW + w];
       v[k] = s;
     }
   }
@@ -53,17 +57,23 @@ PQN_D void rn_row_sum(float (&v)[K], float *lds) {
 template <typename T, int NT, int VW, int NV>
 struct RnRow {
   static constexpr int E = VW * NV;
+  typedef pqn_pack<T, VW> Pack;
   PQN_D static int col(int lane, int i) { return (i * NT + lane) * VW; }
-  // columns behind d hold zeros, which no sum notices
-  PQN_D static void load(float (&r)[E], const void *base, long long off, int d, int lane) {
+  // requests a row: columns behind d repeat the row's first ones and are put to zero by open()
+  PQN_D static void fetch(Pack (&r)[NV], const void *base, long long off, int d, int lane) {
     const T *p = (const T *)base + off;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(lane, i);
-      if (c < d) pqn_load<T, VW>(r + i * VW, p + c);
-      else
+      r[i] = *(const Pack *)(p + (c < d ? c : 0));
+    }
+  }
+  PQN_D static void open(float (&x)[E], const Pack (&r)[NV], int d, int lane) {
 #pragma unroll
-        for (int j = 0; j < VW; ++j) r[i * VW + j] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const bool in = col(lane, i) < d;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) x[i * VW + j] = in ? pqn_to_f32(r[i].v[j]) : 0.f;
     }
   }
   PQN_D static void store(void *base, long long off, const float (&r)[E], int d, int lane) {
@@ -76,20 +86,23 @@ struct RnRow {
   }
   PQN_D static void param(float (&r)[E], const float *p, float absent, int d, int lane) {
 #pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = absent;
+    if (!p) return;
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(lane, i);
-#pragma unroll
-      for (int j = 0; j < VW; ++j) r[i * VW + j] = (p && c < d) ? p[c + j] : absent;
+      if (c < d) pqn_load<float, VW>(r + i * VW, p + c);
     }
   }
   // r -> (r - mean) * inv in place; returns inv = 1 / sqrt(var + eps).  rms: mean = 0
-  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds) {
+  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds, int &turn) {
+    const float per = 1.0f / (float)d;
     if (!rms) {
       float s[1] = {0.f};
 #pragma unroll
       for (int e = 0; e < E; ++e) s[0] += r[e];
-      rn_row_sum<NT>(s, lds);
-      const float mean = s[0] / (float)d;
+      rn_row_sum<NT>(s, lds, turn);
+      const float mean = s[0] * per;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const bool in = col(lane, i) < d;
@@ -100,165 +113,180 @@ struct RnRow {
     float q[1] = {0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) q[0] = fmaf(r[e], r[e], q[0]);
-    rn_row_sum<NT>(q, lds);
-    const float inv = 1.0f / sqrtf(q[0] / (float)d + eps);
+    rn_row_sum<NT>(q, lds, turn);
+    const float inv = 1.0f / sqrtf(fmaf(q[0], per, eps));
 #pragma unroll
     for (int e = 0; e < E; ++e) r[e] *= inv;
     return inv;
   }
   // gradient of the normalisation: dz -> d(input), z = the normalised row
-  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds) {
+  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds, int &turn) {
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       s[0] = fmaf(dz[e], z[e], s[0]);
       s[1] += dz[e];
     }
-    rn_row_sum<NT>(s, lds);
-    const float a = s[0] / (float)d, b = rms ? 0.f : s[1] / (float)d;
+    rn_row_sum<NT>(s, lds, turn);
+    const float per = 1.0f / (float)d, a = s[0] * per, b = rms ? 0.f : s[1] * per;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool in = col(lane, i) < d;
 #pragma unroll
-      for (int j = 0; j < VW; ++j) dz[i * VW + j] = in ? (dz[i * VW + j] - z[i * VW + j] * a - b) * inv : 0.f;
+      for (int j = 0; j < VW; ++j) dz[i * VW + j] = in ? (fmaf(-z[i * VW + j], a, dz[i * VW + j]) - b) * inv : 0.f;
     }
   }
 };
 
-// act(g) and its slope
+// act(g) and its slope; the sigmoid from v_exp_f32 and v_rcp_f32, each within an ulp
 PQN_D void rn_act(int kind, float g, float &act, float &slope) {
   act = 1.f;
   slope = 0.f;
   if (kind == PQN_GATE_NONE) return;
-  const float s = 1.0f / (1.0f + expf(-g));
+  const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
   if (kind == PQN_GATE_SIGMOID) {
     act = s;
     slope = s * (1.0f - s);
   } else {
     act = g * s;
-    slope = s * (1.0f + g * (1.0f - s));
+    slope = s * fmaf(g, 1.0f - s, 1.0f);
   }
 }
 
-// WPB waves (NT = 64) or one row (NT > 64) per workgroup
-template <typename T, int NT, int VW, int NV>
+// A wave per row (NT = 64, four to a workgroup) or a workgroup per row, walking over the rows.
+template <typename T, int NT, int VW, int NV, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
   using Row = RnRow<T, NT, VW, NV>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
-  __shared__ float lds[2 * 16];
+  constexpr bool KEEP = E <= 8;           // the parameters stay in registers
+  __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63;
   const int d = A.d;
-  const long long row = (long long)blockIdx.x * RPB + (NT > 64 ? 0 : threadIdx.x >> 6);
+  int turn = 0;
+  long long row = (long long)blockIdx.x * RPB + (NT > 64 ? 0 : threadIdx.x >> 6);
+  const long long step = (long long)gridDim.x * RPB;
   if (row >= A.n) return;                 // whole waves / workgroups
-  float z[E], y[E], p[E];
-  Row::load(z, A.f, row * A.fs, d, lane);
-  Row::load(y, A.x, row * A.xs, d, lane);
-  if (A.has_post) {
-    Row::normalise(z, A.rms, A.eps, d, lane, lds);
-    Row::param(p, A.post_scale, 1.f, d, lane);
-#pragma unroll
-    for (int e = 0; e < E; ++e) z[e] *= p[e];
-    if (A.post_bias) {
-      Row::param(p, A.post_bias, 0.f, d, lane);
-#pragma unroll
-      for (int e = 0; e < E; ++e) z[e] += p[e];
-    }
-  }
-  if (A.gate_act != PQN_GATE_NONE) {
-    Row::load(p, A.g, row * A.gs, d, lane);
+  typename Row::Pack fx[NV], ff[NV], fg[NV];
+  auto fetch = [&](long long r) {
+    Row::fetch(ff, A.f, r * A.fs, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) Row::fetch(fg, A.g, r * A.gs, d, lane);
+    Row::fetch(fx, A.x, r * A.xs, d, lane);
+  };
+  fetch(row);
+  float ps[E], pb[E], rs[E], qs[E], qb[E];
+  auto params = [&]() {
+    Row::param(ps, A.post_scale, 1.f, d, lane);
+    Row::param(pb, A.post_bias, 0.f, d, lane);
+    Row::param(rs, A.res_scale, 1.f, d, lane);
+    Row::param(qs, A.pre_scale, 1.f, d, lane);
+    Row::param(qb, A.pre_bias, 0.f, d, lane);
+  };
+  if constexpr (KEEP) params();
+  for (; row < A.n; row += step) {
+    float z[E], y[E], g[E];
+    Row::open(z, ff, d, lane);
+    Row::open(y, fx, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
+    if (row + step < A.n) fetch(row + step);
+    if constexpr (!KEEP) params();
+    if (A.has_post) Row::normalise(z, A.rms, A.eps, d, lane, lds, turn);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float act, slope;
-      rn_act(A.gate_act, p[e], act, slope);
-      z[e] *= act;
+      rn_act(ACT, g[e], act, slope);
+      y[e] = fmaf(rs[e], act * fmaf(z[e], ps[e], pb[e]), y[e]);
     }
-  }
-  Row::param(p, A.res_scale, 1.f, d, lane);
+    Row::store(A.y, row * d, y, d, lane);
+    if (A.has_pre) {
+      Row::normalise(y, A.rms, A.eps, d, lane, lds, turn);
 #pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = fmaf(p[e], z[e], y[e]);
-  Row::store(A.y, row * d, y, d, lane);
-  if (A.has_pre) {
-    Row::normalise(y, A.rms, A.eps, d, lane, lds);
-    Row::param(p, A.pre_scale, 1.f, d, lane);
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] *= p[e];
-    if (A.pre_bias) {
-      Row::param(p, A.pre_bias, 0.f, d, lane);
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] += p[e];
+      for (int e = 0; e < E; ++e) y[e] = fmaf(y[e], qs[e], qb[e]);
+      Row::store(A.h, row * d, y, d, lane);
     }
-    Row::store(A.h, row * d, y, d, lane);
   }
 }
 
-// Rows blockIdx, blockIdx + gridDim, ... : the parameter gradients are summed over a thread's rows in registers and leave the
-// workgroup as one partial row per parameter, summed in a fixed order by rn_param_kernel (the same result in every run).
-template <typename T, int NT, int VW, int NV>
+// The parameter gradients are summed over a thread's rows in registers and leave the workgroup as one partial row per parameter,
+// summed in a fixed order by rn_param_kernel (the same result in every run).
+template <typename T, int NT, int VW, int NV, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
   using Row = RnRow<T, NT, VW, NV>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
-  __shared__ float lds[2 * 16];
+  constexpr bool KEEP = E <= 8;
+  __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   __shared__ float fold[NT > 64 ? 1 : 3 * 64 * E];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63, wave = NT > 64 ? 0 : threadIdx.x >> 6;
   const int d = A.d;
+  int turn = 0;
   float sum[RN_PARAMS][E];
 #pragma unroll
   for (int k = 0; k < RN_PARAMS; ++k)
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[k][e] = 0.f;
-  for (long long row = (long long)blockIdx.x * RPB + wave; row < A.n; row += (long long)gridDim.x * RPB) {
-    float z[E], y[E], e_[E], p[E], g[E];
-    Row::load(z, A.f, row * A.fs, d, lane);
-    Row::load(y, A.x, row * A.xs, d, lane);
-    if (A.gate_act != PQN_GATE_NONE) Row::load(g, A.g, row * A.gs, d, lane);
-    if (A.dy) Row::load(e_, A.dy, row * A.dys, d, lane);
-    else
-#pragma unroll
-      for (int e = 0; e < E; ++e) e_[e] = 0.f;
-    float inv_f = 1.f;
-    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds);
-    float ps[E], pb[E], rs[E];
+  long long row = (long long)blockIdx.x * RPB + wave;
+  const long long step = (long long)gridDim.x * RPB;
+  typename Row::Pack fx[NV], ff[NV], fg[NV], fy[NV], fh[NV];
+  auto fetch = [&](long long r) {
+    Row::fetch(ff, A.f, r * A.fs, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) Row::fetch(fg, A.g, r * A.gs, d, lane);
+    Row::fetch(fx, A.x, r * A.xs, d, lane);
+    if (A.dh) Row::fetch(fh, A.dh, r * A.dhs, d, lane);
+    if (A.dy) Row::fetch(fy, A.dy, r * A.dys, d, lane);
+  };
+  if (row < A.n) fetch(row);
+  float ps[E], pb[E], rs[E], qs[E];
+  auto params = [&]() {
     Row::param(ps, A.post_scale, 1.f, d, lane);
     Row::param(pb, A.post_bias, 0.f, d, lane);
     Row::param(rs, A.res_scale, 1.f, d, lane);
+    Row::param(qs, A.pre_scale, 1.f, d, lane);
+  };
+  if constexpr (KEEP) params();
+  for (; row < A.n; row += step) {
+    float z[E], y[E], e_[E], g[E], dh[E];
+    Row::open(z, ff, d, lane);
+    Row::open(y, fx, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
+    if (A.dh) Row::open(dh, fh, d, lane);
+    if (A.dy) Row::open(e_, fy, d, lane);
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) e_[e] = 0.f;
+    if (row + step < A.n) fetch(row + step);
+    if constexpr (!KEEP) params();
+    float inv_f = 1.f, act[E], slope[E];
+    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds, turn);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float act, slope;
-      rn_act(A.gate_act, g[e], act, slope);
-      y[e] = fmaf(rs[e], act * fmaf(z[e], ps[e], pb[e]), y[e]);
+      rn_act(ACT, g[e], act[e], slope[e]);
+      y[e] = fmaf(rs[e], act[e] * fmaf(z[e], ps[e], pb[e]), y[e]);
     }
     if (A.dh) {
-      float dh[E];
-      Row::load(dh, A.dh, row * A.dhs, d, lane);
-      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds);
-      Row::param(p, A.pre_scale, 1.f, d, lane);
+      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds, turn);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         sum[RN_PRE_SCALE][e] = fmaf(dh[e], y[e], sum[RN_PRE_SCALE][e]);
         sum[RN_PRE_BIAS][e] += dh[e];
-        dh[e] *= p[e];
+        dh[e] *= qs[e];
       }
-      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds);
+      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds, turn);
 #pragma unroll
       for (int e = 0; e < E; ++e) e_[e] += dh[e];
     }
     Row::store(A.dx, row * d, e_, d, lane);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float act, slope;
-      rn_act(A.gate_act, g[e], act, slope);
       const float n = fmaf(z[e], ps[e], pb[e]);
-      sum[RN_RES][e] = fmaf(e_[e], act * n, sum[RN_RES][e]);
-      const float da = e_[e] * rs[e];
-      g[e] = da * n * slope;               // dg
-      const float dn = da * act;
+      sum[RN_RES][e] = fmaf(e_[e], act[e] * n, sum[RN_RES][e]);
+      const float da = e_[e] * rs[e], dn = da * act[e];
+      if constexpr (ACT != PQN_GATE_NONE) g[e] = da * n * slope[e];
       sum[RN_POST_SCALE][e] = fmaf(dn, z[e], sum[RN_POST_SCALE][e]);
       sum[RN_POST_BIAS][e] += dn;
-      p[e] = dn * ps[e];
+      e_[e] = dn * ps[e];
     }
-    if (A.gate_act != PQN_GATE_NONE) Row::store(A.dg, row * d, g, d, lane);
-    if (A.has_post) Row::normalise_back(p, z, inv_f, A.rms, d, lane, lds);
-    Row::store(A.df, row * d, p, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) Row::store(A.dg, row * d, g, d, lane);
+    if (A.has_post) Row::normalise_back(e_, z, inv_f, A.rms, d, lane, lds, turn);
+    Row::store(A.df, row * d, e_, d, lane);
   }
   float *out = A.partials + (size_t)blockIdx.x * RN_PARAMS * d;
 #pragma unroll
@@ -278,9 +306,7 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = Row::col(lane, i);
-        if (c < d)
-#pragma unroll
-          for (int j = 0; j < VW; ++j) out[(size_t)k * d + c + j] = sum[k][i * VW + j];
+        if (c < d) pqn_store<float, VW>(out + (size_t)k * d + c, sum[k] + i * VW);
       }
   }
 }
@@ -306,54 +332,60 @@ __global__ __launch_bounds__(1024) void rn_param_kernel(const float *__restrict_
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// Threads per row: a wave while 16 columns per lane hold it (no barrier then), else the smallest workgroup that does.  Vector
-// accesses of 16 B where width, strides and pointers allow them, else one element per lane and access.
-static int rn_threads(int d) { return d <= 64 * RN_MAX ? 64 : d <= 256 * RN_MAX ? 256 : 512; }
-// workgroups of the gradient: enough waves to fill the chip at its register use, few enough that the partial rows stay small
-static int rn_bwd_blocks(long long n, int d) {
+// Threads per row: as few as hold it at 8 columns each -- a wave up to 512 columns (no barrier then), then 128 to 512 threads, which
+// hold the widest rows at 16 columns each.  Vector accesses of up to 16 B where width, strides and pointers allow them, else one
+// element per lane and access.
+static int rn_threads(int d) { return d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : 512; }
+// Workgroups: enough to fill the chip (8 waves per SIMD asked for by the forward, 2 by the gradient with its sums in registers), each
+// walking over its rows; the gradient leaves a partial row per workgroup and parameter.
+static int rn_blocks(long long n, int d, bool grad) {
   const int nt = rn_threads(d);
-  const long long want = nt == 64 ? (n + 3) / 4 : n, cap = 512;
+  const long long want = nt == 64 ? (n + 3) / 4 : n, cap = grad ? (nt <= 128 ? 1024 : 512) : 65536 / (nt == 64 ? 256 : nt) * 8;
   return (int)(want < cap ? want : cap);
 }
 
-template <typename T, bool BWD>
-static int rn_launch(const rn_args &A, bool vec, hipStream_t st) {
+template <typename T, bool BWD, int ACT>
+static int rn_launch_act(const rn_args &A, bool vec, hipStream_t st) {
   constexpr int VW = 16 / (int)sizeof(T);
   const int nt = rn_threads(A.d);
-  const dim3 grid(BWD ? rn_bwd_blocks(A.n, A.d) : (unsigned)(nt == 64 ? (A.n + 3) / 4 : A.n));
-  const int per = (A.d + nt - 1) / nt;
+  const unsigned grid = rn_blocks(A.n, A.d, BWD);
 #define RN_GO(NT, W, NVV)                                                                                         \
   do {                                                                                                            \
-    if constexpr (BWD) rn_bwd_kernel<T, NT, W, NVV><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                      \
-    else rn_fwd_kernel<T, NT, W, NVV><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                                    \
+    if constexpr (BWD) rn_bwd_kernel<T, NT, W, NVV, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                 \
+    else rn_fwd_kernel<T, NT, W, NVV, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                               \
     return pqn_check_launch(BWD ? "pqn_residual_norm_grad" : "pqn_residual_norm");                                \
   } while (0)
   if (vec) {
-    if (nt == 64) {
-      if (per <= VW) RN_GO(64, VW, 1);
-      if (per <= 2 * VW) RN_GO(64, VW, 2);
-      RN_GO(64, VW, RN_MAX / VW);
-    }
-    if (nt == 256) {
-      if (per <= 2 * VW) RN_GO(256, VW, 2);
-      RN_GO(256, VW, RN_MAX / VW);
-    }
-    RN_GO(512, VW, RN_MAX / VW);
+    if (A.d <= 128) RN_GO(64, 2, 1);
+    if (A.d <= 256) RN_GO(64, 4, 1);
+    if (nt == 64) RN_GO(64, VW, 8 / VW);
+    if (nt == 128) RN_GO(128, VW, 8 / VW);
+    if (nt == 256) RN_GO(256, VW, 8 / VW);
+    if (A.d <= 4096) RN_GO(512, VW, 8 / VW);
+    RN_GO(512, VW, 16 / VW);
   }
-  if (nt == 64) {
-    if (per <= 4) RN_GO(64, 1, 4);
-    RN_GO(64, 1, RN_MAX);
-  }
-  if (nt == 256) RN_GO(256, 1, RN_MAX);
-  RN_GO(512, 1, RN_MAX);
+  if (nt == 64) RN_GO(64, 1, 8);
+  if (nt <= 256) RN_GO(256, 1, 8);
+  if (A.d <= 4096) RN_GO(512, 1, 8);
+  RN_GO(512, 1, 16);
 #undef RN_GO
 }
+template <typename T, bool BWD>
+static int rn_launch(const rn_args &A, bool vec, hipStream_t st) {
+  if (A.gate_act == PQN_GATE_SILU) return rn_launch_act<T, BWD, PQN_GATE_SILU>(A, vec, st);
+  if (A.gate_act == PQN_GATE_SIGMOID) return rn_launch_act<T, BWD, PQN_GATE_SIGMOID>(A, vec, st);
+  return rn_launch_act<T, BWD, PQN_GATE_NONE>(A, vec, st);
+}
 
+// 16-byte accesses: whole rows of them, all starting on 16 bytes (parameters too)
 static bool rn_vec_ok(const pqn_residual_norm_t *a, const void *const *ptrs, int np, const int64_t *strides, int ns) {
   const int es = pqn_dtype_size(a->dtype), vw = 16 / es;
   if (a->d % vw) return false;
   for (int i = 0; i < np; ++i)
     if ((uintptr_t)ptrs[i] & 15) return false;
+  const void *params[] = {a->res_scale, a->post_scale, a->post_bias, a->pre_scale, a->pre_bias, a->workspace};
+  for (const void *p : params)
+    if ((uintptr_t)p & 15) return false;
   for (int i = 0; i < ns; ++i)
     if (strides[i] % vw) return false;
   return true;
@@ -405,7 +437,7 @@ extern "C" int pqn_residual_norm(const pqn_residual_norm_t *a, void *stream) {
 
 extern "C" int64_t pqn_residual_norm_workspace_floats(int64_t n, int32_t d) {
   if (n <= 0 || d <= 0 || d > RN_MAX_D) return 0;
-  return (int64_t)rn_bwd_blocks(n, d) * RN_PARAMS * d;
+  return (int64_t)rn_blocks(n, d, true) * RN_PARAMS * d;
 }
 
 extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream) {
@@ -426,7 +458,7 @@ extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream
     if (r != PQN_OK) return r;
   }
   if (!any) return PQN_OK;
-  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_bwd_blocks(a->n, a->d) : 0,
+  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_blocks(a->n, a->d, true) : 0,
                                                                                       a->d, out);
   return pqn_check_launch("pqn_residual_norm_grad");
 }
