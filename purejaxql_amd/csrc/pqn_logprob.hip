@@ -4,9 +4,12 @@
 //   x_j = logit_j / temperature where allowed      lse = log sum e^x      logp = x_a - lse      H = -sum p log p = lse - sum p x
 //
 // One pass over the logits: every lane keeps the running maximum m of what it has seen, s = sum e^(x - m) and t = sum (x - m) e^(x - m),
-// so H = log s - t / s without a second look (t is shifted like s when m grows: t' = e^(m - m') (t + (m - m') s)).  The K best logits
-// come out of the same pass: a key is the logit's order-preserving bits above the complement of its index, so keys are distinct and
-// ties go to the lowest index whatever the order of the work.
+// so H = log s - t / s without a second look (t is shifted like s when m grows: t' = e^(m - m') (t + (m - m') s)).  Powers of two
+// throughout: x is scaled by log2 e / temperature once and v_exp_f32 taken as it is.  The K best logits come out of the same pass: a key
+// is the logit's order-preserving bits above the complement of its index, so keys are distinct and ties go to the lowest index whatever
+// the order of the work.
+//
+// Bound: HBM for many logits (about 9 vector operations and one v_exp_f32 a logit, below the time its bytes take), latency for few.
 #include "pqn_vec.h"
 
 typedef unsigned long long u64;
@@ -14,7 +17,7 @@ static constexpr int LP_MAX_TOP = PQN_LOGPROB_MAX_TOP;
 
 struct lp_args {
   int n, a, top;
-  float inv_temp;
+  float inv_temp, scale;             // 1 / temperature, log2 e / temperature
   const void *logits;
   long long ls;                      // row stride of the logits in elements
   const uint8_t *mask;
@@ -24,7 +27,7 @@ struct lp_args {
   int32_t *top_action;
   // few rows: a row is cut into `splits` parts of `part` columns, one workgroup each, joined by lp_join_kernel
   int splits, part;
-  float *rec;                        // [n][splits][4 + 2 * LP_MAX_TOP] words: m, s, t, nan | keys
+  float *rec;                        // [n][splits][4 + 2 * LP_MAX_TOP] words: m, s, t, - | keys
 };
 static constexpr int LP_REC = 4 + 2 * LP_MAX_TOP;
 
@@ -45,44 +48,55 @@ PQN_D u64 lp_group_max(u64 k) {
   return k;
 }
 
-// (m, s, t) of a set of values; empty: m = -inf, s = t = 0
+// (m, s, t) of a set of logits: m the largest, s = sum 2^z, t = sum z 2^z with z = (logit - m) log2 e / temperature -- the difference
+// first: a type's lowest value times log2 e is no float.  Empty: m = -inf, s = t = 0.  A NaN or +inf among them leaves s NaN.
 struct LpSum {
   float m, s, t;
 };
-PQN_D LpSum lp_join(const LpSum &a, const LpSum &b) {
-  const float m = a.m > b.m ? a.m : (b.m > a.m ? b.m : a.m);   // equal (both may be infinite): either
-  // a part at -inf holds nothing (s = t = 0); equal maxima need no shift, which also keeps inf - inf out
-  const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
-  const float ea = expf(da), eb = expf(db);
-  LpSum r;
-  r.m = m;
-  r.s = a.s * ea + b.s * eb;
-  r.t = (a.s > 0.f ? ea * (a.t + (ea > 0.f ? da * a.s : 0.f)) : 0.f) + (b.s > 0.f ? eb * (b.t + (eb > 0.f ? db * b.s : 0.f)) : 0.f);
-  return r;
+static constexpr float LP_LOG2E = 1.44269504f, LP_LN2 = 0.693147181f;
+PQN_D float lp_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// the sums seen from a larger maximum; 2^-1000 is 0, and so is its share of t
+PQN_D void lp_shift(LpSum &v, float m, float scale) {
+  const float d = v.m == m ? 0.f : fmaxf((v.m - m) * scale, -1000.f), e = lp_exp2(d);   // equal: no shift, which keeps inf - inf out
+  v.t = e * fmaf(d, v.s, v.t);
+  v.s *= e;
+  v.m = m;
+}
+PQN_D LpSum lp_join(LpSum a, LpSum b, float scale) {
+  const float m = fmaxf(a.m, b.m);
+  lp_shift(a, m, scale);
+  lp_shift(b, m, scale);
+  return {m, a.s + b.s, a.t + b.t};
+}
+// one more logit, none of them above m
+PQN_D void lp_add(LpSum &v, float x, float scale) {
+  const float z = (x - v.m) * scale, q = lp_exp2(z);
+  v.s += q;
+  v.t = fmaf(fmaxf(z, -1000.f), q, v.t);
 }
 template <int G>
-PQN_D LpSum lp_group_join(LpSum v) {
+PQN_D LpSum lp_group_join(LpSum v, float scale) {
 #pragma unroll
   for (int d = G / 2; d > 0; d >>= 1) {
     LpSum o = {__shfl_xor(v.m, d, 64), __shfl_xor(v.s, d, 64), __shfl_xor(v.t, d, 64)};
     // lanes d apart join the same two parts in the same order: bit-identical in every lane
-    v = (threadIdx.x & d) ? lp_join(o, v) : lp_join(v, o);
+    v = (threadIdx.x & d) ? lp_join(o, v, scale) : lp_join(v, o, scale);
   }
   return v;
 }
 
-// what a row's sums say; bad = a NaN or +inf among the allowed logits
+// what a row's sums say
 struct LpRow {
   float lse, entropy;
 };
-PQN_D LpRow lp_row(const LpSum &v, bool bad) {
+PQN_D LpRow lp_row(const LpSum &v, float inv_temp) {
   LpRow r;
-  if (bad) r.lse = r.entropy = NAN;
+  if (v.s != v.s) r.lse = r.entropy = NAN;
   else if (!(v.s > 0.f)) r.lse = -INFINITY, r.entropy = 0.f;          // nothing allowed
   else {
-    const float ls = logf(v.s);
-    r.lse = v.m + ls;
-    r.entropy = fmaxf(ls - v.t / v.s, 0.f);
+    const float l = log2f(v.s);
+    r.lse = fmaf(v.m, inv_temp, LP_LN2 * l);
+    r.entropy = fmaxf(LP_LN2 * (l - v.t / v.s), 0.f);
   }
   return r;
 }
@@ -116,30 +130,22 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(lp_args A) {
   const bool live = row0 < A.n;                    // rows behind the last one shuffle along with a copy of it
   const long long row = live ? row0 : A.n - 1;
   float x[E];
-  bool bad = false;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = e * G + lane;
     x[e] = j < A.a ? lp_logit<T>(A, row, j) : -INFINITY;
-    bad = bad || !(x[e] < INFINITY);
   }
   LpSum v = {-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < E; ++e) v.m = fmaxf(v.m, x[e]);
 #pragma unroll
   for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d, 64));
-  v.m *= A.inv_temp;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float z = x[e] * A.inv_temp - v.m, p = x[e] > -INFINITY ? expf(z) : 0.f;
-    v.s += p;
-    v.t += p > 0.f ? z * p : 0.f;
-  }
-  float nbad = bad ? 1.f : 0.f;
+  for (int e = 0; e < E; ++e)
+    if (!(x[e] == -INFINITY)) lp_add(v, x[e], A.scale);
   v.s = pqn_group_sum<G>(v.s);
   v.t = pqn_group_sum<G>(v.t);
-  nbad = pqn_group_sum<G>(nbad);
-  const LpRow r = lp_row(v, nbad > 0.f);
+  const LpRow r = lp_row(v, A.inv_temp);
   if (live && lane == 0) lp_write_row<T>(A, row, r);
   if (A.top > 0) {
     u64 key[E];
@@ -161,99 +167,125 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(lp_args A) {
 PQN_D void lp_insert(u64 &list, u64 key, int top) {
   const int lane = threadIdx.x & 63;
   const int at = __popcll(__ballot(list > key));               // keys above the new one, all in the first lanes
-  const u64 up = (u64)__shfl_up((long long)list, 1, 64);
-  list = lane < at ? list : lane == at ? key : up;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)list, 0x138, 0xf, 0xf, true);           // wave_shr:1
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(list >> 32), 0x138, 0xf, 0xf, true);
+  list = lane < at ? list : lane == at ? key : ((u64)hi << 32) | lo;
   if (lane >= top) list = 0ull;
 }
+// the wave's best of its lanes' VW logits, by order bits o (0 = none) and index j0 + e, and out of the running with it
+template <int VW>
+PQN_D u64 lp_take(uint32_t (&o)[VW], uint32_t j0) {
+  uint32_t mine = o[0];
+#pragma unroll
+  for (int e = 1; e < VW; ++e) mine = max(mine, o[e]);
+  const uint32_t best = pqn_wave_max(mine);
+  uint32_t at = ~0u;
+#pragma unroll
+  for (int e = VW - 1; e >= 0; --e) at = o[e] == best ? j0 + e : at;
+  at = pqn_wave_min(at);
+#pragma unroll
+  for (int e = 0; e < VW; ++e) o[e] = j0 + e == at ? 0u : o[e];
+  return best ? ((u64)best << 32) | (uint32_t)~at : 0ull;
+}
 
-// A workgroup per row (or part of a row), VW logits per lane and access.  NT threads.
+// A workgroup per row (or part of a row), VW logits per lane and access.  The row's first and last logits that fill no whole access
+// are taken one to a lane.  What an alternative has to beat is the best of the waves' K-th keys, which each wave leaves in LDS for the
+// others: a key below any wave's K-th is none of the row's K best, so reading an older one costs time only.
 template <typename T, int NT, int VW>
 __global__ __launch_bounds__(NT) void lp_long_kernel(lp_args A) {
   constexpr int NW = NT / 64;
   __shared__ u64 keys[NW * LP_MAX_TOP];
   __shared__ float sums[NW][4];
+  __shared__ uint32_t bar[NW];                                  // order bits of the waves' K-th keys
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long row = blockIdx.x / A.splits;
   const int part = blockIdx.x % A.splits;
   const int c0 = part * A.part, c1 = min(A.a, c0 + A.part);
   const T *p = (const T *)A.logits + row * A.ls;
   const uint8_t *mk = A.mask ? A.mask + row * A.ms : nullptr;
+  if (threadIdx.x < NW) bar[threadIdx.x] = 0u;
+  __syncthreads();
   LpSum v = {-INFINITY, 0.f, 0.f};
-  u64 list = 0ull, least = 0ull;                                // least = the list's last key: what a newcomer has to beat
-  float least_x = -INFINITY;
-  bool bad = false;
-  for (int base = c0; base < c1; base += NT * VW) {
-    const int j = base + threadIdx.x * VW;
-    float x[VW];
-    if (j + VW <= c1) pqn_load<T, VW>(x, p + j);
-    else
+  u64 list = 0ull;
+  uint32_t least = 0u;                                          // a newcomer's order bits must not be below
+  auto step = [&](auto &x, int j, int have) {                   // logits j .. of this lane, the first `have` of them real
+    constexpr int W = sizeof(x) / sizeof(float);
+    bool ok[W];                                                 // plain selects: a conditional store behind `have` and the mask was miscompiled
 #pragma unroll
-      for (int e = 0; e < VW; ++e) x[e] = j + e < c1 ? pqn_to_f32(p[j + e]) : -INFINITY;
+    for (int e = 0; e < W; ++e) ok[e] = e < have;
     if (mk)
 #pragma unroll
-      for (int e = 0; e < VW; ++e)
-        if (j + e < c1 && !mk[j + e]) x[e] = -INFINITY;
+      for (int e = 0; e < W; ++e) ok[e] = ok[e] & (mk[min(j + e, c1 - 1)] != 0);
+#pragma unroll
+    for (int e = 0; e < W; ++e) x[e] = ok[e] ? x[e] : -INFINITY;
     float top = x[0];
 #pragma unroll
-    for (int e = 0; e < VW; ++e) {
-      bad = bad || !(x[e] < INFINITY);
-      top = fmaxf(top, x[e]);
-    }
-    const float m = fmaxf(v.m, top * A.inv_temp);
-    if (m > -INFINITY) {
-      const float dm = v.m == m ? 0.f : v.m - m, em = expf(dm);
-      v.t = v.s > 0.f ? em * (v.t + (em > 0.f ? dm * v.s : 0.f)) : 0.f;
-      v.s *= em;
-      v.m = m;
+    for (int e = 1; e < W; ++e) top = fmaxf(top, x[e]);
+    if (__any(top > v.m)) lp_shift(v, fmaxf(v.m, top), A.scale);
+    if (v.m > -INFINITY)
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const float z = x[e] * A.inv_temp - m, q = x[e] > -INFINITY ? expf(z) : 0.f;
-        v.s += q;
-        v.t += q > 0.f ? z * q : 0.f;
+      for (int e = 0; e < W; ++e) lp_add(v, x[e], A.scale);
+    else                                                        // nothing but -inf and NaN so far
+#pragma unroll
+      for (int e = 0; e < W; ++e) v.s += x[e] != x[e] ? NAN : 0.f;
+    if (A.top > 0 && __any(top > -INFINITY && lp_order(top) >= least)) {
+      if constexpr (NW > 1) {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) least = max(least, __hip_atomic_load(&bar[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
       }
-    }
-    if (A.top > 0 && __any(top >= least_x && top > -INFINITY)) {
-      u64 key[VW];
+      uint32_t o[W];
 #pragma unroll
-      for (int e = 0; e < VW; ++e) key[e] = lp_key(x[e], j + e);
+      for (int e = 0; e < W; ++e) o[e] = x[e] > -INFINITY ? lp_order(x[e]) : 0u;
       for (;;) {
-        u64 best = key[0];
-#pragma unroll
-        for (int e = 1; e < VW; ++e) best = lp_max(best, key[e]);
-        best = lp_group_max<64>(best);
-        if (best <= least) break;                                // 0 <= least: ends when nothing is left
+        const u64 best = lp_take(o, (uint32_t)j);
+        const u64 last = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(list >> 32), A.top - 1) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)list, A.top - 1);
+        if (best <= last || (uint32_t)(best >> 32) < least) break;   // 0 <= last: ends when nothing is left
         lp_insert(list, best, A.top);
-        least = (u64)__shfl((long long)list, A.top - 1, 64);
-#pragma unroll
-        for (int e = 0; e < VW; ++e) key[e] = key[e] == best ? 0ull : key[e];
       }
-      least_x = least ? lp_unorder((uint32_t)(least >> 32)) : -INFINITY;
+      const uint32_t last = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(list >> 32), A.top - 1);
+      least = max(least, last);
+      if (NW > 1 && lane == 0) __hip_atomic_store(&bar[wave], last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
+  };
+  int body = c0;
+  if constexpr (VW > 1) {
+    const int head = min(c1 - c0, (int)((16 - ((uintptr_t)(p + c0) & 15)) & 15) / (int)sizeof(T));
+    const int tail = (c1 - c0 - head) % VW;
+    if (wave == 0 && head + tail > 0) {
+      const int j = lane < head ? c0 + lane : c1 - tail + (lane - head);
+      float x[1] = {lane < head + tail ? pqn_to_f32(p[j]) : 0.f};
+      step(x, lane < head + tail ? j : c0, lane < head + tail);
+    }
+    body = c0 + head;
   }
-  v = lp_group_join<64>(v);
-  const bool wbad = __any(bad);
+  const int end = body + (c1 - body) / VW * VW;
+  for (int base = body + wave * 64 * VW; base < end; base += NT * VW) {   // whole waves in, lanes behind the end hold nothing
+    const int j = base + lane * VW;
+    float x[VW];
+#pragma unroll
+    for (int e = 0; e < VW; ++e) x[e] = 0.f;
+    if (j < end) pqn_load<T, VW>(x, p + j);
+    step(x, j < end ? j : body, j < end ? VW : 0);
+  }
+  v = lp_group_join<64>(v, A.scale);
   if (lane == 0) {
     sums[wave][0] = v.m;
     sums[wave][1] = v.s;
     sums[wave][2] = v.t;
-    sums[wave][3] = wbad ? 1.f : 0.f;
   }
   if (lane < A.top) keys[wave * A.top + lane] = list;
   __syncthreads();
   if (wave != 0) return;
   v = {sums[0][0], sums[0][1], sums[0][2]};
-  bool any_bad = sums[0][3] > 0.f;
 #pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    v = lp_join(v, {sums[w][0], sums[w][1], sums[w][2]});
-    any_bad = any_bad || sums[w][3] > 0.f;
-  }
+  for (int w = 1; w < NW; ++w) v = lp_join(v, {sums[w][0], sums[w][1], sums[w][2]}, A.scale);
   // the best of the NW lists
-  u64 mine[(NW * LP_MAX_TOP + 63) / 64];
   constexpr int ML = (NW * LP_MAX_TOP + 63) / 64;
+  u64 mine[ML];
 #pragma unroll
   for (int i = 0; i < ML; ++i) mine[i] = i * 64 + lane < NW * A.top ? keys[i * 64 + lane] : 0ull;
-  const LpRow r = lp_row(v, any_bad);
+  const LpRow r = lp_row(v, A.inv_temp);
   float *rec = A.rec + ((size_t)row * A.splits + part) * LP_REC;
   if (lane == 0) {
     if (A.splits == 1) lp_write_row<T>(A, row, r);
@@ -261,7 +293,6 @@ __global__ __launch_bounds__(NT) void lp_long_kernel(lp_args A) {
       rec[0] = v.m;
       rec[1] = v.s;
       rec[2] = v.t;
-      rec[3] = any_bad ? 1.f : 0.f;
     }
   }
   for (int i = 0; i < A.top; ++i) {
@@ -285,13 +316,9 @@ __global__ __launch_bounds__(64) void lp_join_kernel(lp_args A) {
   const int lane = threadIdx.x;
   const float *rec = A.rec + (size_t)row * A.splits * LP_REC;
   LpSum v = {-INFINITY, 0.f, 0.f};
-  bool bad = false;
-  for (int i = lane; i < A.splits; i += 64) {
-    v = lp_join(v, {rec[i * LP_REC], rec[i * LP_REC + 1], rec[i * LP_REC + 2]});
-    bad = bad || rec[i * LP_REC + 3] > 0.f;
-  }
-  v = lp_group_join<64>(v);
-  const LpRow r = lp_row(v, __any(bad));
+  for (int i = lane; i < A.splits; i += 64) v = lp_join(v, {rec[i * LP_REC], rec[i * LP_REC + 1], rec[i * LP_REC + 2]}, A.scale);
+  v = lp_group_join<64>(v, A.scale);
+  const LpRow r = lp_row(v, A.inv_temp);
   if (lane == 0) lp_write_row<T>(A, row, r);
   u64 floor = ~0ull;                        // keys are distinct: the next best is the largest one below the last
   for (int i = 0; i < A.top; ++i) {
@@ -307,48 +334,87 @@ __global__ __launch_bounds__(64) void lp_join_kernel(lp_args A) {
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
-// d/dx_j = dlogp (1[j = action] - p_j) - dentropy p_j (log p_j + H) + dlse p_j, over the temperature.  Elementwise over the logits:
-// a lane's VW logits in one access, the row's five scalars once per lane.
+// d/dx_j = dlogp (1[j = action] - p_j) - dentropy p_j (log p_j + H) + dlse p_j, over the temperature.
 struct lp_grad_args {
   lp_args A;
   const float *dlogp, *dentropy, *dlse;
   void *dlogits;                     // [n][a]
-  int blocks;                        // workgroups per row
+  int blocks;                        // wide rows: workgroups per row
 };
-template <typename T, int VW>
-__global__ __launch_bounds__(256) void lp_grad_kernel(lp_grad_args G) {
-  const lp_args &A = G.A;
-  long long row;
-  int j;
-  if (G.blocks > 0) {
-    row = blockIdx.x / G.blocks;
-    j = ((int)(blockIdx.x % G.blocks) * 256 + threadIdx.x) * VW;
-    if (j >= A.a) return;
-  } else {                            // narrow rows: a flat index over the whole matrix
-    const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * VW;
-    row = e / A.a;
-    j = (int)(e - row * A.a);
-    if (row >= A.n) return;
+struct LpGrad {                      // a row's scalars
+  float lse, h, dlp, dh, dl, inv_temp;
+  int act;
+  bool none;
+  template <typename T>
+  PQN_D void open(const lp_grad_args &G, long long row) {
+    const lp_args &A = G.A;
+    lse = A.lse[row];
+    none = lse == -INFINITY;
+    h = A.entropy[row];
+    act = A.action[row];
+    dlp = G.dlogp ? G.dlogp[row] : 0.f;
+    dh = G.dentropy ? G.dentropy[row] : 0.f;
+    dl = G.dlse ? G.dlse[row] : 0.f;
+    inv_temp = A.inv_temp;
+    // an id outside the row, or an action that is not allowed, has a constant log probability
+    if (act < 0 || act >= A.a || lp_logit<T>(A, row, act) == -INFINITY) dlp = 0.f;
   }
-  const float lse = A.lse[row], h = A.entropy[row];
-  const int act = A.action[row];
-  float dlp = G.dlogp ? G.dlogp[row] : 0.f;
-  const float dh = G.dentropy ? G.dentropy[row] : 0.f, dl = G.dlse ? G.dlse[row] : 0.f;
-  const T *p = (const T *)A.logits + row * A.ls + j;
-  T *o = (T *)G.dlogits + row * A.a + j;
-  // an id outside the row, or an action that is not allowed, has a constant log probability
-  if (act < 0 || act >= A.a || (A.mask && !A.mask[row * A.ms + act]) ||
-      !(pqn_to_f32(((const T *)A.logits)[row * A.ls + act]) > -INFINITY)) dlp = 0.f;
-  float x[VW], g[VW];
-  pqn_load<T, VW>(x, p);
+  PQN_D float at(float x, int j) const {               // x: the logit, -inf where not allowed
+    const float lp = fmaf(x, inv_temp, -lse), q = lp_exp2(lp * LP_LOG2E);
+    const float c = dl - dlp - dh * (fmaxf(lp, -1000.f) + h);          // q is 0 below
+    const float g = ((act == j ? dlp : 0.f) + q * c) * inv_temp;
+    return x == -INFINITY || none ? 0.f : g;
+  }
+};
+// narrow rows: the lanes as in lp_rows_kernel
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void lp_grad_rows_kernel(lp_grad_args P) {
+  const lp_args &A = P.A;
+  const int lane = threadIdx.x & (G - 1);
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+  if (row >= A.n) return;
+  LpGrad R;
+  R.open<T>(P, row);
+  T *o = (T *)P.dlogits + row * A.a;
 #pragma unroll
-  for (int e = 0; e < VW; ++e) {
-    const bool in = (!A.mask || A.mask[row * A.ms + j + e]) && x[e] != -INFINITY && lse != -INFINITY;
-    const float lp = x[e] * A.inv_temp - lse, q = expf(lp);
-    const float c = dl - dlp - (q > 0.f ? dh * (lp + h) : 0.f);
-    g[e] = in ? ((act == j + e ? dlp : 0.f) + q * c) * A.inv_temp : 0.f;
+  for (int e = 0; e < E; ++e) {
+    const int j = e * G + lane;
+    if (j < A.a) o[j] = (T)R.at(lp_logit<T>(A, row, j), j);
   }
-  pqn_store<T, VW>(o, g);
+}
+// wide rows: `blocks` workgroups to a row, LP_SPAN accesses of VW logits a lane.  Rows whose logits and gradients lie alike on 16
+// bytes take whole accesses, their first and last elements one to a lane.
+static constexpr int LP_SPAN = 4;
+template <typename T, int VW>
+__global__ __launch_bounds__(256) void lp_grad_kernel(lp_grad_args P) {
+  const lp_args &A = P.A;
+  const long long row = blockIdx.x / P.blocks;
+  const int block = blockIdx.x % P.blocks;
+  LpGrad R;
+  R.open<T>(P, row);
+  const T *x = (const T *)A.logits + row * A.ls;
+  const uint8_t *mk = A.mask ? A.mask + row * A.ms : nullptr;
+  T *o = (T *)P.dlogits + row * A.a;
+  int head = 0;
+  if constexpr (VW > 1) {
+    head = min(A.a, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+    const int tail = (A.a - head) % VW;
+    if (block == 0 && (int)threadIdx.x < head + tail) {
+      const int j = (int)threadIdx.x < head ? threadIdx.x : A.a - tail + (threadIdx.x - head);
+      o[j] = (T)R.at(mk && !mk[j] ? -INFINITY : pqn_to_f32(x[j]), j);
+    }
+  }
+  const int end = head + (A.a - head) / VW * VW;
+#pragma unroll
+  for (int i = 0; i < LP_SPAN; ++i) {
+    const int j = head + ((block * LP_SPAN + i) * 256 + (int)threadIdx.x) * VW;
+    if (j >= end) break;
+    float v[VW];
+    pqn_load<T, VW>(v, x + j);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) v[e] = R.at(mk && !mk[j + e] ? -INFINITY : v[e], j + e);
+    pqn_store<T, VW>(o + j, v);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -365,6 +431,7 @@ static int lp_check(const pqn_action_logprobs_t *a, const char *who) {
 static lp_args lp_fill(const pqn_action_logprobs_t *a) {
   lp_args A = {};
   A.n = a->n; A.a = a->a; A.top = a->top; A.inv_temp = 1.0f / a->temperature;
+  A.scale = (float)(1.4426950408889634 / (double)a->temperature);
   A.logits = a->logits; A.ls = a->logits_stride; A.mask = a->mask; A.ms = a->mask_stride;
   A.action = a->action; A.logp = a->logp; A.entropy = a->entropy; A.lse = a->lse;
   A.top_logp = a->top_logp; A.top_action = a->top_action;
@@ -385,36 +452,62 @@ static int lp_splits(int n, int a) {
 // columns per part: whole accesses of 8, so that a part starts as well aligned as its row
 static int lp_part(int a, int splits) { return ((a + splits - 1) / splits + 7) / 8 * 8; }
 
+// the lanes and logits per lane that hold a row of up to LP_ROW_MAX logits
+#define LP_ROW_SHAPES(GO, a) \
+  if (a <= 8) GO(8, 1);      \
+  if (a <= 16) GO(8, 2);     \
+  if (a <= 32) GO(16, 2);    \
+  if (a <= 64) GO(32, 2);    \
+  if (a <= 128) GO(64, 2);   \
+  if (a <= 256) GO(64, 4);   \
+  if (a <= 512) GO(64, 8);   \
+  GO(64, 16);
+
 template <typename T>
 static int lp_launch(lp_args A, hipStream_t st) {
   if (A.a <= LP_ROW_MAX) {
-#define LP_GO(G, E)                                                                       \
-  do {                                                                                    \
+#define LP_GO(G, E)                                                                           \
+  do {                                                                                        \
     lp_rows_kernel<T, G, E><<<(unsigned)(((long long)A.n * G + 255) / 256), 256, 0, st>>>(A); \
-    return pqn_check_launch("pqn_action_logprobs");                                       \
+    return pqn_check_launch("pqn_action_logprobs");                                           \
   } while (0)
-    if (A.a <= 8) LP_GO(8, 1);
-    if (A.a <= 16) LP_GO(8, 2);
-    if (A.a <= 32) LP_GO(16, 2);
-    if (A.a <= 64) LP_GO(32, 2);
-    if (A.a <= 128) LP_GO(64, 2);
-    if (A.a <= 256) LP_GO(64, 4);
-    if (A.a <= 512) LP_GO(64, 8);
-    LP_GO(64, 16);
+    LP_ROW_SHAPES(LP_GO, A.a)
 #undef LP_GO
   }
   A.splits = lp_splits(A.n, A.a);
   A.part = lp_part(A.a, A.splits);
   A.splits = (A.a + A.part - 1) / A.part;
-  constexpr int VW = 16 / (int)sizeof(T);
-  const bool vec = ((uintptr_t)A.logits & 15) == 0 && A.ls % VW == 0;
-  const unsigned grid = (unsigned)((long long)A.n * A.splits);
-  if (vec) lp_long_kernel<T, LP_NT, VW><<<grid, LP_NT, 0, st>>>(A);
-  else lp_long_kernel<T, LP_NT, 1><<<grid, LP_NT, 0, st>>>(A);
+  const long long grid = (long long)A.n * A.splits;
+  PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a);
+  lp_long_kernel<T, LP_NT, 16 / (int)sizeof(T)><<<(unsigned)grid, LP_NT, 0, st>>>(A);
   const int rc = pqn_check_launch("pqn_action_logprobs");
   if (rc != PQN_OK || A.splits == 1) return rc;
   lp_join_kernel<T><<<(unsigned)A.n, 64, 0, st>>>(A);
   return pqn_check_launch("pqn_action_logprobs");
+}
+
+template <typename T>
+static int lp_launch_grad(lp_grad_args P, hipStream_t st) {
+  const lp_args &A = P.A;
+  if (A.a <= LP_ROW_MAX) {
+#define LP_GO(G, E)                                                                                \
+  do {                                                                                             \
+    lp_grad_rows_kernel<T, G, E><<<(unsigned)(((long long)A.n * G + 255) / 256), 256, 0, st>>>(P); \
+    return pqn_check_launch("pqn_action_logprobs_grad");                                           \
+  } while (0)
+    LP_ROW_SHAPES(LP_GO, A.a)
+#undef LP_GO
+  }
+  constexpr int VW = 16 / (int)sizeof(T);
+  // every row's logits and gradients the same way off 16 bytes
+  const bool vec = (((uintptr_t)A.logits - (uintptr_t)P.dlogits) & 15) == 0 && (A.ls - A.a) % VW == 0;
+  const int span = 256 * LP_SPAN * (vec ? VW : 1);
+  P.blocks = (A.a + span - 1) / span;
+  const long long grid = (long long)A.n * P.blocks;
+  PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", A.n, A.a);
+  if (vec) lp_grad_kernel<T, VW><<<(unsigned)grid, 256, 0, st>>>(P);
+  else lp_grad_kernel<T, 1><<<(unsigned)grid, 256, 0, st>>>(P);
+  return pqn_check_launch("pqn_action_logprobs_grad");
 }
 
 extern "C" int64_t pqn_action_logprobs_workspace_bytes(int32_t n, int32_t a) {
@@ -441,17 +534,6 @@ extern "C" int pqn_action_logprobs_grad(const pqn_action_logprobs_t *a, void *st
   PQN_REQUIRE(a->dlogits, "pqn_action_logprobs_grad: NULL dlogits");
   PQN_REQUIRE(a->dlogp || a->dentropy || a->dlse, "pqn_action_logprobs_grad: dlogp, dentropy and dlse are all NULL");
   return pqn_with_dtype(a->dtype, [&](auto t) {
-    typedef decltype(t) T;
-    constexpr int VW = 16 / (int)sizeof(T);
-    lp_grad_args G = {lp_fill(a), a->dlogp, a->dentropy, a->dlse, a->dlogits, 0};
-    // 16-B accesses where the rows keep their alignment; below one workgroup's span of columns the rows are packed end to end
-    const bool vec = a->a % VW == 0 && a->logits_stride % VW == 0 && (((uintptr_t)a->logits | (uintptr_t)a->dlogits) & 15) == 0;
-    const int w = vec ? VW : 1, span = 256 * w;
-    G.blocks = a->a >= span ? (a->a + span - 1) / span : 0;
-    const long long grid = G.blocks ? (long long)a->n * G.blocks : ((long long)a->n * a->a / w + 255) / 256;
-    PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", a->n, a->a);
-    if (vec) lp_grad_kernel<T, VW><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(G);
-    else lp_grad_kernel<T, 1><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(G);
-    return pqn_check_launch("pqn_action_logprobs_grad");
+    return lp_launch_grad<decltype(t)>({lp_fill(a), a->dlogp, a->dentropy, a->dlse, a->dlogits, 0}, (hipStream_t)stream);
   });
 }

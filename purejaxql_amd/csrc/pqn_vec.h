@@ -38,16 +38,23 @@ PQN_D float pqn_group_sum(float x) {
   return x;
 }
 
-// sum over the wave, the same in every lane: four DPP steps within the rows of 16 lanes, two broadcasts across them, lane 63 read back
+// reductions over the wave, the same in every lane: four DPP steps within the rows of 16 lanes (zeros come in from their ends, neutral
+// for the sum and the maximum of unsigned values), two broadcasts across them, lane 63 read back
+#define PQN_WAVE_STEPS(OP)                                                                          \
+  OP(0x111, 0xf, true) OP(0x112, 0xf, true) OP(0x114, 0xf, true) OP(0x118, 0xf, true) OP(0x142, 0xa, false) OP(0x143, 0xc, false)
+PQN_D uint32_t pqn_wave_max(uint32_t x) {
+#define PQN_STEP(ctrl, rows, zero) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, zero));
+  PQN_WAVE_STEPS(PQN_STEP)
+#undef PQN_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
 PQN_D float pqn_wave_sum(float x) {
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x111, 0xf, 0xf, true));   // row_shr:1
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x112, 0xf, 0xf, true));   // row_shr:2
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x114, 0xf, 0xf, true));   // row_shr:4
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x118, 0xf, 0xf, true));   // row_shr:8
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x142, 0xa, 0xf, false));  // row_bcast:15 into rows 1, 3
-  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x143, 0xc, 0xf, false));  // row_bcast:31 into rows 2, 3
+#define PQN_STEP(ctrl, rows, zero) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xf, zero));
+  PQN_WAVE_STEPS(PQN_STEP)
+#undef PQN_STEP
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
+PQN_D uint32_t pqn_wave_min(uint32_t x) { return ~pqn_wave_max(~x); }
 
 inline int pqn_dtype_size(int dtype) { return dtype == PQN_DTYPE_F32 ? 4 : 2; }
 inline bool pqn_dtype_known(int dtype) { return dtype == PQN_DTYPE_F32 || dtype == PQN_DTYPE_BF16 || dtype == PQN_DTYPE_F16; }

@@ -94,15 +94,15 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch
 
 def _last_contiguous(t: torch.Tensor, name: str, shape, dtype, device):
     """A tensor of this shape, type and device whose last index is contiguous; other strides are the caller's."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name}: need {tuple(shape)} of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last index must be contiguous, strides are {tuple(t.stride())}")
 
 
-def _exactly(t: Optional[torch.Tensor], name: str, shape, dtype, device):
-    """A contiguous tensor of this shape, type and device, or None."""
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous()):
+def _exactly(t: torch.Tensor, name: str, shape, dtype, device):
+    """A contiguous tensor of this shape, type and device."""
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: need contiguous {tuple(shape)} of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} on {t.device} "
                          f"contig={t.is_contiguous()}")
 
@@ -112,17 +112,18 @@ def _on_gpu(t: torch.Tensor, name: str, dtypes):
         raise ValueError(f"{name}: need a CUDA tensor of {' / '.join(str(d) for d in dtypes)}, got {t.dtype} on {t.device}")
 
 
-def _flags(t: Optional[torch.Tensor]):
-    return t.view(torch.uint8) if t is not None and t.dtype == torch.bool else t
+def _flags(t: torch.Tensor) -> torch.Tensor:
+    return t.view(torch.uint8) if t.dtype == torch.bool else t
 
 
 def _enqueue(fn, args, device: torch.device, what: str):
     """fn(args, stream) on the tensors' own device and torch's current stream there."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(byref(args), torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(byref(args), torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(byref(args), torch.cuda.current_stream().cuda_stream)
+            rc = fn(byref(args), torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         _lib.check(rc, what)
 
@@ -133,30 +134,28 @@ _ATTN_DTYPES = (torch.float32, torch.bfloat16)
 def _attn_args(a, q, k, v, decay, state, reset, scale, step: bool):
     """Checks the common arguments and fills them into `a`; returns (lead shape, state shape)."""
     _on_gpu(q, "q", _ATTN_DTYPES)
-    lead, dk, dv = tuple(q.shape[:-1]), q.shape[-1], v.shape[-1]
-    if len(lead) != (2 if step else 3):
-        raise ValueError(f"q: need {'[M, H, Dk]' if step else '[T, M, H, Dk]'}, got {tuple(q.shape)}")
-    dt, dev = q.dtype, q.device
+    if q.dim() != (3 if step else 4) or v.dim() != q.dim():
+        raise ValueError(f"q, v: need {'[M, H, D]' if step else '[T, M, H, D]'}, got {tuple(q.shape)}, {tuple(v.shape)}")
+    shape, dt, dev = q.shape, q.dtype, q.device
+    lead, dk, dv = shape[:-1], shape[-1], v.shape[-1]
     if not (0 < dk <= _lib.ATTN_MAX_D and 0 < dv <= _lib.ATTN_MAX_D):
         raise ValueError(f"q, v: head widths of 1 .. {_lib.ATTN_MAX_D}, got {dk} and {dv}")
-    _last_contiguous(q, "q", lead + (dk,), dt, dev)
-    _last_contiguous(k, "k", lead + (dk,), dt, dev)
+    _last_contiguous(q, "q", shape, dt, dev)
+    _last_contiguous(k, "k", shape, dt, dev)
     _last_contiguous(v, "v", lead + (dv,), dt, dev)
     m, h = lead[-2:]
     st = (m, h, dk, dv)
     _exactly(decay, "decay", (h,), torch.float32, dev)
-    _exactly(state, "state", st, torch.float32, dev)
-    reset = _flags(reset)
-    _exactly(reset, "reset", lead[:-1], torch.uint8, dev)
     a.t_len, a.m, a.heads, a.dk, a.dv, a.dtype, a.scale = 1 if step else lead[0], m, h, dk, dv, _DTYPES[dt], scale
     a.q, a.k, a.v, a.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
-    if step:
-        a.q_stride[1:], a.k_stride[1:], a.v_stride[1:] = q.stride()[:2], k.stride()[:2], v.stride()[:2]
-    else:
-        a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    time = (0,) if step else ()      # a step has no time stride
+    a.q_stride, a.k_stride, a.v_stride = time + q.stride()[:-1], time + k.stride()[:-1], time + v.stride()[:-1]
     if state is not None:
+        _exactly(state, "state", st, torch.float32, dev)
         a.state_in = state.data_ptr()
     if reset is not None:
+        reset = _flags(reset)
+        _exactly(reset, "reset", lead[:-1], torch.uint8, dev)
         a.reset = reset.data_ptr()
     return lead, st
 
@@ -214,8 +213,9 @@ def decay_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     a = _lib.DecayAttnArgs()
     lead, st = _attn_args(a, q, k, v, decay, state, reset, scale, False)
     _last_contiguous(dout, "dout", lead + (a.dv,), q.dtype, q.device)
-    _exactly(dstate_out, "dstate_out", st, torch.float32, q.device)
-    a.dout, a.dout_stride[:], a.dstate_out = dout.data_ptr(), dout.stride()[:3], _lib.ptr(dstate_out)
+    if dstate_out is not None:
+        _exactly(dstate_out, "dstate_out", st, torch.float32, q.device)
+    a.dout, a.dout_stride, a.dstate_out = dout.data_ptr(), dout.stride()[:-1], _lib.ptr(dstate_out)
     dq, dk = (torch.empty(lead + (a.dk,), dtype=q.dtype, device=q.device) for _ in range(2))
     dv = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
     dstate = torch.empty(st, dtype=torch.float32, device=q.device) if state is not None else None
@@ -247,7 +247,7 @@ def _norm_args(x, f, gate, gate_act, params, norm_type, post, pre, eps):
         raise ValueError(f"norm_type: one of {sorted(_NORMS)}, gate_act: one of {sorted(_GATES)}; got {norm_type!r}, {gate_act!r}")
     if (gate is None) != (gate_act == "none"):
         raise ValueError("gate and gate_act go together: a gate tensor with 'sigmoid' or 'silu', neither with 'none'")
-    shape, d, dt, dev = tuple(x.shape), x.shape[-1], x.dtype, x.device
+    shape, d, dt, dev = x.shape, x.shape[-1], x.dtype, x.device
     a = _lib.ResidualNormArgs()
     x, a.x_stride = _rows(x, "x", shape, dt, dev)
     f, a.f_stride = _rows(f, "f", shape, dt, dev)
@@ -335,8 +335,8 @@ def _logprob_args(logits, actions, mask, temperature, top):
     a = _lib.ActionLogprobsArgs()
     a.n, a.a, a.top, a.dtype, a.temperature = n, width, top, _DTYPES[logits.dtype], temperature
     a.logits, a.logits_stride, a.action = logits.data_ptr(), logits.stride(0), actions.data_ptr()
-    mask = _flags(mask)
     if mask is not None:
+        mask = _flags(mask)
         _last_contiguous(mask, "mask", (n, width), torch.uint8, dev)
         a.mask, a.mask_stride = mask.data_ptr(), mask.stride(0)
     return a

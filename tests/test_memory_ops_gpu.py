@@ -473,8 +473,10 @@ def _logp_check(x, temperature, top, grad=True):
     w = torch.where(lp > -math.inf, w, torch.zeros_like(w))
     size = (dlp.abs() * (hot + p) + dh.abs() * (plogp.abs() + p * h.abs()) + dl.abs() * p + dh.abs() * p) / temperature
     half = HALF[dt]
-    # f16's subnormal step bounds what a tiny gradient may lose
-    floor = 2.0 ** -25 if dt == F16 else 1e-37
+    # f16's subnormal step bounds what a tiny gradient may lose.  A probability below 2^-126, f32's smallest normal number, counts as 0
+    # (the kernels take 2^x from the hardware, which has no subnormal results): the gradient loses at most p (|dlogp| + |dlse| +
+    # |dentropy| (|log p| + H)) / temperature of it, and p |log p| <= 2^-126 * 126 log 2 below p = 2^-126 (it rises with p up to 1/e).
+    floor = 2.0 ** -25 if dt == F16 else 2.0 ** -126 * (dlp.abs() + dl.abs() + dh.abs() * (126 * math.log(2.0) + h.abs().clamp(max=1e6))) / temperature
     _close(d, w, half * w.abs() + (4 * e * (1 + 0) + 16 * U) * size * (1 + math.log(a) + 2 * big) + floor, "dlogits")
 
 
