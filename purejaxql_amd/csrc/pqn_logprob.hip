@@ -10,6 +10,8 @@
 // the order of the work.
 //
 // Bound: HBM for many logits (about 9 vector operations and one v_exp_f32 a logit, below the time its bytes take), latency for few.
+#include <type_traits>
+
 #include "pqn_vec.h"
 
 typedef unsigned long long u64;
@@ -43,6 +45,10 @@ PQN_D u64 lp_key(float logit, int j) {
 PQN_D u64 lp_max(u64 a, u64 b) { return a > b ? a : b; }
 template <int G>
 PQN_D u64 lp_group_max(u64 k) {
+  if constexpr (G == 64) {               // the whole wave: the upper halves first, the lower ones among their best
+    const uint32_t hi = (uint32_t)(k >> 32), best = pqn_wave_max(hi);
+    return ((u64)best << 32) | pqn_wave_max(hi == best ? (uint32_t)k : 0u);
+  }
 #pragma unroll
   for (int d = G / 2; d > 0; d >>= 1) k = lp_max(k, (u64)__shfl_xor((long long)k, d, 64));
   return k;
@@ -188,54 +194,116 @@ PQN_D u64 lp_take(uint32_t (&o)[VW], uint32_t j0) {
   return best ? ((u64)best << 32) | (uint32_t)~at : 0ull;
 }
 
-// A workgroup per row (or part of a row), VW logits per lane and access.  The row's first and last logits that fill no whole access
-// are taken one to a lane.  What an alternative has to beat is the best of the waves' K-th keys, which each wave leaves in LDS for the
-// others: a key below any wave's K-th is none of the row's K best, so reading an older one costs time only.
-template <typename T, int NT, int VW>
-__global__ __launch_bounds__(NT) void lp_long_kernel(lp_args A) {
-  constexpr int NW = NT / 64;
+// A workgroup per row (or part of a row), which it holds in registers: N accesses of VW logits a thread, all requested at once; the
+// row's first and last logits that fill no whole access one to a thread.  Three looks at the registers: the largest of every access,
+// the sums under the thread's own maximum, and the alternatives.  For those, a bar: the K-th largest of a wave's 64 thread maxima is
+// no larger than the wave's K-th logit, so the largest of the waves' bars sorts out all but a few accesses; what is left goes through
+// the wave's list of K keys, and the waves' lists are merged.
+typedef uint32_t lp_u32x4 __attribute__((ext_vector_type(4)));
+// logit e of an access, kept packed
+template <typename T>
+PQN_D float lp_get(const lp_u32x4 &r, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r[e]);
+  else if constexpr (std::is_same<T, pqn_bf16>::value) return __uint_as_float(e & 1 ? r[e >> 1] & 0xffff0000u : r[e >> 1] << 16);
+  else return (float)__builtin_bit_cast(T, (uint16_t)(e & 1 ? r[e >> 1] >> 16 : r[e >> 1]));
+}
+// ... and put to -inf
+template <typename T>
+PQN_D void lp_forbid(lp_u32x4 &r, int e, bool no) {
+  if constexpr (sizeof(T) == 4) r[e] = no ? 0xff800000u : r[e];
+  else {
+    const uint32_t inf = std::is_same<T, pqn_bf16>::value ? 0xff80u : 0xfc00u, u = r[e >> 1];
+    r[e >> 1] = no ? (e & 1 ? (u & 0xffffu) | inf << 16 : (u & 0xffff0000u) | inf) : u;
+  }
+}
+
+template <typename T, int NT, int N>
+__global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
+  constexpr int NW = NT / 64, VW = 16 / (int)sizeof(T);
   __shared__ u64 keys[NW * LP_MAX_TOP];
-  __shared__ float sums[NW][4];
-  __shared__ uint32_t bar[NW];                                  // order bits of the waves' K-th keys
+  __shared__ float sums[NW][3];
+  __shared__ uint32_t bar[NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long row = blockIdx.x / A.splits;
   const int part = blockIdx.x % A.splits;
   const int c0 = part * A.part, c1 = min(A.a, c0 + A.part);
   const T *p = (const T *)A.logits + row * A.ls;
   const uint8_t *mk = A.mask ? A.mask + row * A.ms : nullptr;
-  if (threadIdx.x < NW) bar[threadIdx.x] = 0u;
-  __syncthreads();
-  LpSum v = {-INFINITY, 0.f, 0.f};
-  u64 list = 0ull;
-  uint32_t least = 0u;                                          // a newcomer's order bits must not be below
-  auto step = [&](auto &x, int j, int have) {                   // logits j .. of this lane, the first `have` of them real
-    constexpr int W = sizeof(x) / sizeof(float);
-    bool ok[W];                                                 // plain selects: a conditional store behind `have` and the mask was miscompiled
+  const int head = min(c1 - c0, (int)((16 - ((uintptr_t)(p + c0) & 15)) & 15) / (int)sizeof(T));
+  const int body = c0 + head, end = body + (c1 - body) / VW * VW, rest = head + (c1 - end);
+  auto first = [&](int i) { return body + (i * NT + (int)threadIdx.x) * VW; };
+  lp_u32x4 r[N];
 #pragma unroll
-    for (int e = 0; e < W; ++e) ok[e] = e < have;
-    if (mk)
+  for (int i = 0; i < N; ++i) {
+    r[i] = lp_u32x4{0u, 0u, 0u, 0u};
+    if (body + i * NT * VW < end) r[i] = *(const lp_u32x4 *)(p + (first(i) < end ? first(i) : body));
+  }
+  const bool has_rest = (int)threadIdx.x < rest;
+  const int jr = !has_rest ? c0 : (int)threadIdx.x < head ? c0 + threadIdx.x : end + (threadIdx.x - head);
+  float xr[1] = {pqn_to_f32(p[jr])};
+  xr[0] = has_rest && (!mk || mk[jr] != 0) ? xr[0] : -INFINITY;
+  if (mk) {
 #pragma unroll
-      for (int e = 0; e < W; ++e) ok[e] = ok[e] & (mk[min(j + e, c1 - 1)] != 0);
+    for (int i = 0; i < N; ++i)
+      if (body + i * NT * VW < end) {
 #pragma unroll
-    for (int e = 0; e < W; ++e) x[e] = ok[e] ? x[e] : -INFINITY;
-    float top = x[0];
-#pragma unroll
-    for (int e = 1; e < W; ++e) top = fmaxf(top, x[e]);
-    if (__any(top > v.m)) lp_shift(v, fmaxf(v.m, top), A.scale);
-    if (v.m > -INFINITY)
-#pragma unroll
-      for (int e = 0; e < W; ++e) lp_add(v, x[e], A.scale);
-    else                                                        // nothing but -inf and NaN so far
-#pragma unroll
-      for (int e = 0; e < W; ++e) v.s += x[e] != x[e] ? NAN : 0.f;
-    if (A.top > 0 && __any(top > -INFINITY && lp_order(top) >= least)) {
-      if constexpr (NW > 1) {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) least = max(least, __hip_atomic_load(&bar[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        for (int e = 0; e < VW; ++e) {
+          const bool no = mk[min(first(i) + e, c1 - 1)] == 0;
+          lp_forbid<T>(r[i], e, no);
+        }
       }
+  }
+  float top[N], m = xr[0];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    top[i] = -INFINITY;
+    if (body + i * NT * VW < end) {
+#pragma unroll
+      for (int e = 0; e < VW; ++e) top[i] = fmaxf(top[i], lp_get<T>(r[i], e));
+      top[i] = first(i) < end ? top[i] : -INFINITY;
+    }
+    m = fmaxf(m, top[i]);
+  }
+  LpSum v = {m, 0.f, 0.f};
+  const bool any = m > -INFINITY;
+  if (any && has_rest) lp_add(v, xr[0], A.scale);
+  v.s += has_rest && xr[0] != xr[0] ? NAN : 0.f;                     // also where there is nothing else
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (body + i * NT * VW < end && first(i) < end) {
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) lp_add(v, lp_get<T>(r[i], e), A.scale);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) v.s += lp_get<T>(r[i], e) != lp_get<T>(r[i], e) ? NAN : 0.f;
+      }
+    }
+  v = lp_group_join<64>(v, A.scale);
+  if (lane == 0) {
+    sums[wave][0] = v.m;
+    sums[wave][1] = v.s;
+    sums[wave][2] = v.t;
+  }
+  u64 list = 0ull;
+  if (A.top > 0) {
+    uint32_t mine = m > -INFINITY ? lp_order(m) : 0u, least = 0u;
+    for (int i = 0; i < A.top; ++i) {
+      least = pqn_wave_max(mine);
+      const int at = __ffsll(__ballot(mine == least)) - 1;           // one thread of the best
+      mine = lane == at ? 0u : mine;
+    }
+    if (lane == 0) bar[wave] = least;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) least = max(least, bar[w]);
+    auto look = [&](const auto &x, float best_x, int j) {
+      constexpr int W = sizeof(x) / sizeof(float);
+      const uint32_t best_o = best_x > -INFINITY ? lp_order(best_x) : 0u;
+      if (!__any(best_o >= max(least, 1u))) return;
       uint32_t o[W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) o[e] = x[e] > -INFINITY ? lp_order(x[e]) : 0u;
+      for (int e = 0; e < W; ++e) o[e] = best_o && x[e] > -INFINITY ? lp_order(x[e]) : 0u;
       for (;;) {
         const u64 best = lp_take(o, (uint32_t)j);
         const u64 last = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(list >> 32), A.top - 1) << 32) |
@@ -243,65 +311,45 @@ __global__ __launch_bounds__(NT) void lp_long_kernel(lp_args A) {
         if (best <= last || (uint32_t)(best >> 32) < least) break;   // 0 <= last: ends when nothing is left
         lp_insert(list, best, A.top);
       }
-      const uint32_t last = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(list >> 32), A.top - 1);
-      least = max(least, last);
-      if (NW > 1 && lane == 0) __hip_atomic_store(&bar[wave], last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    }
-  };
-  int body = c0;
-  if constexpr (VW > 1) {
-    const int head = min(c1 - c0, (int)((16 - ((uintptr_t)(p + c0) & 15)) & 15) / (int)sizeof(T));
-    const int tail = (c1 - c0 - head) % VW;
-    if (wave == 0 && head + tail > 0) {
-      const int j = lane < head ? c0 + lane : c1 - tail + (lane - head);
-      float x[1] = {lane < head + tail ? pqn_to_f32(p[j]) : 0.f};
-      step(x, lane < head + tail ? j : c0, lane < head + tail);
-    }
-    body = c0 + head;
-  }
-  const int end = body + (c1 - body) / VW * VW;
-  for (int base = body + wave * 64 * VW; base < end; base += NT * VW) {   // whole waves in, lanes behind the end hold nothing
-    const int j = base + lane * VW;
-    float x[VW];
+    };
+    look(xr, xr[0], jr);
 #pragma unroll
-    for (int e = 0; e < VW; ++e) x[e] = 0.f;
-    if (j < end) pqn_load<T, VW>(x, p + j);
-    step(x, j < end ? j : body, j < end ? VW : 0);
+    for (int i = 0; i < N; ++i)
+      if (body + i * NT * VW < end) {
+        float x[VW];
+#pragma unroll
+        for (int e = 0; e < VW; ++e) x[e] = lp_get<T>(r[i], e);
+        look(x, top[i], first(i));
+      }
+    if (lane < A.top) keys[wave * A.top + lane] = list;
   }
-  v = lp_group_join<64>(v, A.scale);
-  if (lane == 0) {
-    sums[wave][0] = v.m;
-    sums[wave][1] = v.s;
-    sums[wave][2] = v.t;
-  }
-  if (lane < A.top) keys[wave * A.top + lane] = list;
   __syncthreads();
   if (wave != 0) return;
   v = {sums[0][0], sums[0][1], sums[0][2]};
 #pragma unroll
   for (int w = 1; w < NW; ++w) v = lp_join(v, {sums[w][0], sums[w][1], sums[w][2]}, A.scale);
-  // the best of the NW lists
-  constexpr int ML = (NW * LP_MAX_TOP + 63) / 64;
-  u64 mine[ML];
-#pragma unroll
-  for (int i = 0; i < ML; ++i) mine[i] = i * 64 + lane < NW * A.top ? keys[i * 64 + lane] : 0ull;
-  const LpRow r = lp_row(v, A.inv_temp);
+  const LpRow rw = lp_row(v, A.inv_temp);
   float *rec = A.rec + ((size_t)row * A.splits + part) * LP_REC;
   if (lane == 0) {
-    if (A.splits == 1) lp_write_row<T>(A, row, r);
+    if (A.splits == 1) lp_write_row<T>(A, row, rw);
     else {
       rec[0] = v.m;
       rec[1] = v.s;
       rec[2] = v.t;
     }
   }
+  // the best of the NW lists
+  constexpr int ML = (NW * LP_MAX_TOP + 63) / 64;
+  u64 mine[ML];
+#pragma unroll
+  for (int i = 0; i < ML; ++i) mine[i] = i * 64 + lane < NW * A.top ? keys[i * 64 + lane] : 0ull;
   for (int i = 0; i < A.top; ++i) {
     u64 best = mine[0];
 #pragma unroll
     for (int k = 1; k < ML; ++k) best = lp_max(best, mine[k]);
     best = lp_group_max<64>(best);
     if (lane == 0) {
-      if (A.splits == 1) lp_write_top(A, row, i, best, r.lse);
+      if (A.splits == 1) lp_write_top(A, row, i, best, rw.lse);
       else ((u64 *)(rec + 4))[i] = best;
     }
 #pragma unroll
@@ -441,13 +489,15 @@ static lp_args lp_fill(const pqn_action_logprobs_t *a) {
   return A;
 }
 
-// Rows of up to LP_ROW_MAX logits live in a wave's registers.  Longer rows take a workgroup each, or several where there are too few
-// rows to fill the chip (a part keeps at least LP_MIN_PART logits, below which the join costs more than it gives).
-static constexpr int LP_ROW_MAX = 1024, LP_NT = 256, LP_MIN_PART = 4096, LP_FILL = 1024;
-static int lp_splits(int n, int a) {
+// Rows of up to LP_ROW_MAX logits live in a wave's registers, longer ones in a workgroup's, up to 16 accesses a thread (32768 16-bit or
+// 16384 f32 logits); beyond that, or where there are too few rows to fill the chip, a row is cut (a part keeps at least LP_MIN_PART
+// logits, below which the join costs more than it gives).
+static constexpr int LP_ROW_MAX = 1024, LP_NT = 256, LP_MIN_PART = 4096, LP_FILL = 1024, LP_MOST = 16;
+static int lp_splits(int n, int a, int vw) {
   if (a <= LP_ROW_MAX) return 1;
-  const int want = (LP_FILL + n - 1) / n, most = (a + LP_MIN_PART - 1) / LP_MIN_PART;
-  return want < most ? want : most;
+  const int want = (LP_FILL + n - 1) / n, most = (a + LP_MIN_PART - 1) / LP_MIN_PART, cap = LP_NT * vw * LP_MOST;
+  const int least = (a + cap - 1) / cap, s = want < most ? want : most;
+  return s > least ? s : least;
 }
 // columns per part: whole accesses of 8, so that a part starts as well aligned as its row
 static int lp_part(int a, int splits) { return ((a + splits - 1) / splits + 7) / 8 * 8; }
@@ -474,12 +524,17 @@ static int lp_launch(lp_args A, hipStream_t st) {
     LP_ROW_SHAPES(LP_GO, A.a)
 #undef LP_GO
   }
-  A.splits = lp_splits(A.n, A.a);
+  constexpr int VW = 16 / (int)sizeof(T);
+  A.splits = lp_splits(A.n, A.a, VW);
   A.part = lp_part(A.a, A.splits);
   A.splits = (A.a + A.part - 1) / A.part;
   const long long grid = (long long)A.n * A.splits;
   PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a);
-  lp_long_kernel<T, LP_NT, 16 / (int)sizeof(T)><<<(unsigned)grid, LP_NT, 0, st>>>(A);
+  const int each = (A.part + LP_NT * VW - 1) / (LP_NT * VW);
+  if (each <= 1) lp_long_kernel<T, LP_NT, 1><<<(unsigned)grid, LP_NT, 0, st>>>(A);
+  else if (each <= 2) lp_long_kernel<T, LP_NT, 2><<<(unsigned)grid, LP_NT, 0, st>>>(A);
+  else if (each <= 4) lp_long_kernel<T, LP_NT, 4><<<(unsigned)grid, LP_NT, 0, st>>>(A);
+  else lp_long_kernel<T, LP_NT, LP_MOST><<<(unsigned)grid, LP_NT, 0, st>>>(A);
   const int rc = pqn_check_launch("pqn_action_logprobs");
   if (rc != PQN_OK || A.splits == 1) return rc;
   lp_join_kernel<T><<<(unsigned)A.n, 64, 0, st>>>(A);
@@ -512,7 +567,7 @@ static int lp_launch_grad(lp_grad_args P, hipStream_t st) {
 
 extern "C" int64_t pqn_action_logprobs_workspace_bytes(int32_t n, int32_t a) {
   if (n <= 0 || a <= 0 || a > (1 << 30)) return 0;
-  const int s = lp_splits(n, a);
+  const int s = lp_splits(n, a, 4);      // of f32, the most
   return s > 1 ? (int64_t)n * s * LP_REC * 4 : 0;
 }
 
