@@ -43,15 +43,17 @@ PQN_D u64 lp_key(float logit, int j) {
   return logit > -INFINITY ? ((u64)lp_order(logit) << 32) | (uint32_t)~j : 0ull;   // false for NaN too
 }
 PQN_D u64 lp_max(u64 a, u64 b) { return a > b ? a : b; }
+// the best key of a group: the upper halves first, the lower ones among their best
 template <int G>
 PQN_D u64 lp_group_max(u64 k) {
-  if constexpr (G == 64) {               // the whole wave: the upper halves first, the lower ones among their best
-    const uint32_t hi = (uint32_t)(k >> 32), best = pqn_wave_max(hi);
+  const uint32_t hi = (uint32_t)(k >> 32);
+  if constexpr (G == 64) {
+    const uint32_t best = pqn_wave_max(hi);
     return ((u64)best << 32) | pqn_wave_max(hi == best ? (uint32_t)k : 0u);
+  } else {
+    const uint32_t best = pqn_group_max<G>(hi);
+    return ((u64)best << 32) | pqn_group_max<G>(hi == best ? (uint32_t)k : 0u);
   }
-#pragma unroll
-  for (int d = G / 2; d > 0; d >>= 1) k = lp_max(k, (u64)__shfl_xor((long long)k, d, 64));
-  return k;
 }
 
 // (m, s, t) of a set of logits: m the largest, s = sum 2^z, t = sum z 2^z with z = (logit - m) log2 e / temperature -- the difference
@@ -111,17 +113,34 @@ PQN_D float lp_logit(const lp_args &A, long long row, int j) {   // -inf where n
   if (A.mask && !A.mask[row * A.ms + j]) return -INFINITY;
   return pqn_to_f32(((const T *)A.logits)[row * A.ls + j]);
 }
+PQN_D float lp_logp(float logit, const LpRow &r, float inv_temp) {
+  return (r.lse != r.lse) ? NAN : logit > -INFINITY ? fmaf(logit, inv_temp, -r.lse) : -INFINITY;
+}
 template <typename T>
 PQN_D void lp_write_row(const lp_args &A, long long row, const LpRow &r) {
   A.lse[row] = r.lse;
   A.entropy[row] = r.entropy;
   const int act = A.action[row];
-  float lp = 0.f;                                                      // an id outside 0 .. a-1: no action, nothing is read
-  if (act >= 0 && act < A.a) {
-    const float l = lp_logit<T>(A, row, act);
-    lp = (r.lse != r.lse) ? NAN : l > -INFINITY ? l * A.inv_temp - r.lse : -INFINITY;
-  }
-  A.logp[row] = lp;
+  // an id outside 0 .. a-1: no action, nothing is read
+  A.logp[row] = act >= 0 && act < A.a ? lp_logp(lp_logit<T>(A, row, act), r, A.inv_temp) : 0.f;
+}
+// a row over G lanes, element e * G + lane at e: every request first, then the choices
+template <typename T, int G, int E>
+PQN_D void lp_row_load(const lp_args &A, long long row, int lane, float (&x)[E]) {
+  const T *p = (const T *)A.logits + row * A.ls;
+  T raw[E];
+  uint8_t on[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) raw[e] = p[min(e * G + lane, A.a - 1)];
+  if (A.mask) {
+    const uint8_t *mk = A.mask + row * A.ms;
+#pragma unroll
+    for (int e = 0; e < E; ++e) on[e] = mk[min(e * G + lane, A.a - 1)];
+  } else
+#pragma unroll
+    for (int e = 0; e < E; ++e) on[e] = 1;
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = (on[e] != 0) & (e * G + lane < A.a) ? pqn_to_f32(raw[e]) : -INFINITY;
 }
 PQN_D void lp_write_top(const lp_args &A, long long row, int i, u64 key, float lse) {
   A.top_action[row * A.top + i] = key ? (int32_t)~(uint32_t)key : -1;
@@ -135,24 +154,28 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(lp_args A) {
   const long long row0 = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
   const bool live = row0 < A.n;                    // rows behind the last one shuffle along with a copy of it
   const long long row = live ? row0 : A.n - 1;
+  const int act = A.action[row];
   float x[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int j = e * G + lane;
-    x[e] = j < A.a ? lp_logit<T>(A, row, j) : -INFINITY;
-  }
+  lp_row_load<T, G, E>(A, row, lane, x);
   LpSum v = {-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < E; ++e) v.m = fmaxf(v.m, x[e]);
-#pragma unroll
-  for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d, 64));
+  v.m = pqn_group_fmax<G>(v.m);
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (!(x[e] == -INFINITY)) lp_add(v, x[e], A.scale);
   v.s = pqn_group_sum<G>(v.s);
   v.t = pqn_group_sum<G>(v.t);
   const LpRow r = lp_row(v, A.inv_temp);
-  if (live && lane == 0) lp_write_row<T>(A, row, r);
+  // the taken action's logit is in the register of one of the lanes; an id outside the row is in none
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (live && e * G + lane == act && act < A.a) A.logp[row] = lp_logp(x[e], r, A.inv_temp);
+  if (live && lane == 0) {
+    A.lse[row] = r.lse;
+    A.entropy[row] = r.entropy;
+    if (act < 0 || act >= A.a) A.logp[row] = 0.f;
+  }
   if (A.top > 0) {
     u64 key[E];
 #pragma unroll
@@ -424,10 +447,12 @@ __global__ __launch_bounds__(256) void lp_grad_rows_kernel(lp_grad_args P) {
   LpGrad R;
   R.open<T>(P, row);
   T *o = (T *)P.dlogits + row * A.a;
+  float x[E];
+  lp_row_load<T, G, E>(A, row, lane, x);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = e * G + lane;
-    if (j < A.a) o[j] = (T)R.at(lp_logit<T>(A, row, j), j);
+    if (j < A.a) o[j] = (T)R.at(x[e], j);
   }
 }
 // wide rows: `blocks` workgroups to a row, LP_SPAN accesses of VW logits a lane.  Rows whose logits and gradients lie alike on 16

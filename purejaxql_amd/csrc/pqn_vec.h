@@ -30,14 +30,6 @@ PQN_D void pqn_store(T *dst, const float *src) {
   *(pqn_pack<T, W> *)dst = p;
 }
 
-// sum over the lanes of an aligned group of G lanes (G a power of two), the same in every lane
-template <int G = 64>
-PQN_D float pqn_group_sum(float x) {
-#pragma unroll
-  for (int d = G / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-  return x;
-}
-
 // reductions over the wave, the same in every lane: four DPP steps within the rows of 16 lanes (zeros come in from their ends, neutral
 // for the sum and the maximum of unsigned values), two broadcasts across them, lane 63 read back
 #define PQN_WAVE_STEPS(OP)                                                                          \
@@ -55,6 +47,33 @@ PQN_D float pqn_wave_sum(float x) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 PQN_D uint32_t pqn_wave_min(uint32_t x) { return ~pqn_wave_max(~x); }
+
+// the same over aligned groups of G lanes (G = 8, 16, 32, 64), in every lane of the group: exchanges within 4, 8 and 16 lanes by DPP (a
+// mirrored row of equal halves is the other half), across them by a shuffle
+template <int G, typename OP>
+PQN_D uint32_t pqn_group_fold(uint32_t x, OP op) {
+#define PQN_STEP(ctrl) x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true));
+  PQN_STEP(0xb1)                         // quad_perm [1, 0, 3, 2]
+  PQN_STEP(0x4e)                         // quad_perm [2, 3, 0, 1]
+  PQN_STEP(0x141)                        // row_half_mirror
+  if constexpr (G >= 16) { PQN_STEP(0x140) }   // row_mirror
+#undef PQN_STEP
+#pragma unroll
+  for (int d = 16; d < G; d <<= 1) x = op(x, (uint32_t)__shfl_xor((int)x, d, 64));
+  return x;
+}
+template <int G>
+PQN_D float pqn_group_sum(float x) {
+  return __uint_as_float(pqn_group_fold<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+template <int G>
+PQN_D float pqn_group_fmax(float x) {
+  return __uint_as_float(pqn_group_fold<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int G>
+PQN_D uint32_t pqn_group_max(uint32_t x) {
+  return pqn_group_fold<G>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
 
 inline int pqn_dtype_size(int dtype) { return dtype == PQN_DTYPE_F32 ? 4 : 2; }
 inline bool pqn_dtype_known(int dtype) { return dtype == PQN_DTYPE_F32 || dtype == PQN_DTYPE_BF16 || dtype == PQN_DTYPE_F16; }

@@ -92,18 +92,18 @@ class FlatRAdam:
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
-def _last_contiguous(t: torch.Tensor, name: str, shape, dtype, device):
-    """A tensor of this shape, type and device whose last index is contiguous; other strides are the caller's."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name}: need {tuple(shape)} of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+def _last_contiguous(t: torch.Tensor, name: str, shape, dtype, index: int):
+    """A tensor of this shape and type on GPU `index` whose last index is contiguous; other strides are the caller's."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index:
+        raise ValueError(f"{name}: need {tuple(shape)} of {dtype} on cuda:{index}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last index must be contiguous, strides are {tuple(t.stride())}")
 
 
-def _exactly(t: torch.Tensor, name: str, shape, dtype, device):
-    """A contiguous tensor of this shape, type and device."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: need contiguous {tuple(shape)} of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} on {t.device} "
+def _exactly(t: torch.Tensor, name: str, shape, dtype, index: int):
+    """A contiguous tensor of this shape and type on GPU `index`."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: need contiguous {tuple(shape)} of {dtype} on cuda:{index}, got {tuple(t.shape)} of {t.dtype} on {t.device} "
                          f"contig={t.is_contiguous()}")
 
 
@@ -116,13 +116,12 @@ def _flags(t: torch.Tensor) -> torch.Tensor:
     return t.view(torch.uint8) if t.dtype == torch.bool else t
 
 
-def _enqueue(fn, args, device: torch.device, what: str):
-    """fn(args, stream) on the tensors' own device and torch's current stream there."""
-    index = device.index
+def _enqueue(fn, args, index: int, what: str):
+    """fn(args, stream) on the tensors' own GPU and torch's current stream there."""
     if index == torch.cuda.current_device():
         rc = fn(byref(args), torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(byref(args), torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         _lib.check(rc, what)
@@ -136,7 +135,7 @@ def _attn_args(a, q, k, v, decay, state, reset, scale, step: bool):
     _on_gpu(q, "q", _ATTN_DTYPES)
     if q.dim() != (3 if step else 4) or v.dim() != q.dim():
         raise ValueError(f"q, v: need {'[M, H, D]' if step else '[T, M, H, D]'}, got {tuple(q.shape)}, {tuple(v.shape)}")
-    shape, dt, dev = q.shape, q.dtype, q.device
+    shape, dt, dev = q.shape, q.dtype, q.get_device()
     lead, dk, dv = shape[:-1], shape[-1], v.shape[-1]
     if not (0 < dk <= _lib.ATTN_MAX_D and 0 < dv <= _lib.ATTN_MAX_D):
         raise ValueError(f"q, v: head widths of 1 .. {_lib.ATTN_MAX_D}, got {dk} and {dv}")
@@ -184,7 +183,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     new = torch.empty(st, dtype=torch.float32, device=q.device) if want_state else None
     a.out, a.state_out = out.data_ptr(), _lib.ptr(new)
     ws = _attn_workspace(a, 0, q.device)  # noqa: F841 (held until the launch is enqueued)
-    _enqueue(lib.pqn_decay_attn, a, q.device, "pqn_decay_attn")
+    _enqueue(lib.pqn_decay_attn, a, q.get_device(), "pqn_decay_attn")
     return out, new
 
 
@@ -199,7 +198,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     lead, _ = _attn_args(a, q, k, v, decay, state, reset, scale, True)
     out = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
     a.out, a.state_out = out.data_ptr(), a.state_in
-    _enqueue(lib.pqn_decay_attn, a, q.device, "pqn_decay_attn")
+    _enqueue(lib.pqn_decay_attn, a, q.get_device(), "pqn_decay_attn")
     return out
 
 
@@ -212,16 +211,16 @@ def decay_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     lib = _lib.load()
     a = _lib.DecayAttnArgs()
     lead, st = _attn_args(a, q, k, v, decay, state, reset, scale, False)
-    _last_contiguous(dout, "dout", lead + (a.dv,), q.dtype, q.device)
+    _last_contiguous(dout, "dout", lead + (a.dv,), q.dtype, q.get_device())
     if dstate_out is not None:
-        _exactly(dstate_out, "dstate_out", st, torch.float32, q.device)
+        _exactly(dstate_out, "dstate_out", st, torch.float32, q.get_device())
     a.dout, a.dout_stride, a.dstate_out = dout.data_ptr(), dout.stride()[:-1], _lib.ptr(dstate_out)
     dq, dk = (torch.empty(lead + (a.dk,), dtype=q.dtype, device=q.device) for _ in range(2))
     dv = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
     dstate = torch.empty(st, dtype=torch.float32, device=q.device) if state is not None else None
     a.dq, a.dk_out, a.dv_out, a.dstate_in = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dstate)
     ws = _attn_workspace(a, 1, q.device)  # noqa: F841
-    _enqueue(lib.pqn_decay_attn_grad, a, q.device, "pqn_decay_attn_grad")
+    _enqueue(lib.pqn_decay_attn_grad, a, q.get_device(), "pqn_decay_attn_grad")
     return dq, dk, dv, dstate
 
 
@@ -230,9 +229,9 @@ _GATES = {"none": 0, "sigmoid": 1, "silu": 2}
 _NORM_PARAMS = ("res_scale", "post_scale", "post_bias", "pre_scale", "pre_bias")
 
 
-def _rows(t: torch.Tensor, name: str, shape, dtype, device) -> Tuple[torch.Tensor, int]:
+def _rows(t: torch.Tensor, name: str, shape, dtype, index: int) -> Tuple[torch.Tensor, int]:
     """t as rows of its last index: (tensor that holds them, stride between rows)."""
-    _last_contiguous(t, name, shape, dtype, device)
+    _last_contiguous(t, name, shape, dtype, index)
     if t.dim() == 2:
         return t, t.stride(0)
     t = t.reshape(-1, shape[-1])    # a view wherever the rows are evenly spaced, else a copy
@@ -247,7 +246,7 @@ def _norm_args(x, f, gate, gate_act, params, norm_type, post, pre, eps):
         raise ValueError(f"norm_type: one of {sorted(_NORMS)}, gate_act: one of {sorted(_GATES)}; got {norm_type!r}, {gate_act!r}")
     if (gate is None) != (gate_act == "none"):
         raise ValueError("gate and gate_act go together: a gate tensor with 'sigmoid' or 'silu', neither with 'none'")
-    shape, d, dt, dev = x.shape, x.shape[-1], x.dtype, x.device
+    shape, d, dt, dev = x.shape, x.shape[-1], x.dtype, x.get_device()
     a = _lib.ResidualNormArgs()
     x, a.x_stride = _rows(x, "x", shape, dt, dev)
     f, a.f_stride = _rows(f, "f", shape, dt, dev)
@@ -281,7 +280,7 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, gate: Optional[torch.Tensor]
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     h = torch.empty(shape, dtype=x.dtype, device=x.device) if pre else None
     a.y, a.h = y.data_ptr(), _lib.ptr(h)
-    _enqueue(_lib.load().pqn_residual_norm, a, x.device, "pqn_residual_norm")
+    _enqueue(_lib.load().pqn_residual_norm, a, x.get_device(), "pqn_residual_norm")
     return y, h
 
 
@@ -302,7 +301,7 @@ def residual_norm_grad(x: torch.Tensor, f: torch.Tensor, dy: Optional[torch.Tens
     held = []
     for name, g in (("dy", dy), ("dh", dh)):
         if g is not None:
-            g, stride = _rows(g, name, shape, x.dtype, x.device)
+            g, stride = _rows(g, name, shape, x.dtype, x.get_device())
             held.append(g)
             setattr(a, name, g.data_ptr())
             setattr(a, name + "_stride", stride)
@@ -316,7 +315,7 @@ def residual_norm_grad(x: torch.Tensor, f: torch.Tensor, dy: Optional[torch.Tens
     n = lib.pqn_residual_norm_workspace_floats(a.n, a.d)
     ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
     a.workspace = _lib.ptr(ws)
-    _enqueue(lib.pqn_residual_norm_grad, a, x.device, "pqn_residual_norm_grad")
+    _enqueue(lib.pqn_residual_norm_grad, a, x.get_device(), "pqn_residual_norm_grad")
     return got
 
 
@@ -325,7 +324,7 @@ def _logprob_args(logits, actions, mask, temperature, top):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits: need [N, A] with A >= 1, got {tuple(logits.shape)}")
     n, width = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
     _last_contiguous(logits, "logits", (n, width), logits.dtype, dev)
     _exactly(actions, "actions", (n,), torch.int32, dev)
     if not 0 <= top <= min(width, _lib.LOGPROB_MAX_TOP):
@@ -353,7 +352,7 @@ def action_logprobs(logits: torch.Tensor, actions: torch.Tensor, mask: Optional[
     lse -inf and entropy 0."""
     a = _logprob_args(logits, actions, mask, temperature, top)
     n, dev, f32 = a.n, logits.device, torch.float32
-    logp, entropy, lse = (torch.empty(n, dtype=f32, device=dev) for _ in range(3))
+    logp, entropy, lse = torch.empty(3, n, dtype=f32, device=dev).unbind(0)
     top_logp = torch.empty(n, top, dtype=f32, device=dev)
     top_action = torch.empty(n, top, dtype=torch.int32, device=dev)
     a.logp, a.entropy, a.lse, a.top_logp, a.top_action = (t.data_ptr() for t in (logp, entropy, lse, top_logp, top_action))
@@ -361,7 +360,7 @@ def action_logprobs(logits: torch.Tensor, actions: torch.Tensor, mask: Optional[
     size = lib.pqn_action_logprobs_workspace_bytes(n, a.a)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     a.workspace = _lib.ptr(ws)
-    _enqueue(lib.pqn_action_logprobs, a, dev, "pqn_action_logprobs")
+    _enqueue(lib.pqn_action_logprobs, a, dev.index, "pqn_action_logprobs")
     return logp, entropy, lse, top_logp, top_action
 
 
@@ -372,14 +371,14 @@ def action_logprobs_grad(logits: torch.Tensor, actions: torch.Tensor, lse: torch
     """Gradient of action_logprobs with respect to the logits from those of logp, entropy and lse (f32 [N], None: zeros, not all);
     lse and entropy as action_logprobs returned them.  0 where not allowed."""
     a = _logprob_args(logits, actions, mask, temperature, 0)
-    n, dev = a.n, logits.device
+    n, dev = a.n, logits.get_device()
     if dlogp is None and dentropy is None and dlse is None:
         raise ValueError("dlogp, dentropy, dlse: at least one of the gradients is needed")
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy), ("dlse", dlse)):
         if t is not None:
             _exactly(t, name, (n,), torch.float32, dev)
             setattr(a, name, t.data_ptr())
-    dlogits = torch.empty(n, a.a, dtype=logits.dtype, device=dev)
+    dlogits = torch.empty(n, a.a, dtype=logits.dtype, device=logits.device)
     a.dlogits = dlogits.data_ptr()
     _enqueue(_lib.load().pqn_action_logprobs_grad, a, dev, "pqn_action_logprobs_grad")
     return dlogits
