@@ -190,6 +190,11 @@ static int da_run_chunks(da_args &A, int passes, int dtype, int vec, void *works
   const int a = A.pass[0].a, b = A.pass[0].b;
   da_split X = da_cut(A.t_len, rows, passes, a, b, vec);
   const int size = da_state_size(X, a, b);
+  for (int p = 0; p < passes; ++p) {
+    da_pass &P = A.pass[p];
+    const uintptr_t at = (uintptr_t)P.s_in | (uintptr_t)P.s_out;
+    P.s_vec = P.s_cs == 1 && P.b % 2 == 0 && at % 8 == 0 ? 2 : P.s_rs == 1 && P.a % 4 == 0 && at % 16 == 0 ? 4 : 0;
+  }
   X.pass_stride = rows * (X.parts - 1) * size;
   X.cut_stride = (rows * (X.parts - 1) * 4 + 15) / 16 * 4;
   X.state = (float *)workspace;

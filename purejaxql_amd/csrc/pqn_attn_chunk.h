@@ -11,6 +11,7 @@ struct da_pass {
   const float *s_in;
   float *s_out;
   int s_rs, s_cs;                         // element strides of the state's first (q, k) and second (v, o) index
+  int s_vec;                              // 2: pairs of columns lie on 8 bytes; 4: fours of rows on 16; 0: neither
   const uint8_t *reset;                   // flag of the border before step i at reset[i * reset_ts + row]
   long long reset_ts;
   float o_scale, s_scale;                 // on the outputs; on what a step adds to the state
@@ -31,7 +32,7 @@ struct da_args {
 // Everything is computed transposed so that no operand leaves the registers to change its layout: P^T = K Q^T leaves 4 neighbouring
 // j of one t in a lane, O^T = S^T Q^T + V^T P^T takes the state's accumulators as they lie as its left operand, and S += K^T (w V)
 // shares V's fragments with it.  The columns of q, k, v are assigned to accumulator rows so that a lane's 8 values of two stacked
-// 16 x 16 tiles are 8 neighbouring columns (da_col): one 16-byte read of Q, one 16-byte store of O.
+// 16 x 16 tiles are 8 neighbouring columns (da_row, da_col): one 16-byte read of Q, one 16-byte store of O.
 //
 // bf16: v_mfma_f32_16x16x32_bf16 with the state (S^T Q^T) and the weighted products (V^T P^T) rounded to bf16 as operands -- the
 // output is rounded to bf16 anyway -- and w V split in two bf16 pieces (16 significant bits), because the state is an f32 result that
@@ -46,12 +47,15 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short da_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) da_s16x4 da_lds_s16x4;
 
-// column of row (or lane) r of tile `tile`, tiles counted over 16 columns each
+// The state's accumulator tiles: row r of tile i is row da_row(i, r) of the state -- a lane's 8 values of two stacked bf16 tiles are 8
+// neighbouring rows -- and lane r of tile c (of a wave's two) is column da_col(c, r) of the wave's 32: the two tiles' values of a lane
+// lie side by side, for 8-byte accesses to the state and 8 neighbouring outputs in a lane.
 template <typename T>
-PQN_D int da_col(int tile, int r) {
+PQN_D int da_row(int tile, int r) {
   if constexpr (sizeof(T) == 2) return 32 * (tile >> 1) + 8 * (r >> 2) + 4 * (tile & 1) + (r & 3);
   else return 16 * tile + r;
 }
+PQN_D int da_col(int c, int r) { return 2 * r + c; }
 
 // A matrix of W columns in LDS, one row per step.  bf16: rows of W / 8 slots of 16 B, slot s of row r at s ^ swz(r): both the 16-byte
 // reads of 8 rows at one column and the transposing reads (4 rows x 4 slots per 16 lanes) touch every bank once.  f32: rows padded by
@@ -73,23 +77,42 @@ struct DaTile {
     const int lane = threadIdx.x & 63;
     return *(const F *)(m + at(row0 + (lane & 15), col0 + (lane >> 4) * EV));
   }
-  // operand with the column index on the lanes (columns da_col(tile, lane & 15) behind col0), k down the rows from row0.  bf16: a
-  // lane's 8 values are rows 4 g + e and 16 + 4 g + e (e < 4), the order in which two 16 x 16 accumulators lie in a lane
+  // operand with the column index on the lanes (columns da_row(tile, lane & 15)), k down the rows from row0.  bf16: a lane's 8 values are
+  // rows 4 g + e and 16 + 4 g + e (e < 4), the order in which two 16 x 16 accumulators lie in a lane
   template <typename F>
-  PQN_D static F cols(const T *m, int row0, int col0, int tile) {
+  PQN_D static F cols(const T *m, int row0, int tile) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-    F f;
+    if constexpr (sizeof(T) == 2) return turned<F>(m, row0 + 4 * g + (i >> 2), 32 * (tile >> 1) + 8 * (i & 3) + 4 * (tile & 1));
+    else {
+      F f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) f[s] = m[at(row0 + 4 * g + s, 16 * tile + i)];
+      return f;
+    }
+  }
+  // the same for both tiles of the 32 columns from col0 in the order of da_col.  bf16: such a tile's slots hold their 8 columns as the
+  // even ones, then the odd ones (DaLoad, PAIRS), so that a transposing read finds a tile's four neighbours side by side
+  template <typename F>
+  PQN_D static void pairs(const T *m, int row0, int col0, F (&f)[2]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     if constexpr (sizeof(T) == 2) {
-      const int c = col0 + 32 * (tile >> 1) + 8 * (i & 3) + 4 * (tile & 1), r = row0 + 4 * g + (i >> 2);
-      const da_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r, c)));
-      const da_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r + 16, c)));
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      f = __builtin_bit_cast(F, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) f[c] = turned<F>(m, row0 + 4 * g + (i >> 2), col0 + 8 * (i & 3) + 4 * c);
     } else {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) f[s] = m[at(row0 + 4 * g + s, col0 + 16 * tile + i)];
+      for (int s = 0; s < 4; ++s) {
+        const pqn_pack<float, 2> v = *(const pqn_pack<float, 2> *)(m + at(row0 + 4 * g + s, col0 + 2 * i));
+        f[0][s] = v.v[0];
+        f[1][s] = v.v[1];
+      }
     }
-    return f;
+  }
+  template <typename F>
+  PQN_D static F turned(const T *m, int r, int c) {
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const da_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r, c)));
+    const da_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_s16x4 *)(m + at(r + 16, c)));
+    return __builtin_bit_cast(F, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 
@@ -103,7 +126,8 @@ PQN_D f32x4_t da_mfma(f32x4_t a, f32x4_t b, f32x4_t c) {   // k = 4 (lane >> 4) 
 // Rows of one (row, head)'s tensor on their way to a DaTile<T, W> of L rows.  load() only requests: every lane reads some row and column
 // that exists, without a branch, so that all requests are in flight together; store() puts zeros into the rows from n on.  Columns
 // from `width` on are never written: the tile starts out as zeros.
-template <typename T, int W, int L, int NTHR, bool VEC>
+// PAIRS: the slots' even columns before their odd ones (DaTile::pairs; bf16 only)
+template <typename T, int W, int L, int NTHR, bool VEC, bool PAIRS>
 struct DaLoad {
   static constexpr int EV = 16 / (int)sizeof(T), VPR = W / EV, STEP = NTHR / VPR, N = (L + STEP - 1) / STEP;
   static_assert(NTHR % VPR == 0, "whole rows per pass");
@@ -155,7 +179,11 @@ struct DaLoad {
         r[i] = __builtin_bit_cast(u32x4_t, v);
       }
       if (n < L && row >= n) r[i] = u32x4_t{0u, 0u, 0u, 0u};
-      if (inside(row)) *(u32x4_t *)(lds + DaTile<T, W>::at(row, c)) = r[i];
+      u32x4_t x = r[i];
+      if constexpr (PAIRS && sizeof(T) == 2)
+        x = u32x4_t{__builtin_amdgcn_perm(r[i][1], r[i][0], 0x05040100u), __builtin_amdgcn_perm(r[i][3], r[i][2], 0x05040100u),
+                    __builtin_amdgcn_perm(r[i][1], r[i][0], 0x07060302u), __builtin_amdgcn_perm(r[i][3], r[i][2], 0x07060302u)};
+      if (inside(row)) *(u32x4_t *)(lds + DaTile<T, W>::at(row, c)) = x;
     }
   }
   PQN_D static void zero_behind(T *lds, int n) {
@@ -192,8 +220,6 @@ PQN_D uint32_t da_pair(float a, float b) { return __builtin_bit_cast(uint32_t, _
 PQN_D float da_low(uint32_t p) { return __uint_as_float(p << 16); }
 PQN_D float da_high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-static constexpr int DA_WAVES = 2;   // waves per SIMD at least
-
 struct da_split {       // the time axis in `parts` parts of `len` steps, one workgroup each; parts = 1: not cut
   int parts, len;
   int vec;              // every row of every tensor of the launch starts on 16 bytes and is whole 16-byte accesses
@@ -202,10 +228,70 @@ struct da_split {       // the time axis in `parts` parts of `len` steps, one wo
   long long pass_stride, cut_stride;
 };
 
-// STATE: only what the part adds to the state (its first step onwards from zero, the first part from the state that came in)
-template <typename T, int AP, int NW, int L, bool VEC, bool STATE>
-__global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, da_split X, int passes) {
-  constexpr bool B16 = sizeof(T) == 2;
+// A wave's 32 columns of a state in memory, to or from its accumulators: two columns an access where they lie side by side, four rows
+// where those do (a transposed state).  WHOLE: every row and column exists, and the requests go out without a branch between them.
+template <typename T, int NS, bool WRITE, bool WHOLE>
+PQN_D void da_state_of(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = dv0 + 2 * (lane & 15);
+  typedef pqn_pack<float, 2> two;
+  typedef pqn_pack<float, 4> four;
+  if (P.s_vec == 2) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = da_row<T>(i, 4 * g) + e;
+        if (WHOLE || (row < P.a && col < P.b)) {
+          two *p = (two *)(mem + (long long)row * P.s_rs + col);
+          if (WRITE) *p = two{{s[i][0][e], s[i][1][e]}};
+          else {
+            const two v = *p;
+            s[i][0][e] = v.v[0];
+            s[i][1][e] = v.v[1];
+          }
+        }
+      }
+  } else if (P.s_vec == 4) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = da_row<T>(i, 4 * g);
+        if (WHOLE || (row < P.a && col + c < P.b)) {
+          four *p = (four *)(mem + row + (long long)(col + c) * P.s_cs);
+          if (WRITE) *p = __builtin_bit_cast(four, s[i][c]);
+          else s[i][c] = __builtin_bit_cast(f32x4_t, *p);
+        }
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = da_row<T>(i, 4 * g) + e;
+          if (row < P.a && col + c < P.b) {
+            float *p = mem + (long long)row * P.s_rs + (long long)(col + c) * P.s_cs;
+            if (WRITE) *p = s[i][c][e];
+            else s[i][c][e] = *p;
+          }
+        }
+  }
+}
+template <typename T, int NS, int BP, bool WRITE>
+PQN_D void da_state(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) {
+  if (P.a == 16 * NS && P.b == BP) da_state_of<T, NS, WRITE, true>(s, mem, P, dv0);
+  else da_state_of<T, NS, WRITE, false>(s, mem, P, dv0);
+}
+
+// What a workgroup does: MAIN a part of the time axis; STATE only what the part adds to the state (its first step onwards from zero, the
+// first part from the state that came in); ONE a window that is one chunk, with nothing in flight beside the computation and so with
+// registers for twice the waves.
+enum { DA_MAIN, DA_STATE, DA_ONE };
+template <typename T, int AP, int NW, int L, bool VEC, int MODE>
+__global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void da_chunk_kernel(da_args A, da_split X, int passes) {
+  constexpr bool B16 = sizeof(T) == 2, STATE = MODE == DA_STATE;
   constexpr int NTHR = 64 * NW, BP = 32 * NW, KB = B16 ? 32 : 16, NF = AP / KB, NS = AP / 16, NJ = L / KB, NT = L / 16;
   constexpr int EV = 16 / (int)sizeof(T), PER = KB / 16, OUT = B16 ? 1 : 2;
   // The weights between the steps of a chunk: the waves share the tiles out and exchange them through LDS.  A wave alone keeps them in
@@ -230,8 +316,8 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
   const int h = (int)(mh % A.heads), row = (int)(mh / A.heads);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, ln = lane & 15;
   const int t_first = part * X.len, t_end = min(A.t_len, t_first + X.len);
-  DaLoad<T, AP, L, NTHR, VEC> rq, rk;
-  DaLoad<T, BP, L, NTHR, VEC> rv;
+  DaLoad<T, AP, L, NTHR, VEC, false> rq, rk;
+  DaLoad<T, BP, L, NTHR, VEC, true> rv;
   if constexpr (!STATE) rq.start((const T *)P.q + t_first * P.qs[0] + row * P.qs[1] + h * P.qs[2], P.qs[0], P.a);
   rk.start((const T *)P.k + t_first * P.ks[0] + row * P.ks[1] + h * P.ks[2], P.ks[0], P.a);
   rv.start((const T *)P.v + t_first * P.vs[0] + row * P.vs[1] + h * P.vs[2], P.vs[0], P.b);
@@ -253,16 +339,7 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
   const int dv0 = 32 * wave;
   float *xs = X.state + pass * X.pass_stride + (mh * (X.parts - 1)) * (long long)(AP * BP) + wave * (AP * 32) + lane * 4;
   if (part == 0) {
-    if (P.s_in)
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int ra = da_col<T>(i, 4 * g + e), cb = dv0 + da_col<T>(c, ln);
-            if (ra < P.a && cb < P.b) s[i][c][e] = P.s_in[so + (long long)ra * P.s_rs + (long long)cb * P.s_cs];
-          }
+    if (P.s_in) da_state<T, NS, BP, false>(s, const_cast<float *>(P.s_in) + so, P, dv0);
   } else if constexpr (!STATE) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
@@ -278,9 +355,9 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
     }
     for (int i = threadIdx.x; i < L * TB::LD; i += NTHR) Vs[i] = (T)0.f;
   }
-  T *op = STATE ? nullptr : (T *)P.o + t_first * P.os[0] + row * P.os[1] + h * P.os[2] + ln * P.os[0] + dv0 + (B16 ? 8 : 4) * g;
+  T *op = STATE ? nullptr : (T *)P.o + t_first * P.os[0] + row * P.os[1] + h * P.os[2] + ln * P.os[0] + dv0 + 8 * g;
   typedef pqn_pack<T, EV> Out;
-  Out held[NT][OUT];                   // a chunk's outputs, step 16 tt + ln: 8 columns from 8 g, or 4 from 16 c + 4 g
+  Out held[NT][OUT];                   // a chunk's outputs, step 16 tt + ln, 8 columns from 8 g
   int n_held = 0;
   auto write_out = [&]() {
 #pragma unroll
@@ -288,8 +365,8 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
       if (16 * tt + ln >= n_held) continue;
 #pragma unroll
       for (int c = 0; c < OUT; ++c) {
-        T *dst = op + 16 * tt * P.os[0] + 16 * c;
-        const int col = dv0 + (B16 ? 8 * g : 16 * c + 4 * g);
+        T *dst = op + 16 * tt * P.os[0] + 4 * c;
+        const int col = dv0 + 8 * g + 4 * c;
         if constexpr (VEC) {
           if (col < P.b) *(pqn_pack<T, EV> *)dst = held[tt][c];
         } else
@@ -334,6 +411,7 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
   __syncthreads();                                     // pw
   for (int t0 = t_first; t0 < t_end;) {
     int n = min(L, t_end - t0);
+    if (MODE == DA_ONE && t0 > 0) fetch(t0);           // only where a chunk is taken step by step
     rk.store(Ks, n);
     rv.store(Vs, n);
     if constexpr (!STATE) rq.store(Qs, n);
@@ -354,12 +432,12 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
     const unsigned long long cuts = cuts_all & ((1ull << n) - 1ull);
     // Outputs leave one chunk late, in front of the next requests: memory operations end in order, so the wait for a chunk's inputs
     // would otherwise be one for the stores behind them as well.
-    if constexpr (!STATE) write_out();
+    if constexpr (MODE == DA_MAIN) write_out();
     if (t0 + n < t_end) {
       rk.advance(n);
       rv.advance(n);
       if constexpr (!STATE) rq.advance(n);
-      fetch(t0 + n);
+      if constexpr (MODE != DA_ONE) fetch(t0 + n);
     }
     const int first = (t0 == 0 && P.late) ? 0 : 1;     // borders up to and including step 0 of this chunk
     const bool plain = n == L && !cuts && first;
@@ -397,11 +475,9 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
       }
       __syncthreads();
     }
-    F vf[2][NJ];
+    F vf[NJ][2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) vf[c][j] = TB::template cols<F>(Vs, j * KB, dv0, c);
+    for (int j = 0; j < NJ; ++j) TB::template pairs<F>(Vs, j * KB, dv0, vf[j]);
     if constexpr (!STATE) {
       F sf[NF][2];
 #pragma unroll
@@ -451,16 +527,18 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
             pf = __builtin_bit_cast(F, u);
           } else pf = weights(tt, j, qf);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) o[c] = da_mfma(vf[c][j], pf, o[c]);
+          for (int c = 0; c < 2; ++c) o[c] = da_mfma(vf[j][c], pf, o[c]);
         }
         if constexpr (B16)
-          held[tt][0] = __builtin_bit_cast(Out, (u32x4_t{da_pair(o[0][0], o[0][1]), da_pair(o[0][2], o[0][3]),
-                                                                        da_pair(o[1][0], o[1][1]), da_pair(o[1][2], o[1][3])}));
+          held[tt][0] = __builtin_bit_cast(Out, (u32x4_t{da_pair(o[0][0], o[1][0]), da_pair(o[0][1], o[1][1]), da_pair(o[0][2], o[1][2]),
+                                                         da_pair(o[0][3], o[1][3])}));
         else
 #pragma unroll
-          for (int c = 0; c < OUT; ++c) held[tt][c] = __builtin_bit_cast(Out, o[c]);
+          for (int c = 0; c < OUT; ++c)
+            held[tt][c] = __builtin_bit_cast(Out, (f32x4_t{o[0][2 * c], o[1][2 * c], o[0][2 * c + 1], o[1][2 * c + 1]}));
       }
       n_held = n;
+      if constexpr (MODE == DA_ONE) write_out();
     }
     // the state behind the chunk
     const float fade = pw[n - 1 + first];
@@ -486,7 +564,7 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if constexpr (B16) {
-          const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[c][j]);
+          const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[j][c]);
           u32x4_t u[3];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -502,11 +580,11 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
           for (int k = 0; k < 3; ++k) x[c][k] = __builtin_bit_cast(F, u[k]);
         } else
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[c][0][e] = vf[c][j][e] * wu[j][e];
+          for (int e = 0; e < 4; ++e) x[c][0][e] = vf[j][c][e] * wu[j][e];
       }
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const F kf = TA::template cols<F>(Ks, j * KB, 0, i);
+        const F kf = TA::template cols<F>(Ks, j * KB, i);
 #pragma unroll
         for (int k = 0; k < PIECES; ++k)
 #pragma unroll
@@ -516,7 +594,7 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
     t0 += n;
     __syncthreads();                                   // the chunk has been read
   }
-  if constexpr (!STATE) write_out();
+  if constexpr (MODE == DA_MAIN) write_out();
   if constexpr (STATE) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
@@ -524,17 +602,16 @@ __global__ __launch_bounds__(64 * NW, DA_WAVES) void da_chunk_kernel(da_args A, 
       for (int c = 0; c < 2; ++c) *(f32x4_t *)(xs + (long long)part * (AP * BP) + (i * 2 + c) * 256) = s[i][c];
     if (threadIdx.x == 0) X.cut[pass * X.cut_stride + mh * (X.parts - 1) + part] = any_cut;
   } else if (P.s_out && part == X.parts - 1) {
-    const bool cut = P.late && P.reset && P.reset[A.t_len * P.reset_ts + row];
-    const float fade = P.late ? pw[1] : 1.f;
+    if (P.late) {
+      const bool cut = P.reset && P.reset[A.t_len * P.reset_ts + row];
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int ra = da_col<T>(i, 4 * g + e), cb = dv0 + da_col<T>(c, ln);
-          if (ra < P.a && cb < P.b) P.s_out[so + (long long)ra * P.s_rs + (long long)cb * P.s_cs] = cut ? 0.f : s[i][c][e] * fade;
-        }
+          for (int e = 0; e < 4; ++e) s[i][c][e] = cut ? 0.f : s[i][c][e] * pw[1];
+    }
+    da_state<T, NS, BP, true>(s, P.s_out + so, P, dv0);
   }
 }
 
@@ -553,11 +630,12 @@ static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool
   const int ap = da_ap(A.pass[0].a, X.vec), nw = da_nw(A.pass[0].a, A.pass[0].b, X.vec);
   const long long units = (long long)A.m * A.heads * (state ? X.parts - 1 : X.parts), grid = (units + 7) / 8 * 8 * passes;
   PQN_REQUIRE(grid < (1ll << 31), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
-#define DA_GO(AP, NW, VEC)                                                                               \
-  if (ap == AP && nw == NW && (X.vec != 0) == VEC) {                                                     \
-    if (state) da_chunk_kernel<T, AP, NW, L, VEC, true><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);  \
-    else da_chunk_kernel<T, AP, NW, L, VEC, false><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);       \
-    return pqn_check_launch("pqn_decay_attn");                                                           \
+#define DA_GO(AP, NW, VEC)                                                                                                   \
+  if (ap == AP && nw == NW && (X.vec != 0) == VEC) {                                                                         \
+    if (state) da_chunk_kernel<T, AP, NW, L, VEC, DA_STATE><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);               \
+    else if (VEC && A.t_len <= L) da_chunk_kernel<T, AP, NW, L, true, DA_ONE><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes); \
+    else da_chunk_kernel<T, AP, NW, L, VEC, DA_MAIN><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);                      \
+    return pqn_check_launch("pqn_decay_attn");                                                                               \
   }
   DA_GO(32, 1, true)
   DA_GO(32, 2, true)

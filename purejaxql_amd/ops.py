@@ -96,7 +96,7 @@ def _last_contiguous(t: torch.Tensor, name: str, shape, dtype, index: int):
     """A tensor of this shape and type on GPU `index` whose last index is contiguous; other strides are the caller's."""
     if t.shape != shape or t.dtype != dtype or t.get_device() != index:
         raise ValueError(f"{name}: need {tuple(shape)} of {dtype} on cuda:{index}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    if not t.is_contiguous() and t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last index must be contiguous, strides are {tuple(t.stride())}")
 
 
@@ -133,27 +133,30 @@ _ATTN_DTYPES = (torch.float32, torch.bfloat16)
 def _attn_args(a, q, k, v, decay, state, reset, scale, step: bool):
     """Checks the common arguments and fills them into `a`; returns (lead shape, state shape)."""
     _on_gpu(q, "q", _ATTN_DTYPES)
-    if q.dim() != (3 if step else 4) or v.dim() != q.dim():
-        raise ValueError(f"q, v: need {'[M, H, D]' if step else '[T, M, H, D]'}, got {tuple(q.shape)}, {tuple(v.shape)}")
     shape, dt, dev = q.shape, q.dtype, q.get_device()
-    lead, dk, dv = shape[:-1], shape[-1], v.shape[-1]
+    if len(shape) != (3 if step else 4) or v.dim() != len(shape):
+        raise ValueError(f"q, v: need {'[M, H, D]' if step else '[T, M, H, D]'}, got {tuple(q.shape)}, {tuple(v.shape)}")
+    m, h, dk = shape[-3:]
+    lead, dv = shape[:-1], v.shape[-1]
     if not (0 < dk <= _lib.ATTN_MAX_D and 0 < dv <= _lib.ATTN_MAX_D):
         raise ValueError(f"q, v: head widths of 1 .. {_lib.ATTN_MAX_D}, got {dk} and {dv}")
     _last_contiguous(q, "q", shape, dt, dev)
     _last_contiguous(k, "k", shape, dt, dev)
     _last_contiguous(v, "v", lead + (dv,), dt, dev)
-    m, h = lead[-2:]
     st = (m, h, dk, dv)
     _exactly(decay, "decay", (h,), torch.float32, dev)
-    a.t_len, a.m, a.heads, a.dk, a.dv, a.dtype, a.scale = 1 if step else lead[0], m, h, dk, dv, _DTYPES[dt], scale
-    a.q, a.k, a.v, a.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
-    time = (0,) if step else ()      # a step has no time stride
-    a.q_stride, a.k_stride, a.v_stride = time + q.stride()[:-1], time + k.stride()[:-1], time + v.stride()[:-1]
+    (a.t_len, a.m, a.heads, a.dk, a.dv, a.dtype, a.scale, a.q, a.k, a.v, a.decay) = (
+        1 if step else shape[0], m, h, dk, dv, _DTYPES[dt], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr())
+    if step:                         # no time stride
+        a.q_stride, a.k_stride, a.v_stride = (0,) + q.stride()[:2], (0,) + k.stride()[:2], (0,) + v.stride()[:2]
+    else:
+        a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]
     if state is not None:
         _exactly(state, "state", st, torch.float32, dev)
         a.state_in = state.data_ptr()
     if reset is not None:
-        reset = _flags(reset)
+        if reset.dtype == torch.bool:
+            reset = reset.view(torch.uint8)
         _exactly(reset, "reset", lead[:-1], torch.uint8, dev)
         a.reset = reset.data_ptr()
     return lead, st
@@ -179,7 +182,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     lib = _lib.load()
     a = _lib.DecayAttnArgs()
     lead, st = _attn_args(a, q, k, v, decay, state, reset, scale, False)
-    out = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
     new = torch.empty(st, dtype=torch.float32, device=q.device) if want_state else None
     a.out, a.state_out = out.data_ptr(), _lib.ptr(new)
     ws = _attn_workspace(a, 0, q.device)  # noqa: F841 (held until the launch is enqueued)
@@ -196,7 +199,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
         raise ValueError("state: a step advances a state, pass zeros for a new one")
     a = _lib.DecayAttnArgs()
     lead, _ = _attn_args(a, q, k, v, decay, state, reset, scale, True)
-    out = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
     a.out, a.state_out = out.data_ptr(), a.state_in
     _enqueue(lib.pqn_decay_attn, a, q.get_device(), "pqn_decay_attn")
     return out
@@ -215,8 +218,7 @@ def decay_attention_grad(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     if dstate_out is not None:
         _exactly(dstate_out, "dstate_out", st, torch.float32, q.get_device())
     a.dout, a.dout_stride, a.dstate_out = dout.data_ptr(), dout.stride()[:-1], _lib.ptr(dstate_out)
-    dq, dk = (torch.empty(lead + (a.dk,), dtype=q.dtype, device=q.device) for _ in range(2))
-    dv = torch.empty(lead + (a.dv,), dtype=q.dtype, device=q.device)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     dstate = torch.empty(st, dtype=torch.float32, device=q.device) if state is not None else None
     a.dq, a.dk_out, a.dv_out, a.dstate_in = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dstate)
     ws = _attn_workspace(a, 1, q.device)  # noqa: F841
@@ -277,8 +279,8 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, gate: Optional[torch.Tensor]
     no h.  Returns (y, h or None)."""
     params = dict(zip(_NORM_PARAMS, (res_scale, post_scale, post_bias, pre_scale, pre_bias)))
     a, shape, keep = _norm_args(x, f, gate, gate_act, params, norm_type, post, pre, eps)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(shape, dtype=x.dtype, device=x.device) if pre else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = torch.empty_like(x, memory_format=torch.contiguous_format) if pre else None
     a.y, a.h = y.data_ptr(), _lib.ptr(h)
     _enqueue(_lib.load().pqn_residual_norm, a, x.get_device(), "pqn_residual_norm")
     return y, h
