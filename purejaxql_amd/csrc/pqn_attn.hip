@@ -42,13 +42,14 @@ PQN_D void da_state_io(float (&s)[RPT][4], float *mem, const da_pass &P, int r0,
 template <typename T, int RPT, bool VEC>
 __global__ __launch_bounds__(256) void da_recur_kernel(da_args A) {
   const da_pass &P = A.pass[blockIdx.y];
-  const int cb = (P.b + 31) >> 5;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= (long long)A.m * A.heads * cb) return;             // whole waves
+  const uint32_t cb = (P.b + 31) >> 5;                            // 1 .. 4; at most 2^28 (row, head) pairs: 32 bits
+  const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 6);
+  if (unit >= (uint32_t)A.m * (uint32_t)A.heads * cb) return;     // whole waves
   const int lane = threadIdx.x & 63;
-  const long long mh = unit / cb;
-  const int h = (int)(mh % A.heads), row = (int)(mh / A.heads);
-  const int c0 = (int)(unit % cb) * 32 + (lane & 7) * 4, r0 = lane >> 3;
+  const uint32_t mh32 = unit / cb;
+  const int row = (int)(mh32 / (uint32_t)A.heads), h = (int)(mh32 - (uint32_t)row * A.heads);
+  const long long mh = mh32;
+  const int c0 = (int)(unit - mh32 * cb) * 32 + (lane & 7) * 4, r0 = lane >> 3;
   const float decay = A.decay[h];
   const T *q = (const T *)P.q + row * P.qs[1] + h * P.qs[2];
   const T *k = (const T *)P.k + row * P.ks[1] + h * P.ks[2];
@@ -107,13 +108,13 @@ __global__ __launch_bounds__(256) void da_recur_kernel(da_args A) {
 
 // the parts' states in order: part p's own, from zero, becomes the state behind it, S_p = decay^len S_{p-1} + own unless it was cut
 __global__ __launch_bounds__(256) void da_join_kernel(da_args A, da_split X, int size) {
-  const long long block = blockIdx.x, per = (size + 1023) / 1024;
+  const uint32_t block = blockIdx.x, per = (uint32_t)(size + 1023) / 1024u;
   const long long mh = block / per;
   const int e = (int)(block % per) * 1024 + threadIdx.x * 4, pass = blockIdx.y;
   if (e >= size) return;
   float *p = X.state + pass * X.pass_stride + mh * (X.parts - 1) * (long long)size + e;
   const int *cut = X.cut + pass * X.cut_stride + mh * (X.parts - 1);
-  const float fade = (float)pqn_powi((double)A.decay[mh % A.heads], X.len);
+  const float fade = (float)pqn_powi((double)A.decay[(uint32_t)mh % (uint32_t)A.heads], X.len);
   f32x4_t s = *(const f32x4_t *)p;
   for (int i = 1; i < X.parts - 1; ++i) {
     const f32x4_t own = *(const f32x4_t *)(p + (long long)i * size);

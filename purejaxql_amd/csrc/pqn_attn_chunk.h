@@ -290,30 +290,32 @@ PQN_D void da_state(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) 
 // registers for twice the waves.
 enum { DA_MAIN, DA_STATE, DA_ONE };
 template <typename T, int AP, int NW, int L, bool VEC, int MODE>
-__global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void da_chunk_kernel(da_args A, da_split X, int passes) {
+__global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void da_chunk_kernel(da_args A, da_split X, int passes) {
   constexpr bool B16 = sizeof(T) == 2, STATE = MODE == DA_STATE;
   constexpr int NTHR = 64 * NW, BP = 32 * NW, KB = B16 ? 32 : 16, NF = AP / KB, NS = AP / 16, NJ = L / KB, NT = L / 16;
   constexpr int EV = 16 / (int)sizeof(T), PER = KB / 16, OUT = B16 ? 1 : 2;
   // The weights between the steps of a chunk: the waves share the tiles out and exchange them through LDS.  A wave alone keeps them in
   // its registers, where they lie as the next product's operand already.
   constexpr bool SHARE = NW > 1 && !STATE;
+  // ONE: Q takes V's place in LDS once V lies in registers, and more workgroups share a CU.
+  constexpr bool ALIAS = MODE == DA_ONE;
   typedef typename std::conditional<B16, bf16x8_t, f32x4_t>::type F;
   typedef DaTile<T, AP> TA;
   typedef DaTile<T, BP> TB;
   typedef DaTile<T, L> TP;
-  __shared__ __attribute__((aligned(16))) T Qs[STATE ? 8 : L * TA::LD], Ks[L * TA::LD], Vs[L * TB::LD], Ps[SHARE ? L * TP::LD : 8];
+  __shared__ __attribute__((aligned(16))) T Qs[STATE || ALIAS ? 8 : L * TA::LD], Ks[L * TA::LD], Ps[SHARE ? L * TP::LD : 8];
+  __shared__ __attribute__((aligned(16))) T Vs[L * (ALIAS && TA::LD > TB::LD ? TA::LD : TB::LD)];
+  T *const Q = ALIAS ? Vs : Qs;
   __shared__ __attribute__((aligned(16))) float pw[L + 4];
   __shared__ int bad[NW];
-  // the passes of one (row, head) meet in one XCD's L2: workgroups go round the 8 XCDs
-  const int parts = STATE ? X.parts - 1 : X.parts;
-  const long long nunits = (long long)A.m * A.heads * parts;
-  const long long block = blockIdx.x, unit = block / (8 * passes) * 8 + block % 8;
-  const int pass = (int)(block / 8 % passes);
-  if (unit >= nunits) return;
+  // the passes of one (row, head) meet in one XCD's L2: workgroups go round the 8 XCDs.  32-bit divisions: the launch has checked
+  const uint32_t parts = STATE ? X.parts - 1 : X.parts;
+  const uint32_t block = blockIdx.x, unit = block / (8u * passes) * 8u + block % 8u, pass = block / 8u % (uint32_t)passes;
+  if (unit >= (uint32_t)A.m * (uint32_t)A.heads * parts) return;
   const da_pass &P = A.pass[pass];
-  const long long mh = unit / parts;
-  const int part = (int)(unit % parts);
-  const int h = (int)(mh % A.heads), row = (int)(mh / A.heads);
+  const uint32_t mh32 = unit / parts;
+  const int part = (int)(unit - mh32 * parts), row = (int)(mh32 / (uint32_t)A.heads), h = (int)(mh32 - (uint32_t)row * A.heads);
+  const long long mh = mh32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, ln = lane & 15;
   const int t_first = part * X.len, t_end = min(A.t_len, t_first + X.len);
   DaLoad<T, AP, L, NTHR, VEC, false> rq, rk;
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
   for (int i = threadIdx.x; i <= L; i += NTHR) pw[i] = (float)pqn_powi(decay, i);   // every power rounded once
   if (P.a < AP || P.b < BP) {
     for (int i = threadIdx.x; i < L * TA::LD; i += NTHR) {
-      if constexpr (!STATE) Qs[i] = (T)0.f;
+      if constexpr (!STATE && !ALIAS) Qs[i] = (T)0.f;
       Ks[i] = (T)0.f;
     }
     for (int i = threadIdx.x; i < L * TB::LD; i += NTHR) Vs[i] = (T)0.f;
@@ -379,42 +381,34 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
   };
   // What depends on the decay alone for a whole chunk without an episode's end is made once: the weights between steps, of the state
   // on the outputs and of the steps on the state behind them.  `usual` says that they are those.
-  float wt[NT][NT][4], wc[NT], wu[NJ][EV];
+  float wt[NT][NT][4], wu[NJ][EV];
   bool usual = false, any_cut = false;
-  auto make_weights = [&](int n, unsigned long long cuts, int first) {
+  auto weigh_steps = [&](int tt, int jt, unsigned long long cuts) {      // of steps 16 jt + 4 g + e on step 16 tt + ln
+    const int t = 16 * tt + ln;
+    const unsigned long long upto = cuts & ((2ull << t) - 1ull);
+    const int from = upto ? 63 - __clzll(upto) : 0;                      // first step of t's episode in this chunk
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = 16 * jt + 4 * g + e;
+      wt[tt][jt][e] = j <= t && j >= from ? pw[max(t - j, 0)] * (P.s_scale * P.o_scale) : 0.f;
+    }
+  };
+  auto weigh_state = [&](int j, int n, unsigned long long cuts) {
     const int last_cut = cuts ? 63 - __clzll(cuts) : 0;
-    if constexpr (!STATE)
 #pragma unroll
-      for (int tt = 0; tt < NT; ++tt) {
-        const int t = 16 * tt + ln;
-        const unsigned long long upto = cuts & ((2ull << t) - 1ull);
-        const int from = upto ? 63 - __clzll(upto) : 0;      // first step of t's episode in this chunk
-        wc[tt] = pw[t + first] * P.o_scale;
-#pragma unroll
-        for (int jt = 0; jt <= tt; ++jt) {
-          if (SHARE && (tt * (tt + 1) / 2 + jt) % NW != wave) continue;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 16 * jt + 4 * g + e;
-            wt[tt][jt][e] = j <= t && j >= from ? pw[max(t - j, 0)] * (P.s_scale * P.o_scale) : 0.f;
-          }
-        }
-      }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int e = 0; e < EV; ++e) {
-        const int at = j * KB + 4 * g + (e & 3) + 16 * (e >> 2);
-        wu[j][e] = at < n && at >= last_cut ? pw[max(n - 1 - at, 0)] * P.s_scale : 0.f;
-      }
+    for (int e = 0; e < EV; ++e) {
+      const int at = j * KB + 4 * g + (e & 3) + 16 * (e >> 2);
+      wu[j][e] = at < n && at >= last_cut ? pw[max(n - 1 - at, 0)] * P.s_scale : 0.f;
+    }
   };
   __syncthreads();                                     // pw
   for (int t0 = t_first; t0 < t_end;) {
     int n = min(L, t_end - t0);
+    const int n_loaded = n;
     if (MODE == DA_ONE && t0 > 0) fetch(t0);           // only where a chunk is taken step by step
     rk.store(Ks, n);
     rv.store(Vs, n);
-    if constexpr (!STATE) rq.store(Qs, n);
+    if constexpr (!STATE && !ALIAS) rq.store(Qs, n);
     const bool nf = __any(rk.not_finite() || rv.not_finite());
     if (lane == 0) bad[wave] = nf;
     const unsigned long long cuts_all = __ballot(flag != 0 && lane < n && (t0 + lane > 0 || !P.late));
@@ -441,17 +435,38 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
     }
     const int first = (t0 == 0 && P.late) ? 0 : 1;     // borders up to and including step 0 of this chunk
     const bool plain = n == L && !cuts && first;
-    if (!(plain && usual)) make_weights(n, cuts, first);
+    if (MODE != DA_ONE && !(plain && usual)) {         // ONE makes them where they are needed
+      if constexpr (!STATE)
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+          for (int jt = 0; jt <= tt; ++jt)
+            if (!SHARE || (tt * (tt + 1) / 2 + jt) % NW == wave) weigh_steps(tt, jt, cuts);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) weigh_state(j, n, cuts);
+    }
     usual = plain;
-    // the weights of steps 16 jt + 4 g + e on step 16 tt + ln
     auto weights = [&](int tt, int jt, const F (&qf)[NF]) {
       f32x4_t p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int f = 0; f < NF; ++f) p = da_mfma(TA::template rows<F>(Ks, 16 * jt, f * KB), qf[f], p);
+      if constexpr (MODE == DA_ONE) weigh_steps(tt, jt, cuts);
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] *= wt[tt][jt][e];
       return p;
     };
+    F vf[NJ][2];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) TB::template pairs<F>(Vs, j * KB, dv0, vf[j]);
+    if constexpr (ALIAS) {
+      __syncthreads();                                 // V has been read
+      if (P.a < AP) {
+        for (int i = threadIdx.x; i < L * TA::LD; i += NTHR) Q[i] = (T)0.f;
+        __syncthreads();
+      }
+      rq.store(Q, n_loaded);
+      __syncthreads();
+    }
     if constexpr (SHARE) {
 #pragma unroll
       for (int tt = 0; tt < NT; ++tt) {
@@ -463,7 +478,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
           if (jt <= tt) {
             F qf[NF];
 #pragma unroll
-            for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Qs, 16 * tt, f * KB);
+            for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Q, 16 * tt, f * KB);
             p = weights(tt, jt, qf);
           }
           if constexpr (B16) {                                   // in the order of DaTile::cols
@@ -475,9 +490,6 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
       }
       __syncthreads();
     }
-    F vf[NJ][2];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) TB::template pairs<F>(Vs, j * KB, dv0, vf[j]);
     if constexpr (!STATE) {
       F sf[NF][2];
 #pragma unroll
@@ -493,12 +505,13 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
         if (16 * tt >= n) continue;
         F qf[NF];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Qs, 16 * tt, f * KB);
+        for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Q, 16 * tt, f * KB);
         f32x4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
           for (int c = 0; c < 2; ++c) o[c] = da_mfma(sf[f][c], qf[f], o[c]);
+        const float wc = pw[16 * tt + ln + first] * P.o_scale;
         if (cuts) {                                              // a choice, not a product: the state may be NaN
           const bool carried = (cuts & ((2ull << (16 * tt + ln)) - 1ull)) == 0;
 #pragma unroll
@@ -509,7 +522,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][e] *= wc[tt];
+          for (int e = 0; e < 4; ++e) o[c][e] *= wc;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if (j * KB >= 16 * (tt + 1)) continue;
@@ -559,6 +572,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 4 : 2) void d
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if (j * KB >= n) continue;
+      if constexpr (MODE == DA_ONE) weigh_state(j, n, cuts);
       constexpr int PIECES = B16 ? 3 : 1;
       F x[2][PIECES];                                  // w v is its pieces' sum exactly
 #pragma unroll
