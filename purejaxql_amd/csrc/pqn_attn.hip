@@ -151,8 +151,14 @@ static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
 #undef DA_GO
 }
 
-// One step at a time up to this length, chunks beyond.
-static constexpr int DA_RECUR_MAX = 4;
+// Windows of up to this many steps go step by step, longer ones by chunks.  Measured on both sides, us forward / gradient: 4096 x 4 heads
+// of 32, f32, 2 steps 30 / 90 against 46 / 113 by chunks, 4 steps 37 / 110 against 45 / 107, 6 steps 46 / 135 against 45 / 107; 1024 x 8
+// heads of 64, f32, 1 step 48 / 137 against 75 / 175; 1024 x 8 heads of 128, 1 step, f32 218 / 585 against 224 / 508, bf16 216 / 657
+// against 196 / 356, 2 steps bf16 257 / 806 against 213 / 366.
+static bool da_by_steps(const pqn_decay_attn_t *a, bool grad) {
+  const int w = a->dk > a->dv ? a->dk : a->dv;
+  return a->t_len <= (w <= 32 ? 4 : w <= 64 || (a->dtype == PQN_DTYPE_F32 && !grad) || (long long)a->m * a->heads < 2048 ? 1 : 0);
+}
 // The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
 // reading of k and v and a state written and read), as many as make DA_FILL waves.
 static constexpr int DA_MIN_PART = 64, DA_FILL = 2048;
@@ -164,7 +170,7 @@ static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int 
   const long long most = t_len / DA_MIN_PART;
   if (want > most) want = most;
   if (want < 1) want = 1;
-  X.len = (int)(((t_len + want - 1) / want + 63) / 64 * 64);      // whole chunks
+  X.len = (int)(((t_len + want - 1) / want + 31) / 32 * 32);      // whole chunks
   X.parts = X.len > 0 ? (t_len + X.len - 1) / X.len : 1;
   if (X.parts < 1) X.parts = 1;
   X.vec = vec;
@@ -262,7 +268,7 @@ static da_pass da_make(const pqn_decay_attn_t *a, const void *q, const int64_t *
 }
 
 extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
-  if (da_check(a, "pqn_decay_attn_workspace_bytes") != PQN_OK || a->t_len <= DA_RECUR_MAX || a->m == 0) return 0;
+  if (da_check(a, "pqn_decay_attn_workspace_bytes") != PQN_OK || da_by_steps(a, grad != 0) || a->m == 0) return 0;
   const long long rows = (long long)a->m * a->heads;
   const int vec = da_vec(a, grad);
   auto need = [&](int passes, int wa, int wb) { return da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb, vec), rows, passes, wa, wb); };
@@ -287,7 +293,7 @@ extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
   P.s_out = a->state_out;
   P.s_rs = a->dv;
   P.s_cs = 1;
-  if (a->t_len > DA_RECUR_MAX) {
+  if (!da_by_steps(a, false)) {
     const int vec = da_vec(a, 0);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 0) == 0, "pqn_decay_attn: NULL workspace");
     return da_run_chunks(A, 1, a->dtype, vec, a->workspace, (hipStream_t)stream);
@@ -318,7 +324,7 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   V.s_out = a->dstate_in;
   V.s_rs = a->dv;
   V.s_cs = 1;
-  if (a->t_len > DA_RECUR_MAX) {
+  if (!da_by_steps(a, true)) {
     const int vec = da_vec(a, 1);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
     if (a->dk == a->dv) return da_run_chunks(A, 3, a->dtype, vec, a->workspace, (hipStream_t)stream);

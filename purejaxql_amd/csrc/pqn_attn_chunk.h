@@ -116,11 +116,53 @@ struct DaTile {
   }
 };
 
-PQN_D f32x4_t da_mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-PQN_D f32x4_t da_mfma(f32x4_t a, f32x4_t b, f32x4_t c) {   // k = 4 (lane >> 4) + s in both operands
+// c += a b.  bf16 as asm, volatile and with the accumulator tied: the builtin lets the compiler give this instruction a destination
+// that partly overlaps its accumulator input, which has given results that differed between runs.  `s_nop 1` covers an operand that a
+// vector instruction has just written; a result is read by the next product of its chain or behind da_drain, and by nothing else.
+PQN_D void da_mfma(bf16x8_t a, bf16x8_t b, f32x4_t &c) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+PQN_D void da_mfma2(bf16x8_t a0, bf16x8_t a1, bf16x8_t b0, bf16x8_t b1, f32x4_t (&c)[2]) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %4, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %5, %1"
+               : "+v"(c[0]), "+v"(c[1])
+               : "v"(a0), "v"(a1), "v"(b0), "v"(b1));
+}
+// both of c by a and the three pieces of b
+PQN_D void da_mfma6(bf16x8_t a, const bf16x8_t (&b)[2][3], f32x4_t (&c)[2]) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %3, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %2, %6, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %2, %4, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %2, %7, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %2, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %2, %8, %1"
+               : "+v"(c[0]), "+v"(c[1])
+               : "v"(a), "v"(b[0][0]), "v"(b[0][1]), "v"(b[0][2]), "v"(b[1][0]), "v"(b[1][1]), "v"(b[1][2]));
+}
+// waits for the products before it and hands on their results: the one wait for all of x
+template <typename F, int N>
+PQN_D void da_drain(f32x4_t (&x)[N][2]) {
+  if constexpr (std::is_same<F, bf16x8_t>::value) {
+    asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x[0][0]), "+v"(x[0][1]));
+#pragma unroll
+    for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]));
+  }
+}
+template <typename F>
+PQN_D void da_drain(f32x4_t (&c)[2]) {
+  if constexpr (std::is_same<F, bf16x8_t>::value) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c[0]), "+v"(c[1]));
+}
+template <typename F>
+PQN_D void da_drain(f32x4_t &c) {
+  if constexpr (std::is_same<F, bf16x8_t>::value) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c));
+}
+// f32: the builtin, whose results the compiler waits for; k = 4 (lane >> 4) + s in both operands
+PQN_D void da_mfma(f32x4_t a, f32x4_t b, f32x4_t &c) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
-  return c;
+}
+PQN_D void da_mfma2(f32x4_t a0, f32x4_t a1, f32x4_t b0, f32x4_t b1, f32x4_t (&c)[2]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    c[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[s], b0[s], c[0], 0, 0, 0);
+    c[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[s], b1[s], c[1], 0, 0, 0);
+  }
 }
 
 // Rows of one (row, head)'s tensor on their way to a DaTile<T, W> of L rows.  load() only requests: every lane reads some row and column
@@ -169,6 +211,11 @@ struct DaLoad {
       for (int i = 0; i < N; ++i) r[i] = u32x4_t{0u, 0u, 0u, 0u};          // not_finite() looks at these too
       return;
     }
+    if (n < L) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (row0() + i * STEP >= n) r[i] = u32x4_t{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = row0() + i * STEP;
@@ -178,7 +225,6 @@ struct DaLoad {
         for (int e = 0; e < EV; ++e) v.v[e] = c + e < width ? v.v[e] : (T)0.f;
         r[i] = __builtin_bit_cast(u32x4_t, v);
       }
-      if (n < L && row >= n) r[i] = u32x4_t{0u, 0u, 0u, 0u};
       u32x4_t x = r[i];
       if constexpr (PAIRS && sizeof(T) == 2)
         x = u32x4_t{__builtin_amdgcn_perm(r[i][1], r[i][0], 0x05040100u), __builtin_amdgcn_perm(r[i][3], r[i][2], 0x05040100u),
@@ -229,27 +275,21 @@ struct da_split {       // the time axis in `parts` parts of `len` steps, one wo
 };
 
 // A wave's 32 columns of a state in memory, to or from its accumulators: two columns an access where they lie side by side, four rows
-// where those do (a transposed state).  WHOLE: every row and column exists, and the requests go out without a branch between them.
-template <typename T, int NS, bool WRITE, bool WHOLE>
-PQN_D void da_state_of(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) {
+// where those do (a transposed state).  Reads go out without a branch between them: a row or column that does not exist reads the
+// first and counts as zero.  WHOLE: all of them exist.
+template <typename T, int NS, bool WHOLE>
+PQN_D void da_state_in(f32x4_t (&s)[NS][2], const float *mem, const da_pass &P, int dv0) {
   const int lane = threadIdx.x & 63, g = lane >> 4, col = dv0 + 2 * (lane & 15);
-  typedef pqn_pack<float, 2> two;
-  typedef pqn_pack<float, 4> four;
   if (P.s_vec == 2) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = da_row<T>(i, 4 * g) + e;
-        if (WHOLE || (row < P.a && col < P.b)) {
-          two *p = (two *)(mem + (long long)row * P.s_rs + col);
-          if (WRITE) *p = two{{s[i][0][e], s[i][1][e]}};
-          else {
-            const two v = *p;
-            s[i][0][e] = v.v[0];
-            s[i][1][e] = v.v[1];
-          }
-        }
+        const bool in = WHOLE || (row < P.a && col < P.b);
+        const pqn_pack<float, 2> v = *(const pqn_pack<float, 2> *)(mem + (in ? (long long)row * P.s_rs + col : 0ll));
+        s[i][0][e] = in ? v.v[0] : 0.f;
+        s[i][1][e] = in ? v.v[1] : 0.f;
       }
   } else if (P.s_vec == 4) {
 #pragma unroll
@@ -257,11 +297,9 @@ PQN_D void da_state_of(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int row = da_row<T>(i, 4 * g);
-        if (WHOLE || (row < P.a && col + c < P.b)) {
-          four *p = (four *)(mem + row + (long long)(col + c) * P.s_cs);
-          if (WRITE) *p = __builtin_bit_cast(four, s[i][c]);
-          else s[i][c] = __builtin_bit_cast(f32x4_t, *p);
-        }
+        const bool in = WHOLE || (row < P.a && col + c < P.b);
+        const f32x4_t v = *(const f32x4_t *)(mem + (in ? row + (long long)(col + c) * P.s_cs : 0ll));
+        s[i][c] = in ? v : f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
   } else {
 #pragma unroll
@@ -271,18 +309,31 @@ PQN_D void da_state_of(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = da_row<T>(i, 4 * g) + e;
-          if (row < P.a && col + c < P.b) {
-            float *p = mem + (long long)row * P.s_rs + (long long)(col + c) * P.s_cs;
-            if (WRITE) *p = s[i][c][e];
-            else s[i][c][e] = *p;
-          }
+          const bool in = WHOLE || (row < P.a && col + c < P.b);
+          const float v = mem[in ? (long long)row * P.s_rs + (long long)(col + c) * P.s_cs : 0ll];
+          s[i][c][e] = in ? v : 0.f;
         }
   }
 }
-template <typename T, int NS, int BP, bool WRITE>
-PQN_D void da_state(f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) {
-  if (P.a == 16 * NS && P.b == BP) da_state_of<T, NS, WRITE, true>(s, mem, P, dv0);
-  else da_state_of<T, NS, WRITE, false>(s, mem, P, dv0);
+template <typename T, int NS, bool WHOLE>
+PQN_D void da_state_out(const f32x4_t (&s)[NS][2], float *mem, const da_pass &P, int dv0) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = dv0 + 2 * (lane & 15);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int row = da_row<T>(i, 4 * g);
+    if (P.s_vec == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (WHOLE || (row + e < P.a && col < P.b))
+          *(pqn_pack<float, 2> *)(mem + (long long)(row + e) * P.s_rs + col) = pqn_pack<float, 2>{{s[i][0][e], s[i][1][e]}};
+    } else {                       // a state that goes out is never transposed
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row + e < P.a && col + c < P.b) mem[(long long)(row + e) * P.s_rs + (long long)(col + c) * P.s_cs] = s[i][c][e];
+    }
+  }
 }
 
 // What a workgroup does: MAIN a part of the time axis; STATE only what the part adds to the state (its first step onwards from zero, the
@@ -339,9 +390,10 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
     for (int c = 0; c < 2; ++c) s[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const long long so = mh * ((long long)P.a * P.b);
   const int dv0 = 32 * wave;
+  const bool whole = P.a == AP && P.b == BP;
   float *xs = X.state + pass * X.pass_stride + (mh * (X.parts - 1)) * (long long)(AP * BP) + wave * (AP * 32) + lane * 4;
   if (part == 0) {
-    if (P.s_in) da_state<T, NS, BP, false>(s, const_cast<float *>(P.s_in) + so, P, dv0);
+    if (P.s_in) whole ? da_state_in<T, NS, true>(s, P.s_in + so, P, dv0) : da_state_in<T, NS, false>(s, P.s_in + so, P, dv0);
   } else if constexpr (!STATE) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
@@ -449,7 +501,8 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
     auto weights = [&](int tt, int jt, const F (&qf)[NF]) {
       f32x4_t p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int f = 0; f < NF; ++f) p = da_mfma(TA::template rows<F>(Ks, 16 * jt, f * KB), qf[f], p);
+      for (int f = 0; f < NF; ++f) da_mfma(TA::template rows<F>(Ks, 16 * jt, f * KB), qf[f], p);
+      da_drain<F>(p);
       if constexpr (MODE == DA_ONE) weigh_steps(tt, jt, cuts);
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] *= wt[tt][jt][e];
@@ -508,9 +561,8 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
         for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Q, 16 * tt, f * KB);
         f32x4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) o[c] = da_mfma(sf[f][c], qf[f], o[c]);
+        for (int f = 0; f < NF; ++f) da_mfma2(sf[f][0], sf[f][1], qf[f], qf[f], o);
+        da_drain<F>(o);
         const float wc = pw[16 * tt + ln + first] * P.o_scale;
         if (cuts) {                                              // a choice, not a product: the state may be NaN
           const bool carried = (cuts & ((2ull << (16 * tt + ln)) - 1ull)) == 0;
@@ -539,9 +591,9 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
             }
             pf = __builtin_bit_cast(F, u);
           } else pf = weights(tt, j, qf);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) o[c] = da_mfma(vf[j][c], pf, o[c]);
+          da_mfma2(vf[j][0], vf[j][1], pf, pf, o);
         }
+        da_drain<F>(o);
         if constexpr (B16)
           held[tt][0] = __builtin_bit_cast(Out, (u32x4_t{da_pair(o[0][0], o[1][0]), da_pair(o[0][1], o[1][1]), da_pair(o[0][2], o[1][2]),
                                                          da_pair(o[0][3], o[1][3])}));
@@ -599,12 +651,11 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const F kf = TA::template cols<F>(Ks, j * KB, i);
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) s[i][c] = da_mfma(kf, x[c][k], s[i][c]);
+        if constexpr (B16) da_mfma6(kf, x, s[i]);
+        else da_mfma2(kf, kf, x[0][0], x[1][0], s[i]);
       }
     }
+    da_drain<F>(s);
     t0 += n;
     __syncthreads();                                   // the chunk has been read
   }
@@ -625,7 +676,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[i][c][e] = cut ? 0.f : s[i][c][e] * pw[1];
     }
-    da_state<T, NS, BP, true>(s, P.s_out + so, P, dv0);
+    whole ? da_state_out<T, NS, true>(s, P.s_out + so, P, dv0) : da_state_out<T, NS, false>(s, P.s_out + so, P, dv0);
   }
 }
 
