@@ -27,7 +27,12 @@ struct rn_args {
   long long dys, dhs;
   void *dx, *df, *dg;
   float *partials;                        // [gridDim.x][RN_PARAMS][d]
+  struct RnStat *stats;                   // rows of more than RN_WIDE columns: [n]
 };
+struct RnStat {                           // of a row: f's and y's mean and 1 / sqrt(var + eps); mean(dh' u), mean(dh') of y's norm
+  float mean_f, inv_f, mean_y, inv_y, a, b;
+};
+static constexpr int RN_WIDE = 4096;
 enum { RN_RES = 0, RN_POST_SCALE, RN_POST_BIAS, RN_PRE_SCALE, RN_PRE_BIAS, RN_PARAMS };
 
 // K sums at once over the NT threads that hold a row, the same in every thread.  `turn` alternates between two places in LDS, so
@@ -95,7 +100,7 @@ struct RnRow {
     }
   }
   // r -> (r - mean) * inv in place; returns inv = 1 / sqrt(var + eps).  rms: mean = 0
-  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds, int &turn) {
+  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds, int &turn, float *mean_out = nullptr) {
     const float per = 1.0f / (float)d;
     if (!rms) {
       float s[1] = {0.f};
@@ -103,6 +108,7 @@ struct RnRow {
       for (int e = 0; e < E; ++e) s[0] += r[e];
       rn_row_sum<NT>(s, lds, turn);
       const float mean = s[0] * per;
+      if (mean_out) *mean_out = mean;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const bool in = col(lane, i) < d;
@@ -119,8 +125,9 @@ struct RnRow {
     for (int e = 0; e < E; ++e) r[e] *= inv;
     return inv;
   }
-  // gradient of the normalisation: dz -> d(input), z = the normalised row
-  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds, int &turn) {
+  // gradient of the normalisation: dz -> d(input), z = the normalised row; ab: mean(dz z), mean(dz)
+  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds, int &turn,
+                                   float *ab = nullptr) {
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -129,6 +136,10 @@ struct RnRow {
     }
     rn_row_sum<NT>(s, lds, turn);
     const float per = 1.0f / (float)d, a = s[0] * per, b = rms ? 0.f : s[1] * per;
+    if (ab) {
+      ab[0] = a;
+      ab[1] = b;
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool in = col(lane, i) < d;
@@ -158,7 +169,7 @@ template <typename T, int NT, int VW, int NV, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
   using Row = RnRow<T, NT, VW, NV>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
-  constexpr bool KEEP = E <= 8;           // the parameters stay in registers
+  constexpr bool KEEP = NT < 1024;        // the parameters stay in registers, and the next row is in flight
   __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63;
   const int d = A.d;
@@ -172,24 +183,30 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
     if constexpr (ACT != PQN_GATE_NONE) Row::fetch(fg, A.g, r * A.gs, d, lane);
     Row::fetch(fx, A.x, r * A.xs, d, lane);
   };
-  fetch(row);
   float ps[E], pb[E], rs[E], qs[E], qb[E];
-  auto params = [&]() {
+  auto params_in = [&]() {
     Row::param(ps, A.post_scale, 1.f, d, lane);
     Row::param(pb, A.post_bias, 0.f, d, lane);
     Row::param(rs, A.res_scale, 1.f, d, lane);
+  };
+  auto params_out = [&]() {
     Row::param(qs, A.pre_scale, 1.f, d, lane);
     Row::param(qb, A.pre_bias, 0.f, d, lane);
   };
-  if constexpr (KEEP) params();
+  if constexpr (KEEP) {
+    fetch(row);
+    params_in();
+    params_out();
+  }
   for (; row < A.n; row += step) {
     float z[E], y[E], g[E];
+    if constexpr (!KEEP) fetch(row);
     Row::open(z, ff, d, lane);
     Row::open(y, fx, d, lane);
     if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
-    if (row + step < A.n) fetch(row + step);
-    if constexpr (!KEEP) params();
+    if (KEEP && row + step < A.n) fetch(row + step);
     if (A.has_post) Row::normalise(z, A.rms, A.eps, d, lane, lds, turn);
+    if constexpr (!KEEP) params_in();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float act, slope;
@@ -199,6 +216,7 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
     Row::store(A.y, row * d, y, d, lane);
     if (A.has_pre) {
       Row::normalise(y, A.rms, A.eps, d, lane, lds, turn);
+      if constexpr (!KEEP) params_out();
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = fmaf(y[e], qs[e], qb[e]);
       Row::store(A.h, row * d, y, d, lane);
@@ -207,22 +225,24 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
 }
 
 // The parameter gradients are summed over a thread's rows in registers and leave the workgroup as one partial row per parameter,
-// summed in a fixed order by rn_param_kernel (the same result in every run).
+// summed in a fixed order by rn_param_kernel (the same result in every run).  NT = 1024 has no registers for the sums: it leaves the
+// row's statistics instead, and rn_sums_kernel reads the rows a second time.
 template <typename T, int NT, int VW, int NV, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
   using Row = RnRow<T, NT, VW, NV>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
-  constexpr bool KEEP = E <= 8;
+  constexpr bool KEEP = NT < 1024, SUMS = KEEP;
   __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   __shared__ float fold[NT > 64 ? 1 : 3 * 64 * E];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63, wave = NT > 64 ? 0 : threadIdx.x >> 6;
   const int d = A.d;
   int turn = 0;
-  float sum[RN_PARAMS][E];
+  float sum[SUMS ? RN_PARAMS : 1][E];
+  if constexpr (SUMS)
 #pragma unroll
-  for (int k = 0; k < RN_PARAMS; ++k)
+    for (int k = 0; k < RN_PARAMS; ++k)
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum[k][e] = 0.f;
+      for (int e = 0; e < E; ++e) sum[k][e] = 0.f;
   long long row = (long long)blockIdx.x * RPB + wave;
   const long long step = (long long)gridDim.x * RPB;
   typename Row::Pack fx[NV], ff[NV], fg[NV], fy[NV], fh[NV];
@@ -233,17 +253,20 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
     if (A.dh) Row::fetch(fh, A.dh, r * A.dhs, d, lane);
     if (A.dy) Row::fetch(fy, A.dy, r * A.dys, d, lane);
   };
-  if (row < A.n) fetch(row);
+  if (KEEP && row < A.n) fetch(row);
   float ps[E], pb[E], rs[E], qs[E];
   auto params = [&]() {
     Row::param(ps, A.post_scale, 1.f, d, lane);
     Row::param(pb, A.post_bias, 0.f, d, lane);
     Row::param(rs, A.res_scale, 1.f, d, lane);
-    Row::param(qs, A.pre_scale, 1.f, d, lane);
   };
-  if constexpr (KEEP) params();
+  if constexpr (KEEP) {
+    params();
+    Row::param(qs, A.pre_scale, 1.f, d, lane);
+  }
   for (; row < A.n; row += step) {
     float z[E], y[E], e_[E], g[E], dh[E];
+    if constexpr (!KEEP) fetch(row);
     Row::open(z, ff, d, lane);
     Row::open(y, fx, d, lane);
     if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
@@ -252,45 +275,56 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
     else
 #pragma unroll
       for (int e = 0; e < E; ++e) e_[e] = 0.f;
-    if (row + step < A.n) fetch(row + step);
+    if (KEEP && row + step < A.n) fetch(row + step);
     if constexpr (!KEEP) params();
     float inv_f = 1.f, act[E], slope[E];
-    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds, turn);
+    RnStat st = {0.f, 1.f, 0.f, 1.f, 0.f, 0.f};
+    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds, turn, &st.mean_f);
+    st.inv_f = inv_f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       rn_act(ACT, g[e], act[e], slope[e]);
       y[e] = fmaf(rs[e], act[e] * fmaf(z[e], ps[e], pb[e]), y[e]);
     }
     if (A.dh) {
-      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds, turn);
+      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds, turn, &st.mean_y);
+      st.inv_y = inv_y;
+      if constexpr (!KEEP) Row::param(qs, A.pre_scale, 1.f, d, lane);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        sum[RN_PRE_SCALE][e] = fmaf(dh[e], y[e], sum[RN_PRE_SCALE][e]);
-        sum[RN_PRE_BIAS][e] += dh[e];
+        if constexpr (SUMS) {
+          sum[RN_PRE_SCALE][e] = fmaf(dh[e], y[e], sum[RN_PRE_SCALE][e]);
+          sum[RN_PRE_BIAS][e] += dh[e];
+        }
         dh[e] *= qs[e];
       }
-      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds, turn);
+      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds, turn, &st.a);
 #pragma unroll
       for (int e = 0; e < E; ++e) e_[e] += dh[e];
     }
     Row::store(A.dx, row * d, e_, d, lane);
+    if constexpr (!KEEP) params();          // read and made again rather than held
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float n = fmaf(z[e], ps[e], pb[e]);
-      sum[RN_RES][e] = fmaf(e_[e], act[e] * n, sum[RN_RES][e]);
-      const float da = e_[e] * rs[e], dn = da * act[e];
+      if constexpr (!KEEP) rn_act(ACT, g[e], act[e], slope[e]);
+      const float n = fmaf(z[e], ps[e], pb[e]), da = e_[e] * rs[e], dn = da * act[e];
       if constexpr (ACT != PQN_GATE_NONE) g[e] = da * n * slope[e];
-      sum[RN_POST_SCALE][e] = fmaf(dn, z[e], sum[RN_POST_SCALE][e]);
-      sum[RN_POST_BIAS][e] += dn;
+      if constexpr (SUMS) {
+        sum[RN_RES][e] = fmaf(e_[e], act[e] * n, sum[RN_RES][e]);
+        sum[RN_POST_SCALE][e] = fmaf(dn, z[e], sum[RN_POST_SCALE][e]);
+        sum[RN_POST_BIAS][e] += dn;
+      }
       e_[e] = dn * ps[e];
     }
     if constexpr (ACT != PQN_GATE_NONE) Row::store(A.dg, row * d, g, d, lane);
     if (A.has_post) Row::normalise_back(e_, z, inv_f, A.rms, d, lane, lds, turn);
     Row::store(A.df, row * d, e_, d, lane);
+    if (!SUMS && threadIdx.x == 0) A.stats[row] = st;
   }
+  if constexpr (!SUMS) return;
   float *out = A.partials + (size_t)blockIdx.x * RN_PARAMS * d;
 #pragma unroll
-  for (int k = 0; k < RN_PARAMS; ++k) {
+  for (int k = 0; k < (SUMS ? RN_PARAMS : 0); ++k) {
     if constexpr (NT == 64) {              // waves 1 .. 3 hand their sums to wave 0
       __syncthreads();
       if (wave > 0)
@@ -309,6 +343,57 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
         if (c < d) pqn_store<float, VW>(out + (size_t)k * d + c, sum[k] + i * VW);
       }
   }
+}
+
+// The parameter gradients of wide rows: a thread's VW columns over the rows of its slice, from the statistics that rn_bwd_kernel left.
+template <typename T, int VW, int ACT>
+__global__ __launch_bounds__(256) void rn_sums_kernel(rn_args A) {
+  const int d = A.d, c = (blockIdx.x * 256 + threadIdx.x) * VW;
+  if (c >= d) return;
+  float ps[VW], pb[VW], rs[VW], qs[VW], sum[RN_PARAMS][VW];
+  auto param = [&](float (&r)[VW], const float *p, float absent) {
+#pragma unroll
+    for (int e = 0; e < VW; ++e) r[e] = p ? p[c + e] : absent;
+  };
+  param(ps, A.post_scale, 1.f);
+  param(pb, A.post_bias, 0.f);
+  param(rs, A.res_scale, 1.f);
+  param(qs, A.pre_scale, 1.f);
+#pragma unroll
+  for (int k = 0; k < RN_PARAMS; ++k)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) sum[k][e] = 0.f;
+  for (long long row = blockIdx.y; row < A.n; row += gridDim.y) {
+    float x[VW], f[VW], g[VW], dy[VW], dh[VW];
+    pqn_load<T, VW>(f, (const T *)A.f + row * A.fs + c);
+    pqn_load<T, VW>(x, (const T *)A.x + row * A.xs + c);
+    if constexpr (ACT != PQN_GATE_NONE) pqn_load<T, VW>(g, (const T *)A.g + row * A.gs + c);
+    if (A.dh) pqn_load<T, VW>(dh, (const T *)A.dh + row * A.dhs + c);
+    if (A.dy) pqn_load<T, VW>(dy, (const T *)A.dy + row * A.dys + c);
+    const RnStat st = A.stats[row];
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      float act, slope;
+      rn_act(ACT, g[e], act, slope);
+      const float z = (f[e] - st.mean_f) * st.inv_f, n = fmaf(z, ps[e], pb[e]);
+      float grad = A.dy ? dy[e] : 0.f;
+      if (A.dh) {
+        const float u = (fmaf(rs[e], act * n, x[e]) - st.mean_y) * st.inv_y;
+        sum[RN_PRE_SCALE][e] = fmaf(dh[e], u, sum[RN_PRE_SCALE][e]);
+        sum[RN_PRE_BIAS][e] += dh[e];
+        grad += (fmaf(-u, st.a, dh[e] * qs[e]) - st.b) * st.inv_y;
+      }
+      const float dn = grad * rs[e] * act;
+      sum[RN_RES][e] = fmaf(grad, act * n, sum[RN_RES][e]);
+      sum[RN_POST_SCALE][e] = fmaf(dn, z, sum[RN_POST_SCALE][e]);
+      sum[RN_POST_BIAS][e] += dn;
+    }
+  }
+  float *out = A.partials + (size_t)blockIdx.y * RN_PARAMS * d + c;
+#pragma unroll
+  for (int k = 0; k < RN_PARAMS; ++k)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) out[(size_t)k * d + e] = sum[k][e];
 }
 
 // column sums of the partials: 64 columns x 16 row groups per workgroup, fixed order
@@ -332,17 +417,19 @@ __global__ __launch_bounds__(1024) void rn_param_kernel(const float *__restrict_
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// Threads per row: as few as hold it at 8 columns each -- a wave up to 512 columns (no barrier then), then 128 to 512 threads, which
-// hold the widest rows at 16 columns each.  Vector accesses of up to 16 B where width, strides and pointers allow them, else one
-// element per lane and access.
-static int rn_threads(int d) { return d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : 512; }
+// Threads per row: as few as hold it at 8 columns each -- a wave up to 512 columns (no barrier then), then 128 to 1024 threads, the
+// last without the registers for parameters and a row in flight.  Vector accesses of up to 16 B where width, strides and pointers allow
+// them, else one element per lane and access.
+static int rn_threads(int d) { return d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024; }
 // Workgroups: enough to fill the chip (8 waves per SIMD asked for by the forward, 2 by the gradient with its sums in registers), each
-// walking over its rows; the gradient leaves a partial row per workgroup and parameter.
+// walking over its rows; the gradient leaves a partial row per workgroup and parameter, wide rows one per slice of rn_sums_kernel.
 static int rn_blocks(long long n, int d, bool grad) {
   const int nt = rn_threads(d);
-  const long long want = nt == 64 ? (n + 3) / 4 : n, cap = grad ? (nt <= 128 ? 1024 : 512) : 65536 / (nt == 64 ? 256 : nt) * 8;
+  const long long want = nt == 64 ? (n + 3) / 4 : n;
+  const long long cap = grad && nt < 1024 ? (nt <= 128 ? 1024 : 512) : 65536 / (nt == 64 ? 256 : nt) * 8;
   return (int)(want < cap ? want : cap);
 }
+static int rn_parts(long long n, int d) { return d <= RN_WIDE ? rn_blocks(n, d, true) : (int)(n < 256 ? n : 256); }
 
 template <typename T, bool BWD, int ACT>
 static int rn_launch_act(const rn_args &A, bool vec, hipStream_t st) {
@@ -361,14 +448,32 @@ static int rn_launch_act(const rn_args &A, bool vec, hipStream_t st) {
     if (nt == 64) RN_GO(64, VW, 8 / VW);
     if (nt == 128) RN_GO(128, VW, 8 / VW);
     if (nt == 256) RN_GO(256, VW, 8 / VW);
-    if (A.d <= 4096) RN_GO(512, VW, 8 / VW);
-    RN_GO(512, VW, 16 / VW);
+    if (nt == 512) RN_GO(512, VW, 8 / VW);
+    RN_GO(1024, VW, 8 / VW);
   }
+  if (A.d <= 128) RN_GO(64, 1, 2);
   if (nt == 64) RN_GO(64, 1, 8);
-  if (nt <= 256) RN_GO(256, 1, 8);
-  if (A.d <= 4096) RN_GO(512, 1, 8);
-  RN_GO(512, 1, 16);
+  if (nt == 128) RN_GO(128, 1, 8);
+  if (nt == 256) RN_GO(256, 1, 8);
+  if (nt == 512) RN_GO(512, 1, 8);
+  RN_GO(1024, 1, 8);
 #undef RN_GO
+}
+template <typename T>
+static int rn_launch_sums(const rn_args &A, bool vec, hipStream_t st) {
+  constexpr int VW = 16 / (int)sizeof(T);
+  const int w = vec ? VW : 1;
+  const dim3 grid((A.d + 256 * w - 1) / (256 * w), rn_parts(A.n, A.d));
+#define RN_GO(ACT)                                                       \
+  if (A.gate_act == ACT) {                                               \
+    if (vec) rn_sums_kernel<T, VW, ACT><<<grid, 256, 0, st>>>(A);        \
+    else rn_sums_kernel<T, 1, ACT><<<grid, 256, 0, st>>>(A);             \
+  }
+  RN_GO(PQN_GATE_NONE)
+  RN_GO(PQN_GATE_SIGMOID)
+  RN_GO(PQN_GATE_SILU)
+#undef RN_GO
+  return pqn_check_launch("pqn_residual_norm_grad");
 }
 template <typename T, bool BWD>
 static int rn_launch(const rn_args &A, bool vec, hipStream_t st) {
@@ -421,6 +526,7 @@ static rn_args rn_fill(const pqn_residual_norm_t *a) {
   A.dy = a->dy; A.dh = a->dh; A.dys = a->dy_stride; A.dhs = a->dh_stride;
   A.dx = a->dx; A.df = a->df; A.dg = a->dgate;
   A.partials = a->workspace;
+  A.stats = (RnStat *)(a->workspace + (a->n > 0 ? (int64_t)rn_parts(a->n, a->d) * RN_PARAMS * a->d : 0));
   return A;
 }
 
@@ -437,7 +543,7 @@ extern "C" int pqn_residual_norm(const pqn_residual_norm_t *a, void *stream) {
 
 extern "C" int64_t pqn_residual_norm_workspace_floats(int64_t n, int32_t d) {
   if (n <= 0 || d <= 0 || d > RN_MAX_D) return 0;
-  return (int64_t)rn_blocks(n, d, true) * RN_PARAMS * d;
+  return (int64_t)rn_parts(n, d) * RN_PARAMS * d + (d > RN_WIDE ? n * (int64_t)(sizeof(RnStat) / 4) : 0);
 }
 
 extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream) {
@@ -454,11 +560,14 @@ extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream
     const void *ptrs[] = {a->x, a->f, a->gate, a->dy, a->dh, a->dx, a->df, a->dgate};
     const int64_t strides[] = {a->x_stride, a->f_stride, a->gate ? a->gate_stride : 0, a->dy ? a->dy_stride : 0, a->dh ? a->dh_stride : 0};
     const bool vec = rn_vec_ok(a, ptrs, 8, strides, 5);
-    const int r = pqn_with_dtype(a->dtype, [&](auto t) { return rn_launch<decltype(t), true>(rn_fill(a), vec, (hipStream_t)stream); });
+    const int r = pqn_with_dtype(a->dtype, [&](auto t) {
+      const int rc = rn_launch<decltype(t), true>(rn_fill(a), vec, (hipStream_t)stream);
+      return rc == PQN_OK && any && a->d > RN_WIDE ? rn_launch_sums<decltype(t)>(rn_fill(a), vec, (hipStream_t)stream) : rc;
+    });
     if (r != PQN_OK) return r;
   }
   if (!any) return PQN_OK;
-  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_blocks(a->n, a->d, true) : 0,
+  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_parts(a->n, a->d) : 0,
                                                                                       a->d, out);
   return pqn_check_launch("pqn_residual_norm_grad");
 }
