@@ -42,7 +42,7 @@ def main():
         with tempfile.TemporaryDirectory() as td:
             out = os.path.join(td, "x.s")
             extra = ["-fno-slp-vectorize"] if os.path.basename(f) == "pqn_qnet_pos.hip" else []     # as the Makefile builds it
-            subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", *extra,
+            subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *extra,
                             "--cuda-device-only", "-S", f, "-o", out], check=True, cwd=CSRC, stderr=subprocess.DEVNULL)
             hits = scan(out)
             if os.path.basename(f) == "pqn_qnet_pos.hip":
