@@ -225,6 +225,7 @@ static int da_check(const pqn_decay_attn_t *a, const char *who) {
   PQN_REQUIRE(a, "%s: NULL argument block", who);
   PQN_REQUIRE(a->dtype == PQN_DTYPE_F32 || a->dtype == PQN_DTYPE_BF16, "%s: dtype %d is neither f32 nor bf16", who, a->dtype);
   PQN_REQUIRE(a->t_len >= 0 && a->m >= 0 && a->heads > 0, "%s: t_len, m must be >= 0 and heads > 0 (%d, %d, %d)", who, a->t_len, a->m, a->heads);
+  PQN_REQUIRE(a->t_len <= (1 << 30), "%s: up to 2^30 steps (t_len=%d)", who, a->t_len);
   PQN_REQUIRE(a->dk > 0 && a->dk <= PQN_ATTN_MAX_D && a->dv > 0 && a->dv <= PQN_ATTN_MAX_D, "%s: head widths of 1 .. %d (dk=%d dv=%d)", who,
               PQN_ATTN_MAX_D, a->dk, a->dv);
   PQN_REQUIRE((long long)a->m * a->heads <= (1ll << 28), "%s: up to 2^28 (row, head) pairs (m=%d heads=%d)", who, a->m, a->heads);
@@ -270,8 +271,12 @@ static da_pass da_make(const pqn_decay_attn_t *a, const void *q, const int64_t *
 extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int32_t grad) {
   if (da_check(a, "pqn_decay_attn_workspace_bytes") != PQN_OK || da_by_steps(a, grad != 0) || a->m == 0) return 0;
   const long long rows = (long long)a->m * a->heads;
-  const int vec = da_vec(a, grad);
-  auto need = [&](int passes, int wa, int wb) { return da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb, vec), rows, passes, wa, wb); };
+  // of both forms, so that the answer goes by sizes alone and not by the tensors' addresses and strides
+  auto need = [&](int passes, int wa, int wb) {
+    const long long x = da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb, 0), rows, passes, wa, wb);
+    const long long y = da_ws_bytes(da_cut(a->t_len, rows, passes, wa, wb, 1), rows, passes, wa, wb);
+    return x > y ? x : y;
+  };
   if (!grad) return need(1, a->dk, a->dv);
   if (a->dk == a->dv) return need(3, a->dk, a->dv);
   const long long one = need(2, a->dv, a->dk), two = need(1, a->dk, a->dv);         // one after the other

@@ -505,7 +505,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
       da_drain<F>(p);
       if constexpr (MODE == DA_ONE) weigh_steps(tt, jt, cuts);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] *= wt[tt][jt][e];
+      for (int e = 0; e < 4; ++e) p[e] = wt[tt][jt][e] == 0.f ? 0.f : p[e] * wt[tt][jt][e];   // a later step's product may overflow
       return p;
     };
     F vf[NJ][2];

@@ -5,7 +5,7 @@ Tolerances, derived before the first run, with u = 2^-24 (f32's half step) and h
   attention, f32: every term passes at most 2 roundings per step it is carried (decay, addition; in the chunked form fewer) and one per
     product and addition over the head width: (2 T + Dk + Dv + 16) u abs.
   attention, bf16: the weights between two steps of a chunk, or the state, are an operand of a matrix product in bf16: h abs, and what
-    is added to a state is split in two bf16 pieces: h^2 abs; the output is rounded once: h |ref|.  States are f32: no last term.
+    is added to a state is split in bf16 pieces, at least two: h^2 abs; the output is rounded once: h |ref|.  States are f32: no last term.
   norms: the terms of a row's sums are of one row: (D + 32) u of the largest intermediate; see rn_tol.
   log probabilities: x = logit / temperature has |x| u, the exponent of e^(x - m) as much again, the sum A u at most; see lp_tol.
 """
@@ -174,6 +174,76 @@ def test_steps_in_place_are_the_window(gpu, dtype, m, h, dk, dv):
     n = (2 * t + dk + dv + 16) * U
     _close(torch.stack(outs), r_out, (n + h_ + h_ * h_) * a_out + h_ * r_out.abs(), "out")
     _close(state, r_new, (n + h_ * h_) * a_new + 1e-30, "state")
+
+
+@pytest.mark.parametrize("dk,dv,m,h", [(128, 128, 525, 4), (96, 72, 300, 7), (8, 128, 1100, 2), (67, 128, 130, 16)])
+def test_steps_in_place_of_many_wide_rows(gpu, dk, dv, m, h):
+    """Steps of so many wide bf16 rows that they go by another kernel than those of few: still the window's outputs and state."""
+    from purejaxql_amd import ops
+    t = 3
+    x = _attn_inputs(gpu, t, m, h, dk, dv, BF16, 22, True, 0.3)
+    state = x["state"].clone()
+    outs = [ops.decay_attention_step(x["q"][i], x["k"][i], x["v"][i], x["decay"], state, reset=x["reset"][i], scale=0.3) for i in range(t)]
+    args = [x[n].double() for n in ("q", "k", "v", "decay", "state")]
+    r_out, r_new = ref.attention(*args, x["reset"], 0.3)
+    a_out, a_new = ref.attention(*[a.abs() for a in args], x["reset"], 0.3)
+    n, h_ = (2 * t + dk + dv + 16) * U, HALF[BF16]
+    _close(torch.stack(outs), r_out, (n + h_ + h_ * h_) * a_out + h_ * r_out.abs(), "out")
+    _close(state, r_new, (n + h_ * h_) * a_new + 1e-30, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t,d", [(20, 32), (75, 64), (40, 128)])
+def test_products_that_overflow_behind_a_step_or_episode(gpu, dtype, t, d):
+    """k of a step times q of an earlier one, or of another episode, is no term of any sum, though it is larger than a float."""
+    x = _attn_inputs(gpu, t, 2, 2, d, d, dtype, 6, True, 0.0)
+    x["q"][2, 0] *= 2.0 ** 100
+    x["k"][5, 0] *= 2.0 ** 100
+    x["reset"] = torch.zeros(t, 2, dtype=torch.uint8, device=gpu)
+    x["reset"][8, 1] = 1
+    x["k"][7, 1] *= 2.0 ** 100
+    x["q"][9, 1] *= 2.0 ** 100
+    x["dstate"] = None
+    _attn_check(x, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t,m,h,dk,dv", [(700, 1, 2, 33, 50), (333, 3, 1, 64, 64), (260, 2, 3, 128, 96)])
+def test_long_windows_off_sixteen_bytes(gpu, dtype, t, m, h, dk, dv):
+    """Slices that start off 16 bytes, few rows and a long window: element by element, the time axis cut."""
+    x = _attn_inputs(gpu, t, m, h, dk, dv, dtype, 31, True, 0.004, spread=True)
+    for n in ("q", "k", "v", "dout"):
+        wide = torch.zeros(t, m, h, x[n].shape[-1] + 1, dtype=dtype, device=gpu)
+        wide[..., 1:] = x[n]
+        x[n] = wide[..., 1:]
+    _attn_check(x, scale=dk ** -0.5)
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Two calls in flight together, of the same sizes with workspaces of their own, give what each gives alone."""
+    from purejaxql_amd import ops
+    xs = [_attn_inputs(gpu, 900, 1, 3, 64, 64, BF16, s, True, 0.002) for s in (1, 2)]
+    ls = [_logit_inputs(gpu, 2, 70000, BF16, s, True) for s in (3, 4)]
+    ns = [_norm_inputs(gpu, 700, 4500, F32, s, "silu", True) for s in (5, 6)]
+
+    def run(x, l, n):
+        o = ops.decay_attention(x["q"], x["k"], x["v"], x["decay"], state=x["state"], reset=x["reset"])
+        g = ops.decay_attention_grad(x["q"], x["k"], x["v"], x["decay"], x["dout"], state=x["state"], reset=x["reset"])
+        p = ops.action_logprobs(l["logits"], l["actions"], mask=l["mask"], top=5)
+        r = ops.residual_norm_grad(n["x"], n["f"], n["dy"], n["dh"], gate=n["gate"], gate_act="silu", **{k: n[k] for k in NORM_PARAMS})
+        return [*o, *g, *p, *r.values()]
+
+    want = [run(*a) for a in zip(xs, ls, ns)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for st, a in zip(streams, zip(xs, ls, ns)):
+            with torch.cuda.stream(st):
+                got.append(run(*a))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(i, j) for i, j in zip(a, b))
 
 
 def test_attention_lengths_of_zero(gpu):
@@ -367,6 +437,13 @@ def test_residual_norm_options(gpu, kind, act, params, post, pre, strided):
     _norm_check(_norm_inputs(gpu, 37, 96, F32, 3, act, params, strided), kind, act, post, pre)
 
 
+@pytest.mark.parametrize("n,d,dtype,params,strided", [(900, 4100, F32, True, False), (300, 5001, BF16, True, True), (520, 6000, F16, False, False),
+                                                      (70, 8191, F32, True, True)])
+def test_residual_norm_wide_rows(gpu, n, d, dtype, params, strided):
+    """Rows over 4096 columns: the parameter gradients come from a second look at the rows."""
+    _norm_check(_norm_inputs(gpu, n, d, dtype, d, "silu", params, strided), "layer_norm", "silu")
+
+
 @pytest.mark.parametrize("use_dy,use_dh", [(True, False), (False, True)])
 def test_residual_norm_one_gradient(gpu, use_dy, use_dh):
     _norm_check(_norm_inputs(gpu, 50, 200, BF16, 8, "sigmoid", True), "layer_norm", "sigmoid", use_dy=use_dy, use_dh=use_dh)
@@ -558,6 +635,21 @@ def test_action_logprobs_gradient_against_differences(gpu):
         z = x["logits"].double()
         diff = (loss(z + 1e-5 * d) - loss(z - 1e-5 * d)) / 2e-5
         assert abs(diff - float((g * d).sum())) <= 2e-5 * float((g.abs() * d.abs()).sum())
+
+
+@pytest.mark.parametrize("n,a", [(6, 300), (4, 5000), (3, 40001)])
+def test_action_logprobs_strided_and_bool_masks(gpu, n, a):
+    """A mask of truth values, and one that is a slice of a wider tensor at an odd offset."""
+    from purejaxql_amd import ops
+    x = _logit_inputs(gpu, n, a, BF16, a, True)
+    want = ops.action_logprobs(x["logits"], x["actions"], mask=x["mask"], top=6)
+    wide = torch.ones(n, a + 3, dtype=torch.uint8, device=gpu)
+    wide[:, 3:] = x["mask"]
+    for mask in (x["mask"].bool(), wide[:, 3:]):
+        got = ops.action_logprobs(x["logits"], x["actions"], mask=mask, top=6)
+        assert all(torch.equal(i, j) for i, j in zip(got, want))
+    x["mask"] = wide[:, 3:]
+    _logp_check(x, 1.3, 6)
 
 
 def test_action_logprobs_no_rows(gpu):
