@@ -151,16 +151,28 @@ static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
 #undef DA_GO
 }
 
+static bool da_vec(const pqn_decay_attn_t *a, int grad) {
+  const int ev = 16 / pqn_dtype_size(a->dtype);
+  uintptr_t at = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (grad ? (uintptr_t)a->dout | (uintptr_t)a->dq | (uintptr_t)a->dk_out | (uintptr_t)a->dv_out : (uintptr_t)a->out);
+  bool vec = a->dk % ev == 0 && a->dv % ev == 0 && (at & 15) == 0;
+  for (int i = 0; i < 3; ++i)
+    vec = vec && a->q_stride[i] % ev == 0 && a->k_stride[i] % ev == 0 && a->v_stride[i] % ev == 0 && (!grad || a->dout_stride[i] % ev == 0);
+  return vec;
+}
+
 // Windows of up to this many steps go step by step, longer ones by chunks.  Measured on both sides, us forward / gradient: 4096 x 4 heads
 // of 32, f32, 2 steps 30 / 90 against 46 / 113 by chunks, 4 steps 37 / 110 against 45 / 107, 6 steps 46 / 135 against 45 / 107; 1024 x 8
 // heads of 64, f32, 1 step 48 / 137 against 75 / 175; 1024 x 8 heads of 128, 1 step, f32 218 / 585 against 224 / 508, bf16 216 / 657
-// against 196 / 356, 2 steps bf16 257 / 806 against 213 / 366.
+// against 196 / 356, 2 steps bf16 257 / 806 against 213 / 366.  Off 16 bytes chunks load element by element: 1000 x 4 heads of 127, 3 steps
+// f32 212 / 396 against 238 / 547, 2 steps bf16 219 / 395 against 216 / 521, 4 steps bf16 275 / 575 against 219 / 528; 4000 x 8 heads of 33
+// and 65, 3 steps bf16 328 / 1170 against 645 / 2429.
 static bool da_by_steps(const pqn_decay_attn_t *a, bool grad) {
   const int w = a->dk > a->dv ? a->dk : a->dv;
-  return a->t_len <= (w <= 32 ? 4 : w <= 64 || (a->dtype == PQN_DTYPE_F32 && !grad) || (long long)a->m * a->heads < 2048 ? 1 : 0);
+  return a->t_len <= (w <= 32 ? 4 : !da_vec(a, grad) ? 3 : w <= 64 || (a->dtype == PQN_DTYPE_F32 && !grad) || (long long)a->m * a->heads < 2048 ? 1 : 0);
 }
 // The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
-// reading of k and v and a state written and read), as many as make DA_FILL waves.
+// reading of k and v and a state written and read), as many as make DA_FILL waves.  Measured, 1001 steps x 35 rows of 48 and 80 columns,
+// f32, forward / gradient: parts of 64 or more 61 / 174 us, 128 63 / 202, 256 97 / 273; 16001 x 16 rows, bf16: 2048 waves 112 us, 4096 121.
 static constexpr int DA_MIN_PART = 64, DA_FILL = 2048;
 
 static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int vec) {
@@ -176,14 +188,6 @@ static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int 
   X.vec = vec;
   return X;
 }
-static bool da_vec(const pqn_decay_attn_t *a, int grad) {
-  const int ev = 16 / pqn_dtype_size(a->dtype);
-  uintptr_t at = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (grad ? (uintptr_t)a->dout | (uintptr_t)a->dq | (uintptr_t)a->dk_out | (uintptr_t)a->dv_out : (uintptr_t)a->out);
-  bool vec = a->dk % ev == 0 && a->dv % ev == 0 && (at & 15) == 0;
-  for (int i = 0; i < 3; ++i)
-    vec = vec && a->q_stride[i] % ev == 0 && a->k_stride[i] % ev == 0 && a->v_stride[i] % ev == 0 && (!grad || a->dout_stride[i] % ev == 0);
-  return vec;
-}
 // workspace of one launch of `passes` scans: the parts' states, then their cut flags
 static int da_state_size(const da_split &X, int a, int b) { return da_ap(a, X.vec) * 32 * da_nw(a, b, X.vec); }
 static long long da_ws_bytes(const da_split &X, long long rows, int passes, int a, int b) {
@@ -191,10 +195,10 @@ static long long da_ws_bytes(const da_split &X, long long rows, int passes, int 
   return passes * (rows * (X.parts - 1) * 4ll * da_state_size(X, a, b) + (rows * (X.parts - 1) * 4 + 15) / 16 * 16);
 }
 
-// passes of equal widths, chunked, in one launch each of: the parts' states, their join, the scan
+// the passes, chunked, in one launch each of: the parts' states, their join, the scan
 static int da_run_chunks(da_args &A, int passes, int dtype, int vec, void *workspace, hipStream_t st) {
   const long long rows = (long long)A.m * A.heads;
-  const int a = A.pass[0].a, b = A.pass[0].b;
+  const int a = da_widest(A, passes, &da_pass::a), b = da_widest(A, passes, &da_pass::b);
   da_split X = da_cut(A.t_len, rows, passes, a, b, vec);
   const int size = da_state_size(X, a, b);
   for (int p = 0; p < passes; ++p) {
@@ -278,9 +282,9 @@ extern "C" int64_t pqn_decay_attn_workspace_bytes(const pqn_decay_attn_t *a, int
     return x > y ? x : y;
   };
   if (!grad) return need(1, a->dk, a->dv);
-  if (a->dk == a->dv) return need(3, a->dk, a->dv);
-  const long long one = need(2, a->dv, a->dk), two = need(1, a->dk, a->dv);         // one after the other
-  return one > two ? one : two;
+  const int w = a->dk > a->dv ? a->dk : a->dv;
+  const long long all = need(3, w, w), one = need(2, a->dv, a->dk), two = need(1, a->dk, a->dv);   // together, or one after the other
+  return all > one ? (all > two ? all : two) : one > two ? one : two;
 }
 
 extern "C" int pqn_decay_attn(const pqn_decay_attn_t *a, void *stream) {
@@ -332,7 +336,16 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   if (!da_by_steps(a, true)) {
     const int vec = da_vec(a, 1);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
-    if (a->dk == a->dv) return da_run_chunks(A, 3, a->dtype, vec, a->workspace, (hipStream_t)stream);
+    // dq and dk have states of [dv][dk], dv of [dk][dv].  One launch of the kernel that holds both where that is the kernel of each, or
+    // where there is little to do in several launches (the time axis is cut) and they are more than the padding.  Measured on both
+    // sides, together / one after the other, us: 300 steps x 6 rows, 32 and 128 columns, f32 48 / 77, bf16 33 / 57; 1001 x 35, 48 and 80,
+    // f32 166 / 148, bf16 79 / 90; 5000 x 8, 64 and 128, bf16 75 / 114; 4000 x 160, 32 and 64, f32 782 / 582, bf16 328 / 281; 32 x 512,
+    // 80 and 48, f32 61 / 52 (not cut).
+    const int w = a->dk > a->dv ? a->dk : a->dv, least = a->dk + a->dv - w;
+    const bool alike = da_ap(least, vec) == da_ap(w, vec) && da_nw(least, w, vec) == da_nw(w, w, vec) && da_nw(w, least, vec) == da_nw(w, w, vec);
+    const long long rows = (long long)a->m * a->heads;
+    if (alike || (a->t_len * rows <= (a->dtype == PQN_DTYPE_F32 ? 1 << 14 : 1 << 16) && da_cut(a->t_len, rows, 3, w, w, vec).parts > 1))
+      return da_run_chunks(A, 3, a->dtype, vec, a->workspace, (hipStream_t)stream);
     int rc = da_run_chunks(A, 2, a->dtype, vec, a->workspace, (hipStream_t)stream);      // dq, dk: states of [dv][dk]
     if (rc != PQN_OK) return rc;
     A.pass[0] = A.pass[2];                                                          // dv: [dk][dv]

@@ -681,18 +681,24 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
 }
 
 // widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave.  Tensors whose rows are not whole 16-byte
-// accesses take the widest kernel, whose loads go element by element.
-inline int da_ap(int a, int vec) { return !vec ? 128 : a <= 32 ? 32 : a <= 64 ? 64 : 128; }
+// accesses go element by element, in fewer forms.
+inline int da_ap(int a, int vec) { return a <= 32 && vec ? 32 : a <= 64 ? 64 : 128; }
 inline int da_nw(int a, int b, int vec) {
   const int nw = b <= 32 ? 1 : b <= 64 ? 2 : 4;
-  return !vec ? 4 : a > 64 && nw < 2 ? 2 : nw;    // a wave alone would hold 128 registers of loads in flight
+  return !vec ? a > 64 || nw == 4 ? 4 : 2 : a > 64 && nw < 2 ? 2 : nw;    // a wave alone would hold 128 registers of loads in flight
+}
+// the kernel for passes of unequal widths is the one that holds the widest
+inline int da_widest(const da_args &A, int passes, int da_pass::*width) {
+  int w = 0;
+  for (int p = 0; p < passes; ++p) w = A.pass[p].*width > w ? A.pass[p].*width : w;
+  return w;
 }
 int da_launch_chunk_f32(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st);
 int da_launch_chunk_bf16(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st);
 
 template <typename T, int L>
 static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st) {
-  const int ap = da_ap(A.pass[0].a, X.vec), nw = da_nw(A.pass[0].a, A.pass[0].b, X.vec);
+  const int a = da_widest(A, passes, &da_pass::a), ap = da_ap(a, X.vec), nw = da_nw(a, da_widest(A, passes, &da_pass::b), X.vec);
   const long long units = (long long)A.m * A.heads * (state ? X.parts - 1 : X.parts), grid = (units + 7) / 8 * 8 * passes;
   PQN_REQUIRE(grid < (1ll << 31), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
 #define DA_GO(AP, NW, VEC)                                                                                                   \
@@ -710,8 +716,10 @@ static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool
   DA_GO(64, 4, true)
   DA_GO(128, 2, true)
   DA_GO(128, 4, true)
+  DA_GO(64, 2, false)
+  DA_GO(64, 4, false)
   DA_GO(128, 4, false)
 #undef DA_GO
-  pqn_set_error("pqn_decay_attn: no kernel for widths %d, %d", A.pass[0].a, A.pass[0].b);
+  pqn_set_error("pqn_decay_attn: no kernel for widths of up to %d", a);
   return PQN_E_UNSUPPORTED;
 }
