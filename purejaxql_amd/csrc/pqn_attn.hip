@@ -116,13 +116,23 @@ __global__ __launch_bounds__(256) void da_join_kernel(da_args A, da_split X, int
   const int *cut = X.cut + pass * X.cut_stride + mh * (X.parts - 1);
   const float fade = (float)pqn_powi((double)A.decay[(uint32_t)mh % (uint32_t)A.heads], X.len);
   f32x4_t s = *(const f32x4_t *)p;
-  for (int i = 1; i < X.parts - 1; ++i) {
-    const f32x4_t own = *(const f32x4_t *)(p + (long long)i * size);
-    if (cut[i]) s = own;
-    else
+  const int last = X.parts - 2;
+  constexpr int AHEAD = 8;                                        // states requested together: the walk waits once for so many
+  for (int i0 = 1; i0 <= last; i0 += AHEAD) {
+    f32x4_t own[AHEAD];
+    int ends[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = fmaf(s[j], fade, own[j]);
-    *(f32x4_t *)(p + (long long)i * size) = s;
+    for (int i = 0; i < AHEAD; ++i) {
+      own[i] = *(const f32x4_t *)(p + (long long)min(i0 + i, last) * size);
+      ends[i] = cut[min(i0 + i, last)];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (i0 + i > last) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = ends[i] ? own[i][j] : fmaf(s[j], fade, own[i][j]);
+      *(f32x4_t *)(p + (long long)(i0 + i) * size) = s;
+    }
   }
 }
 

@@ -396,23 +396,27 @@ __global__ __launch_bounds__(256) void rn_sums_kernel(rn_args A) {
     for (int e = 0; e < VW; ++e) out[(size_t)k * d + e] = sum[k][e];
 }
 
-// column sums of the partials: 64 columns x 16 row groups per workgroup, fixed order
+// column sums of the partials: COLS columns x 1024 / COLS row groups per workgroup, fixed order
 struct rn_param_out {
   float *p[RN_PARAMS];
 };
+template <int COLS>
 __global__ __launch_bounds__(1024) void rn_param_kernel(const float *__restrict__ partials, int parts, int d, rn_param_out out) {
-  __shared__ float s[16][64];
-  const int k = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+  constexpr int ROWS = 1024 / COLS;
+  __shared__ float s[ROWS][COLS + 1];
+  const int k = blockIdx.y, cc = threadIdx.x % COLS, c = blockIdx.x * COLS + cc, r = threadIdx.x / COLS;
   if (!out.p[k]) return;
   float a = 0.f;
-  if (c < d)
-    for (int i = r; i < parts; i += 16) a += partials[((size_t)i * RN_PARAMS + k) * d + c];
-  s[r][threadIdx.x & 63] = a;
+  if (c < d) {
+#pragma unroll 8
+    for (int i = r; i < parts; i += ROWS) a += partials[((size_t)i * RN_PARAMS + k) * d + c];
+  }
+  s[r][cc] = a;
   __syncthreads();
-  if (r == 0 && c < d) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) a += s[i][threadIdx.x];
-    out.p[k][c] = a;
+  const int lane = threadIdx.x & 63;
+  for (int col = threadIdx.x >> 6; col < COLS; col += 16) {       // a wave per column
+    a = pqn_wave_sum(lane < ROWS ? s[lane % ROWS][col] : 0.f);
+    if (lane == 0 && blockIdx.x * COLS + col < d) out.p[k][blockIdx.x * COLS + col] = a;
   }
 }
 
@@ -567,7 +571,10 @@ extern "C" int pqn_residual_norm_grad(const pqn_residual_norm_t *a, void *stream
     if (r != PQN_OK) return r;
   }
   if (!any) return PQN_OK;
-  rn_param_kernel<<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, a->n > 0 ? rn_parts(a->n, a->d) : 0,
-                                                                                      a->d, out);
+  // few columns are shared out finely, or too few workgroups read.  us with 16 / 64 columns a workgroup: d = 1024, 1024 parts 9 / 23;
+  // d = 4095, 512 parts 20 / 14
+  const int parts = a->n > 0 ? rn_parts(a->n, a->d) : 0;
+  if (a->d <= 2048) rn_param_kernel<16><<<dim3((a->d + 15) / 16, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, parts, a->d, out);
+  else rn_param_kernel<64><<<dim3((a->d + 63) / 64, RN_PARAMS), 1024, 0, (hipStream_t)stream>>>(a->workspace, parts, a->d, out);
   return pqn_check_launch("pqn_residual_norm_grad");
 }

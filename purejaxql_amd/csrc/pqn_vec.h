@@ -48,14 +48,14 @@ PQN_D float pqn_wave_sum(float x) {
 }
 PQN_D uint32_t pqn_wave_min(uint32_t x) { return ~pqn_wave_max(~x); }
 
-// the same over aligned groups of G lanes (G = 8, 16, 32, 64), in every lane of the group: exchanges within 4, 8 and 16 lanes by DPP (a
+// the same over aligned groups of G lanes (G = 4, 8, 16, 32, 64), in every lane of the group: exchanges within 4, 8 and 16 lanes by DPP (a
 // mirrored row of equal halves is the other half), across them by a shuffle
 template <int G, typename OP>
 PQN_D uint32_t pqn_group_fold(uint32_t x, OP op) {
 #define PQN_STEP(ctrl) x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true));
   PQN_STEP(0xb1)                         // quad_perm [1, 0, 3, 2]
   PQN_STEP(0x4e)                         // quad_perm [2, 3, 0, 1]
-  PQN_STEP(0x141)                        // row_half_mirror
+  if constexpr (G >= 8) { PQN_STEP(0x141) }    // row_half_mirror
   if constexpr (G >= 16) { PQN_STEP(0x140) }   // row_mirror
 #undef PQN_STEP
 #pragma unroll
