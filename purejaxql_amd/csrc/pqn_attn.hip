@@ -15,7 +15,8 @@
 
 // ---- the recurrence, step by step ------------------------------------------------------------------------------------------
 // A wave owns 32 columns of one (row, head)'s state in registers for the whole scan: 8 lanes x 4 columns across, 8 lane groups down
-// the rows, RPT rows per lane.  A step reads q, k, v once and reduces o over the lane groups by shuffles; no shared memory.
+// the rows, RPT rows per lane.  A step reads q, k, v once and reduces o over the lane groups by shuffles; no shared memory.  Bound: the
+// state's bytes (HBM) for a step of many rows, latency for few: 128 rows x 4 heads of 32, f32, one step 4.8 us (10.5 with the call).
 template <int RPT, bool VEC>
 PQN_D void da_state_io(float (&s)[RPT][4], float *mem, const da_pass &P, int r0, int c0, bool write) {
 #pragma unroll

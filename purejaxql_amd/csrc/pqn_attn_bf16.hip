@@ -1,5 +1,5 @@
-// pqn_attn_bf16.hip -- the chunked scan of pqn_attn.hip on bf16 tensors.  Chunks of 64 steps: 57 KB of LDS at the widest heads, two
-// workgroups to a CU.
+// pqn_attn_bf16.hip -- the chunked scan of pqn_attn.hip on bf16 tensors.  Chunks of 32 steps: 27 KB of LDS at the widest heads, two waves
+// a SIMD by registers.
 #include "pqn_attn_chunk.h"
 
 int da_launch_chunk_bf16(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st) {

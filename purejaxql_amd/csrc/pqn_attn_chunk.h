@@ -35,12 +35,18 @@ struct da_args {
 // 16 x 16 tiles are 8 neighbouring columns (da_row, da_col): one 16-byte read of Q, one 16-byte store of O.
 //
 // bf16: v_mfma_f32_16x16x32_bf16 with the state (S^T Q^T) and the weighted products (V^T P^T) rounded to bf16 as operands -- the
-// output is rounded to bf16 anyway -- and w V split in two bf16 pieces (16 significant bits), because the state is an f32 result that
-// is carried on.  f32: v_mfma_f32_16x16x4_f32 throughout, four of them per 16 values of k.
+// output is rounded to bf16 anyway -- and w V split in three bf16 pieces, which hold it exactly, because the state is an f32 result
+// that is carried on (two pieces left it 3e-6 off after some hundred steps).  f32: v_mfma_f32_16x16x4_f32 throughout, four of them per
+// 16 values of k.
 //
-// Bound: HBM.  A chunk of 64 steps of 128 + 128 columns moves 64 KB (about 7300 cycles of a CU's share of the bandwidth) and costs
-// about 2000 cycles of MFMA, 2400 of LDS and 2000 of VALU per workgroup; two workgroups share a CU, and the next chunk's loads are
-// in flight in registers while a chunk is computed.
+// Bound: HBM where there are rows enough.  A chunk of 32 steps of 128 + 128 bf16 columns moves 32 KB (about 3900 cycles of a CU's share
+// of the bandwidth) and costs a wave 71 matrix instructions of 16 cycles; f32 doubles the bytes and costs four times the instructions at
+// 32 cycles each, about as much as the bytes.  Chunks of 32 steps and not 64: half the registers in flight, no spills, two waves a SIMD
+// (heads of 128, 128 steps x 2048 rows, bf16, gradient: 267 us).  Next chunk's loads are in flight in registers while a chunk is computed.
+// Measured, forward / gradient: bf16, 128 steps x 2048 rows of 128 x 128: 128 / 267 us (floors 106 / 171 by the bytes at 5.08 TB/s); f32,
+// 32 steps x 16384 rows of 32 x 32: 118 / 267 us (79 / 132; the three scans of the gradient read the window nearly twice); one step of
+// 8192 bf16 rows of 128 x 128: 216 us, 5.0 TB/s; f32, 1001 steps x 35 rows of 48 x 80: 52 / 148 us (latency: three launches a scan, each
+// a few chunks deep).
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef pqn_bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));

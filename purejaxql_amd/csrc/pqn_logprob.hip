@@ -10,6 +10,9 @@
 // the order of the work.
 //
 // Bound: HBM for many logits (about 9 vector operations and one v_exp_f32 a logit, below the time its bytes take), latency for few.
+// Measured, forward / gradient: 4096 x 32000 bf16, five alternatives, 85 / 84 us at best (3.1 / 6.2 TB/s: the gradient's reads come from
+// the last-level cache in part); 131072 x 17 f32 with masks and three alternatives 9.0 / 8.6 us (vector work of joining 17 logits over
+// lanes); 8 x 100003 bf16, eight alternatives, 10.7 us and 6.5 us for joining 25 parts a row (latency).
 #include <type_traits>
 
 #include "pqn_vec.h"
@@ -220,8 +223,10 @@ PQN_D u64 lp_take(uint32_t (&o)[VW], uint32_t j0) {
 // A workgroup per row (or part of a row), which it holds in registers: N accesses of VW logits a thread, all requested at once; the
 // row's first and last logits that fill no whole access one to a thread.  Three looks at the registers: the largest of every access,
 // the sums under the thread's own maximum, and the alternatives.  For those, a bar: the K-th largest of a wave's 64 thread maxima is
-// no larger than the wave's K-th logit, so the largest of the waves' bars sorts out all but a few accesses; what is left goes through
-// the wave's list of K keys, and the waves' lists are merged.
+// no larger than the wave's K-th logit, so the largest of the waves' bars sorts out all but some K logits; their keys are collected in
+// LDS, in whatever order (they are distinct), and the first wave takes the K best.  Where LP_CAND do not hold them (many equal logits),
+// they go through a list of K keys per wave instead, an access of the wave at a time.
+static constexpr int LP_CAND = 256;
 typedef uint32_t lp_u32x4 __attribute__((ext_vector_type(4)));
 // logit e of an access, kept packed
 template <typename T>
@@ -243,7 +248,9 @@ PQN_D void lp_forbid(lp_u32x4 &r, int e, bool no) {
 template <typename T, int NT, int N>
 __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
   constexpr int NW = NT / 64, VW = 16 / (int)sizeof(T);
-  __shared__ u64 keys[NW * LP_MAX_TOP];
+  static_assert(NW * LP_MAX_TOP <= LP_CAND, "the waves' lists fit");
+  __shared__ u64 keys[LP_CAND];
+  __shared__ int found;
   __shared__ float sums[NW][3];
   __shared__ uint32_t bar[NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -308,7 +315,8 @@ __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
     sums[wave][1] = v.s;
     sums[wave][2] = v.t;
   }
-  u64 list = 0ull;
+  int count = 0;
+  bool lists = false;
   if (A.top > 0) {
     uint32_t mine = m > -INFINITY ? lp_order(m) : 0u, least = 0u;
     for (int i = 0; i < A.top; ++i) {
@@ -317,7 +325,30 @@ __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
       mine = lane == at ? 0u : mine;
     }
     if (lane == 0) bar[wave] = least;
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) least = max(least, bar[w]);
+    const float above = lp_unorder(max(least, 1u << 23));            // least = 0: every number (order 2^23 is the lowest float's)
+    auto offer = [&](float x, int j) {
+      if (x >= above) {                                              // false for NaN
+        const int at = atomicAdd(&found, 1);
+        if (at < LP_CAND) keys[at] = lp_key(x, j);
+      }
+    };
+    offer(xr[0], jr);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (top[i] >= above) {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) offer(lp_get<T>(r[i], e), first(i) + e);
+      }
+    __syncthreads();
+    count = found;
+  }
+  if (count > LP_CAND) {
+    u64 list = 0ull;
+    uint32_t least = 0u;
 #pragma unroll
     for (int w = 0; w < NW; ++w) least = max(least, bar[w]);
     auto look = [&](const auto &x, float best_x, int j) {
@@ -345,6 +376,8 @@ __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
         look(x, top[i], first(i));
       }
     if (lane < A.top) keys[wave * A.top + lane] = list;
+    count = NW * A.top;
+    lists = true;
   }
   __syncthreads();
   if (wave != 0) return;
@@ -361,20 +394,32 @@ __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
       rec[2] = v.t;
     }
   }
-  // the best of the NW lists
-  constexpr int ML = (NW * LP_MAX_TOP + 63) / 64;
+  auto put = [&](int i, u64 key) {
+    if (A.splits == 1) lp_write_top(A, row, i, key, rw.lse);
+    else ((u64 *)(rec + 4))[i] = key;
+  };
+  if (count <= 64 && !lists) {                    // distinct keys, one to a lane: a key's place is the number of those above it
+    const u64 mine = lane < count ? keys[lane] : 0ull;
+    int place = 0;
+    for (int j = 0; j < count; ++j) {
+      const u64 other = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), j) << 32) |
+                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, j);
+      place += other > mine;
+    }
+    if (lane >= count) place = lane;              // empty places
+    if (place < A.top) put(place, mine);
+    return;
+  }
+  constexpr int ML = LP_CAND / 64;
   u64 mine[ML];
 #pragma unroll
-  for (int i = 0; i < ML; ++i) mine[i] = i * 64 + lane < NW * A.top ? keys[i * 64 + lane] : 0ull;
+  for (int i = 0; i < ML; ++i) mine[i] = i * 64 + lane < count ? keys[i * 64 + lane] : 0ull;
   for (int i = 0; i < A.top; ++i) {
     u64 best = mine[0];
 #pragma unroll
     for (int k = 1; k < ML; ++k) best = lp_max(best, mine[k]);
     best = lp_group_max<64>(best);
-    if (lane == 0) {
-      if (A.splits == 1) lp_write_top(A, row, i, best, rw.lse);
-      else ((u64 *)(rec + 4))[i] = best;
-    }
+    if (lane == 0) put(i, best);
 #pragma unroll
     for (int k = 0; k < ML; ++k) mine[k] = mine[k] == best ? 0ull : mine[k];
   }
@@ -523,7 +568,7 @@ static lp_args lp_fill(const pqn_action_logprobs_t *a) {
   return A;
 }
 
-// Rows of up to LP_ROW_MAX logits live in a wave's registers, longer ones in a workgroup's, up to 16 accesses a thread (32768 16-bit or
+// Rows of up to LP_ROW_MAX logits live in a wave's registers (lp_rows_kernel or lp_long_kernel), longer ones in a workgroup's, up to 16 accesses a thread (32768 16-bit or
 // 16384 f32 logits); beyond that, or where there are too few rows to fill the chip, a row is cut (a part keeps at least LP_MIN_PART
 // logits, below which the join costs more than it gives).
 static constexpr int LP_ROW_MAX = 1024, LP_NT = 256, LP_MIN_PART = 4096, LP_FILL = 1024, LP_MOST = 16;
@@ -551,7 +596,9 @@ static int lp_part(int a, int splits) { return ((a + splits - 1) / splits + 7) /
 
 template <typename T>
 static int lp_launch(lp_args A, hipStream_t st) {
-  if (A.a <= LP_ROW_MAX) {
+  // By the rows kernel an alternative costs a search over all of a lane's logits, by the long one only the collected: 60000 x 1000 f32 in
+  // us, rows / long, no alternatives 38 / 50, 4 88 / 60, 8 136 / 76; x 300, none 21 / 37, 4 50 / 50; x 500, 16 128 / 76.
+  if (A.a <= 256 || (A.a <= 512 && A.top <= 3) || (A.a <= LP_ROW_MAX && A.top <= 1)) {
 #define LP_GO(G, E)                                                                           \
   do {                                                                                        \
     lp_rows_kernel<T, G, E><<<(unsigned)(((long long)A.n * G + 255) / 256), 256, 0, st>>>(A); \
@@ -567,7 +614,13 @@ static int lp_launch(lp_args A, hipStream_t st) {
   const long long grid = (long long)A.n * A.splits;
   PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a);
   const int each = (A.part + LP_NT * VW - 1) / (LP_NT * VW);
-  if (each <= 1) lp_long_kernel<T, LP_NT, 1><<<(unsigned)grid, LP_NT, 0, st>>>(A);
+  // few accesses: a wave or two to a row, with less to join.  16000 x 4000 bf16, 8 alternatives, 128 / 256 threads 52 / 69 us; 60000 x
+  // 1100, 64 / 256 threads 88 / 195
+  const int wave = (A.part + 64 * VW - 1) / (64 * VW);
+  if (A.splits == 1 && wave <= 2) lp_long_kernel<T, 64, 2><<<(unsigned)grid, 64, 0, st>>>(A);
+  else if (A.splits == 1 && wave <= 4) lp_long_kernel<T, 64, 4><<<(unsigned)grid, 64, 0, st>>>(A);
+  else if (A.splits == 1 && wave <= 8) lp_long_kernel<T, 128, 4><<<(unsigned)grid, 128, 0, st>>>(A);
+  else if (each <= 1) lp_long_kernel<T, LP_NT, 1><<<(unsigned)grid, LP_NT, 0, st>>>(A);
   else if (each <= 2) lp_long_kernel<T, LP_NT, 2><<<(unsigned)grid, LP_NT, 0, st>>>(A);
   else if (each <= 4) lp_long_kernel<T, LP_NT, 4><<<(unsigned)grid, LP_NT, 0, st>>>(A);
   else lp_long_kernel<T, LP_NT, LP_MOST><<<(unsigned)grid, LP_NT, 0, st>>>(A);

@@ -652,6 +652,31 @@ def test_action_logprobs_strided_and_bool_masks(gpu, n, a):
     _logp_check(x, 1.3, 6)
 
 
+@pytest.mark.parametrize("a", [300, 700, 1500, 3000, 9000, 33001])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_action_logprobs_alternatives_among_equals(gpu, a, dtype):
+    """The lowest indexes of 1, 40, 100, 290 and all equal best logits, of fewer allowed than asked for, and of rising and falling rows."""
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(a)
+    l = torch.randn(9, a, generator=gen, device=gpu) - 8.0
+    for i, k in enumerate((1, 40, 100, 290, a)):
+        l[i, torch.randperm(a, generator=gen, device=gpu)[:k]] = 4.0
+    l[5] = torch.arange(a, device=gpu) / a
+    l[6] = -l[5]
+    l[7] = -math.inf
+    l[7, a // 3:a // 3 + 5] = torch.tensor([-3.0, 0.0, -0.0, -math.inf, 2.0], device=gpu)
+    l[8] = torch.finfo(BF16).min
+    x = _logit_inputs(gpu, 9, a, dtype, a, False)
+    x["logits"] = l.to(dtype)
+    from purejaxql_amd import ops
+    for top in (1, 8, 16):
+        got = ops.action_logprobs(x["logits"], x["actions"], top=top)
+        key = x["logits"].double().cpu() + 0.0
+        want = torch.sort(key, dim=-1, descending=True, stable=True)
+        ids = torch.where(want.values[:, :top] > -math.inf, want.indices[:, :top], torch.full_like(want.indices[:, :top], -1))
+        assert torch.equal(got[4].cpu().long(), ids), top
+
+
 def test_action_logprobs_no_rows(gpu):
     from purejaxql_amd import ops
     e = torch.empty(0, 9, device=gpu)
