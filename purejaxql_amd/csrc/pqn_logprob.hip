@@ -98,15 +98,16 @@ PQN_D LpSum lp_group_join(LpSum v, float scale) {
 
 // what a row's sums say
 struct LpRow {
-  float lse, entropy;
+  float lse, entropy, m, log_s;      // lse = m / temperature + log_s
 };
 PQN_D LpRow lp_row(const LpSum &v, float inv_temp) {
-  LpRow r;
-  if (v.s != v.s) r.lse = r.entropy = NAN;
-  else if (!(v.s > 0.f)) r.lse = -INFINITY, r.entropy = 0.f;          // nothing allowed
+  LpRow r = {NAN, NAN, v.m, 0.f};
+  if (v.s != v.s) return r;
+  if (!(v.s > 0.f)) r.lse = -INFINITY, r.entropy = 0.f;          // nothing allowed
   else {
     const float l = log2f(v.s);
-    r.lse = fmaf(v.m, inv_temp, LP_LN2 * l);
+    r.log_s = LP_LN2 * l;
+    r.lse = fmaf(v.m, inv_temp, r.log_s);
     r.entropy = fmaxf(LP_LN2 * (l - v.t / v.s), 0.f);
   }
   return r;
@@ -116,8 +117,9 @@ PQN_D float lp_logit(const lp_args &A, long long row, int j) {   // -inf where n
   if (A.mask && !A.mask[row * A.ms + j]) return -INFINITY;
   return pqn_to_f32(((const T *)A.logits)[row * A.ls + j]);
 }
+// from the difference to the largest logit: logit / temperature and lse may be beyond the largest float, or large and nearly equal
 PQN_D float lp_logp(float logit, const LpRow &r, float inv_temp) {
-  return (r.lse != r.lse) ? NAN : logit > -INFINITY ? fmaf(logit, inv_temp, -r.lse) : -INFINITY;
+  return (r.lse != r.lse) ? NAN : logit > -INFINITY ? fmaf(logit - r.m, inv_temp, -r.log_s) : -INFINITY;
 }
 template <typename T>
 PQN_D void lp_write_row(const lp_args &A, long long row, const LpRow &r) {
@@ -145,9 +147,9 @@ PQN_D void lp_row_load(const lp_args &A, long long row, int lane, float (&x)[E])
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = (on[e] != 0) & (e * G + lane < A.a) ? pqn_to_f32(raw[e]) : -INFINITY;
 }
-PQN_D void lp_write_top(const lp_args &A, long long row, int i, u64 key, float lse) {
+PQN_D void lp_write_top(const lp_args &A, long long row, int i, u64 key, const LpRow &r) {
   A.top_action[row * A.top + i] = key ? (int32_t)~(uint32_t)key : -1;
-  A.top_logp[row * A.top + i] = key ? lp_unorder((uint32_t)(key >> 32)) * A.inv_temp - lse : -INFINITY;
+  A.top_logp[row * A.top + i] = key ? lp_logp(lp_unorder((uint32_t)(key >> 32)), r, A.inv_temp) : -INFINITY;
 }
 
 // A row in the registers of G lanes, E logits each (a <= G * E): 64 / G rows per wave, no shared memory.
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(lp_args A) {
 #pragma unroll
       for (int e = 1; e < E; ++e) best = lp_max(best, key[e]);
       best = lp_group_max<G>(best);
-      if (live && lane == 0) lp_write_top(A, row, i, best, r.lse);
+      if (live && lane == 0) lp_write_top(A, row, i, best, r);
 #pragma unroll
       for (int e = 0; e < E; ++e) key[e] = key[e] == best ? 0ull : key[e];
     }
@@ -395,7 +397,7 @@ __global__ __launch_bounds__(NT, 4) void lp_long_kernel(lp_args A) {
     }
   }
   auto put = [&](int i, u64 key) {
-    if (A.splits == 1) lp_write_top(A, row, i, key, rw.lse);
+    if (A.splits == 1) lp_write_top(A, row, i, key, rw);
     else ((u64 *)(rec + 4))[i] = key;
   };
   if (count <= 64 && !lists) {                    // distinct keys, one to a lane: a key's place is the number of those above it
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(64) void lp_join_kernel(lp_args A) {
       if (k < floor) best = lp_max(best, k);
     }
     best = lp_group_max<64>(best);
-    if (lane == 0) lp_write_top(A, row, i, best, r.lse);
+    if (lane == 0) lp_write_top(A, row, i, best, r);
     floor = best;
   }
 }
@@ -474,7 +476,7 @@ struct LpGrad {                      // a row's scalars
   PQN_D void open(const lp_grad_args &G, long long row) {
     const lp_args &A = G.A;
     lse = A.lse[row];
-    none = lse == -INFINITY;
+    none = fabsf(lse) == INFINITY;       // nothing allowed, or beyond the largest float
     h = A.entropy[row];
     act = A.action[row];
     dlp = G.dlogp ? G.dlogp[row] : 0.f;

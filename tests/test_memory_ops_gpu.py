@@ -652,6 +652,31 @@ def test_action_logprobs_strided_and_bool_masks(gpu, n, a):
     _logp_check(x, 1.3, 6)
 
 
+@pytest.mark.parametrize("a", [17, 300, 5000, 70000])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_action_logprobs_beyond_the_largest_float(gpu, a, dtype):
+    """logits / temperature overflows: the log probabilities come from differences of logits; lse is infinite and the gradient 0.  A row
+    of large logits near each other: no cancellation (differences are exact, the sum of A terms is off by (64 + A / 64) u)."""
+    from purejaxql_amd import ops
+    big = torch.finfo(dtype).max
+    l = torch.empty(3, a, device=gpu)
+    l[0], l[1] = -big, big
+    l[2] = 2.0 ** 20 + torch.arange(a, device=gpu) % 2 * 2.0 ** 14
+    x = l.to(dtype)
+    act = torch.tensor([1, 2, 3], dtype=torch.int32, device=gpu)
+    logp, ent, lse, top_logp, top = ops.action_logprobs(x, act, temperature=0.25, top=2)
+    tol = torch.full((3,), (64 + a / 64 + 64 * math.log(a)) * U, device=gpu)
+    want = torch.full((3,), -math.log(a), device=gpu, dtype=torch.float64)
+    want[2] = -math.log(a // 2)
+    _close(logp, want, tol, "logp")
+    _close(ent, -want, tol, "entropy")
+    _close(top_logp, want[:, None].expand(3, 2), tol[:, None].expand(3, 2), "top_logp")
+    assert top.tolist() == [[0, 1], [0, 1], [1, 3]] and lse[0] == -math.inf and lse[1] == math.inf
+    one = torch.ones(3, device=gpu)
+    d = ops.action_logprobs_grad(x, act, lse, ent, one, one, one, temperature=0.25)
+    assert bool((d[:2] == 0).all()) and bool(torch.isfinite(d).all())
+
+
 @pytest.mark.parametrize("a", [300, 700, 1500, 3000, 9000, 33001])
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_action_logprobs_alternatives_among_equals(gpu, a, dtype):
