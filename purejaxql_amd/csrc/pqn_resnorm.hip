@@ -12,6 +12,8 @@
 // the gradient's row tensors, parameters and five column sums within the registers of three waves per SIMD.  Measured, forward /
 // gradient: 131072 x 1024 bf16 with a gate and all parameters 275 / 445 + 10 us (column sums), 4.9 / 4.8 TB/s; 4099 x 4095 f32, element by
 // element, 63 / 113 + 14 us, 5.3 / 4.7 TB/s; 128 x 128 f32 3.7 us, latency (12.5 with the call).
+#include <type_traits>
+
 #include "pqn_vec.h"
 
 static constexpr int RN_MAX_D = 8192;
@@ -61,48 +63,65 @@ PQN_D void rn_row_sum(float (&v)[K], float *lds, int &turn) {
   }
 }
 
-template <typename T, int NT, int VW, int NV>
+// Thread `lane` of the NT holds NV accesses of VW columns, the i-th from (i NT + lane) VW on.  LOOSE: the rows start anywhere and their
+// width is no multiple of VW; the access that would end behind the row ends at its last column instead, and what it shares with the one
+// before is that one's.  For rows of more than RN_WIDE columns, whose kernels have no registers for an address and a condition per
+// element: 2799 x 5394 bf16, forward / gradient 67 / 168 us, element by element 101 / 362; 18326 x 1163 60 / 157 and 56 / 145.
+template <typename T, int NT, int VW, int NV, bool LOOSE>
 struct RnRow {
   static constexpr int E = VW * NV;
-  typedef pqn_pack<T, VW> Pack;
-  PQN_D static int col(int lane, int i) { return (i * NT + lane) * VW; }
-  // requests a row: columns behind d repeat the row's first ones and are put to zero by open()
-  PQN_D static void fetch(Pack (&r)[NV], const void *base, long long off, int d, int lane) {
+  template <typename U>
+  using PackOf = typename std::conditional<LOOSE, pqn_loose<U, VW>, pqn_pack<U, VW>>::type;
+  typedef PackOf<T> Pack;
+  int d, lane;
+  PQN_D int first(int i) const { return (i * NT + lane) * VW; }
+  PQN_D int at(int i) const {                        // where the access is made
+    const int c = first(i);
+    return LOOSE ? min(c, d - VW) : c < d ? c : 0;
+  }
+  PQN_D bool own(int i, int j) const { return LOOSE ? at(i) + j >= first(i) : first(i) < d; }
+  PQN_D void fetch(Pack (&r)[NV], const void *base, long long off) const {
     const T *p = (const T *)base + off;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = col(lane, i);
-      r[i] = *(const Pack *)(p + (c < d ? c : 0));
-    }
+    for (int i = 0; i < NV; ++i) r[i] = *(const Pack *)(p + at(i));
   }
-  PQN_D static void open(float (&x)[E], const Pack (&r)[NV], int d, int lane) {
+  PQN_D void open(float (&x)[E], const Pack (&r)[NV]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VW; ++j) x[i * VW + j] = own(i, j) ? pqn_to_f32(r[i].v[j]) : 0.f;
+  }
+  template <typename U>
+  PQN_D void store(U *p, const float (&r)[E]) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const bool in = col(lane, i) < d;
+      const int c = first(i);
+      if (LOOSE ? c + VW <= d : c < d) {
+        PackOf<U> x;
 #pragma unroll
-      for (int j = 0; j < VW; ++j) x[i * VW + j] = in ? pqn_to_f32(r[i].v[j]) : 0.f;
+        for (int j = 0; j < VW; ++j) x.v[j] = (U)r[i * VW + j];
+        *(PackOf<U> *)(p + c) = x;
+      } else if (LOOSE && c < d) {
+#pragma unroll
+        for (int j = 0; j < VW; ++j)
+          if (own(i, j)) p[at(i) + j] = (U)r[i * VW + j];
+      }
     }
   }
-  PQN_D static void store(void *base, long long off, const float (&r)[E], int d, int lane) {
-    T *p = (T *)base + off;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = col(lane, i);
-      if (c < d) pqn_store<T, VW>(p + c, r + i * VW);
-    }
-  }
-  PQN_D static void param(float (&r)[E], const float *p, float absent, int d, int lane) {
+  PQN_D void store(void *base, long long off, const float (&r)[E]) const { store((T *)base + off, r); }
+  PQN_D void param(float (&r)[E], const float *p, float absent) const {
 #pragma unroll
     for (int e = 0; e < E; ++e) r[e] = absent;
     if (!p) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = col(lane, i);
-      if (c < d) pqn_load<float, VW>(r + i * VW, p + c);
+      const PackOf<float> x = *(const PackOf<float> *)(p + at(i));
+#pragma unroll
+      for (int j = 0; j < VW; ++j) r[i * VW + j] = own(i, j) ? x.v[j] : absent;
     }
   }
   // r -> (r - mean) * inv in place; returns inv = 1 / sqrt(var + eps).  rms: mean = 0
-  PQN_D static float normalise(float (&r)[E], int rms, float eps, int d, int lane, float *lds, int &turn, float *mean_out = nullptr) {
+  PQN_D float normalise(float (&r)[E], int rms, float eps, float *lds, int &turn, float *mean_out = nullptr) const {
     const float per = 1.0f / (float)d;
     if (!rms) {
       float s[1] = {0.f};
@@ -112,11 +131,9 @@ struct RnRow {
       const float mean = s[0] * per;
       if (mean_out) *mean_out = mean;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const bool in = col(lane, i) < d;
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < VW; ++j) r[i * VW + j] = in ? r[i * VW + j] - mean : 0.f;
-      }
+        for (int j = 0; j < VW; ++j) r[i * VW + j] = own(i, j) ? r[i * VW + j] - mean : 0.f;
     }
     float q[1] = {0.f};
 #pragma unroll
@@ -128,8 +145,7 @@ struct RnRow {
     return inv;
   }
   // gradient of the normalisation: dz -> d(input), z = the normalised row; ab: mean(dz z), mean(dz)
-  PQN_D static void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, int d, int lane, float *lds, int &turn,
-                                   float *ab = nullptr) {
+  PQN_D void normalise_back(float (&dz)[E], const float (&z)[E], float inv, int rms, float *lds, int &turn, float *ab = nullptr) const {
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -143,11 +159,9 @@ struct RnRow {
       ab[1] = b;
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = col(lane, i) < d;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < VW; ++j) dz[i * VW + j] = in ? (fmaf(-z[i * VW + j], a, dz[i * VW + j]) - b) * inv : 0.f;
-    }
+      for (int j = 0; j < VW; ++j) dz[i * VW + j] = own(i, j) ? (fmaf(-z[i * VW + j], a, dz[i * VW + j]) - b) * inv : 0.f;
   }
 };
 
@@ -167,33 +181,34 @@ PQN_D void rn_act(int kind, float g, float &act, float &slope) {
 }
 
 // A wave per row (NT = 64, four to a workgroup) or a workgroup per row, walking over the rows.
-template <typename T, int NT, int VW, int NV, int ACT>
+template <typename T, int NT, int VW, int NV, bool LOOSE, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
-  using Row = RnRow<T, NT, VW, NV>;
+  using Row = RnRow<T, NT, VW, NV, LOOSE>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
   constexpr bool KEEP = NT < 1024;        // the parameters stay in registers, and the next row is in flight
   __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63;
   const int d = A.d;
+  const Row rw = {d, lane};
   int turn = 0;
   long long row = (long long)blockIdx.x * RPB + (NT > 64 ? 0 : threadIdx.x >> 6);
   const long long step = (long long)gridDim.x * RPB;
   if (row >= A.n) return;                 // whole waves / workgroups
   typename Row::Pack fx[NV], ff[NV], fg[NV];
   auto fetch = [&](long long r) {
-    Row::fetch(ff, A.f, r * A.fs, d, lane);
-    if constexpr (ACT != PQN_GATE_NONE) Row::fetch(fg, A.g, r * A.gs, d, lane);
-    Row::fetch(fx, A.x, r * A.xs, d, lane);
+    rw.fetch(ff, A.f, r * A.fs);
+    if constexpr (ACT != PQN_GATE_NONE) rw.fetch(fg, A.g, r * A.gs);
+    rw.fetch(fx, A.x, r * A.xs);
   };
   float ps[E], pb[E], rs[E], qs[E], qb[E];
   auto params_in = [&]() {
-    Row::param(ps, A.post_scale, 1.f, d, lane);
-    Row::param(pb, A.post_bias, 0.f, d, lane);
-    Row::param(rs, A.res_scale, 1.f, d, lane);
+    rw.param(ps, A.post_scale, 1.f);
+    rw.param(pb, A.post_bias, 0.f);
+    rw.param(rs, A.res_scale, 1.f);
   };
   auto params_out = [&]() {
-    Row::param(qs, A.pre_scale, 1.f, d, lane);
-    Row::param(qb, A.pre_bias, 0.f, d, lane);
+    rw.param(qs, A.pre_scale, 1.f);
+    rw.param(qb, A.pre_bias, 0.f);
   };
   if constexpr (KEEP) {
     fetch(row);
@@ -203,11 +218,11 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
   for (; row < A.n; row += step) {
     float z[E], y[E], g[E];
     if constexpr (!KEEP) fetch(row);
-    Row::open(z, ff, d, lane);
-    Row::open(y, fx, d, lane);
-    if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
+    rw.open(z, ff);
+    rw.open(y, fx);
+    if constexpr (ACT != PQN_GATE_NONE) rw.open(g, fg);
     if (KEEP && row + step < A.n) fetch(row + step);
-    if (A.has_post) Row::normalise(z, A.rms, A.eps, d, lane, lds, turn);
+    if (A.has_post) rw.normalise(z, A.rms, A.eps, lds, turn);
     if constexpr (!KEEP) params_in();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -215,13 +230,13 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
       rn_act(ACT, g[e], act, slope);
       y[e] = fmaf(rs[e], act * fmaf(z[e], ps[e], pb[e]), y[e]);
     }
-    Row::store(A.y, row * d, y, d, lane);
+    rw.store(A.y, row * d, y);
     if (A.has_pre) {
-      Row::normalise(y, A.rms, A.eps, d, lane, lds, turn);
+      rw.normalise(y, A.rms, A.eps, lds, turn);
       if constexpr (!KEEP) params_out();
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = fmaf(y[e], qs[e], qb[e]);
-      Row::store(A.h, row * d, y, d, lane);
+      rw.store(A.h, row * d, y);
     }
   }
 }
@@ -229,15 +244,16 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_fwd_kernel(rn_args A) {
 // The parameter gradients are summed over a thread's rows in registers and leave the workgroup as one partial row per parameter,
 // summed in a fixed order by rn_param_kernel (the same result in every run).  NT = 1024 has no registers for the sums: it leaves the
 // row's statistics instead, and rn_sums_kernel reads the rows a second time.
-template <typename T, int NT, int VW, int NV, int ACT>
+template <typename T, int NT, int VW, int NV, bool LOOSE, int ACT>
 __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
-  using Row = RnRow<T, NT, VW, NV>;
+  using Row = RnRow<T, NT, VW, NV, LOOSE>;
   constexpr int E = Row::E, RPB = NT > 64 ? 1 : 4;
   constexpr bool KEEP = NT < 1024, SUMS = KEEP;
   __shared__ float lds[NT > 64 ? 4 * NT / 64 : 1];
   __shared__ float fold[NT > 64 ? 1 : 3 * 64 * E];
   const int lane = NT > 64 ? threadIdx.x : threadIdx.x & 63, wave = NT > 64 ? 0 : threadIdx.x >> 6;
   const int d = A.d;
+  const Row rw = {d, lane};
   int turn = 0;
   float sum[SUMS ? RN_PARAMS : 1][E];
   if constexpr (SUMS)
@@ -249,31 +265,31 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
   const long long step = (long long)gridDim.x * RPB;
   typename Row::Pack fx[NV], ff[NV], fg[NV], fy[NV], fh[NV];
   auto fetch = [&](long long r) {
-    Row::fetch(ff, A.f, r * A.fs, d, lane);
-    if constexpr (ACT != PQN_GATE_NONE) Row::fetch(fg, A.g, r * A.gs, d, lane);
-    Row::fetch(fx, A.x, r * A.xs, d, lane);
-    if (A.dh) Row::fetch(fh, A.dh, r * A.dhs, d, lane);
-    if (A.dy) Row::fetch(fy, A.dy, r * A.dys, d, lane);
+    rw.fetch(ff, A.f, r * A.fs);
+    if constexpr (ACT != PQN_GATE_NONE) rw.fetch(fg, A.g, r * A.gs);
+    rw.fetch(fx, A.x, r * A.xs);
+    if (A.dh) rw.fetch(fh, A.dh, r * A.dhs);
+    if (A.dy) rw.fetch(fy, A.dy, r * A.dys);
   };
   if (KEEP && row < A.n) fetch(row);
   float ps[E], pb[E], rs[E], qs[E];
   auto params = [&]() {
-    Row::param(ps, A.post_scale, 1.f, d, lane);
-    Row::param(pb, A.post_bias, 0.f, d, lane);
-    Row::param(rs, A.res_scale, 1.f, d, lane);
+    rw.param(ps, A.post_scale, 1.f);
+    rw.param(pb, A.post_bias, 0.f);
+    rw.param(rs, A.res_scale, 1.f);
   };
   if constexpr (KEEP) {
     params();
-    Row::param(qs, A.pre_scale, 1.f, d, lane);
+    rw.param(qs, A.pre_scale, 1.f);
   }
   for (; row < A.n; row += step) {
     float z[E], y[E], e_[E], g[E], dh[E];
     if constexpr (!KEEP) fetch(row);
-    Row::open(z, ff, d, lane);
-    Row::open(y, fx, d, lane);
-    if constexpr (ACT != PQN_GATE_NONE) Row::open(g, fg, d, lane);
-    if (A.dh) Row::open(dh, fh, d, lane);
-    if (A.dy) Row::open(e_, fy, d, lane);
+    rw.open(z, ff);
+    rw.open(y, fx);
+    if constexpr (ACT != PQN_GATE_NONE) rw.open(g, fg);
+    if (A.dh) rw.open(dh, fh);
+    if (A.dy) rw.open(e_, fy);
     else
 #pragma unroll
       for (int e = 0; e < E; ++e) e_[e] = 0.f;
@@ -281,7 +297,7 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
     if constexpr (!KEEP) params();
     float inv_f = 1.f, act[E], slope[E];
     RnStat st = {0.f, 1.f, 0.f, 1.f, 0.f, 0.f};
-    if (A.has_post) inv_f = Row::normalise(z, A.rms, A.eps, d, lane, lds, turn, &st.mean_f);
+    if (A.has_post) inv_f = rw.normalise(z, A.rms, A.eps, lds, turn, &st.mean_f);
     st.inv_f = inv_f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -289,9 +305,9 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
       y[e] = fmaf(rs[e], act[e] * fmaf(z[e], ps[e], pb[e]), y[e]);
     }
     if (A.dh) {
-      const float inv_y = Row::normalise(y, A.rms, A.eps, d, lane, lds, turn, &st.mean_y);
+      const float inv_y = rw.normalise(y, A.rms, A.eps, lds, turn, &st.mean_y);
       st.inv_y = inv_y;
-      if constexpr (!KEEP) Row::param(qs, A.pre_scale, 1.f, d, lane);
+      if constexpr (!KEEP) rw.param(qs, A.pre_scale, 1.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if constexpr (SUMS) {
@@ -300,11 +316,11 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
         }
         dh[e] *= qs[e];
       }
-      Row::normalise_back(dh, y, inv_y, A.rms, d, lane, lds, turn, &st.a);
+      rw.normalise_back(dh, y, inv_y, A.rms, lds, turn, &st.a);
 #pragma unroll
       for (int e = 0; e < E; ++e) e_[e] += dh[e];
     }
-    Row::store(A.dx, row * d, e_, d, lane);
+    rw.store(A.dx, row * d, e_);
     if constexpr (!KEEP) params();          // read and made again rather than held
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -318,9 +334,9 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
       }
       e_[e] = dn * ps[e];
     }
-    if constexpr (ACT != PQN_GATE_NONE) Row::store(A.dg, row * d, g, d, lane);
-    if (A.has_post) Row::normalise_back(e_, z, inv_f, A.rms, d, lane, lds, turn);
-    Row::store(A.df, row * d, e_, d, lane);
+    if constexpr (ACT != PQN_GATE_NONE) rw.store(A.dg, row * d, g);
+    if (A.has_post) rw.normalise_back(e_, z, inv_f, A.rms, lds, turn);
+    rw.store(A.df, row * d, e_);
     if (!SUMS && threadIdx.x == 0) A.stats[row] = st;
   }
   if constexpr (!SUMS) return;
@@ -338,20 +354,22 @@ __global__ __launch_bounds__(NT > 64 ? NT : 256) void rn_bwd_kernel(rn_args A) {
         for (int e = 0; e < E; ++e)
           sum[k][e] = ((sum[k][e] + fold[e * 64 + lane]) + fold[(E + e) * 64 + lane]) + fold[(2 * E + e) * 64 + lane];
     }
-    if (wave == 0)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = Row::col(lane, i);
-        if (c < d) pqn_store<float, VW>(out + (size_t)k * d + c, sum[k] + i * VW);
-      }
+    if (wave == 0) rw.store(out + (size_t)k * d, sum[k]);
   }
 }
 
 // The parameter gradients of wide rows: a thread's VW columns over the rows of its slice, from the statistics that rn_bwd_kernel left.
-template <typename T, int VW, int ACT>
+template <typename T, int VW, bool LOOSE, int ACT>
 __global__ __launch_bounds__(256) void rn_sums_kernel(rn_args A) {
-  const int d = A.d, c = (blockIdx.x * 256 + threadIdx.x) * VW;
-  if (c >= d) return;
+  const int d = A.d, mine = (blockIdx.x * 256 + threadIdx.x) * VW;
+  if (mine >= d) return;
+  const int c = LOOSE ? min(mine, d - VW) : mine;            // as in RnRow
+  typedef typename std::conditional<LOOSE, pqn_loose<T, VW>, pqn_pack<T, VW>>::type Pack;
+  auto load = [&](float (&r)[VW], const void *base, long long off) {
+    const Pack x = *(const Pack *)((const T *)base + off + c);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) r[e] = pqn_to_f32(x.v[e]);
+  };
   float ps[VW], pb[VW], rs[VW], qs[VW], sum[RN_PARAMS][VW];
   auto param = [&](float (&r)[VW], const float *p, float absent) {
 #pragma unroll
@@ -367,11 +385,11 @@ __global__ __launch_bounds__(256) void rn_sums_kernel(rn_args A) {
     for (int e = 0; e < VW; ++e) sum[k][e] = 0.f;
   for (long long row = blockIdx.y; row < A.n; row += gridDim.y) {
     float x[VW], f[VW], g[VW], dy[VW], dh[VW];
-    pqn_load<T, VW>(f, (const T *)A.f + row * A.fs + c);
-    pqn_load<T, VW>(x, (const T *)A.x + row * A.xs + c);
-    if constexpr (ACT != PQN_GATE_NONE) pqn_load<T, VW>(g, (const T *)A.g + row * A.gs + c);
-    if (A.dh) pqn_load<T, VW>(dh, (const T *)A.dh + row * A.dhs + c);
-    if (A.dy) pqn_load<T, VW>(dy, (const T *)A.dy + row * A.dys + c);
+    load(f, A.f, row * A.fs);
+    load(x, A.x, row * A.xs);
+    if constexpr (ACT != PQN_GATE_NONE) load(g, A.g, row * A.gs);
+    if (A.dh) load(dh, A.dh, row * A.dhs);
+    if (A.dy) load(dy, A.dy, row * A.dys);
     const RnStat st = A.stats[row];
 #pragma unroll
     for (int e = 0; e < VW; ++e) {
@@ -395,7 +413,8 @@ __global__ __launch_bounds__(256) void rn_sums_kernel(rn_args A) {
 #pragma unroll
   for (int k = 0; k < RN_PARAMS; ++k)
 #pragma unroll
-    for (int e = 0; e < VW; ++e) out[(size_t)k * d + e] = sum[k][e];
+    for (int e = 0; e < VW; ++e)
+      if (c + e >= mine) out[(size_t)k * d + e] = sum[k][e];
 }
 
 // column sums of the partials: COLS columns x 1024 / COLS row groups per workgroup, fixed order
@@ -425,7 +444,7 @@ __global__ __launch_bounds__(1024) void rn_param_kernel(const float *__restrict_
 // ---------------------------------------------------------------------------------------------------------------------------
 // Threads per row: as few as hold it at 8 columns each -- a wave up to 512 columns (no barrier then), then 128 to 1024 threads, the
 // last without the registers for parameters and a row in flight.  Vector accesses of up to 16 B where width, strides and pointers allow
-// them, else one element per lane and access.
+// them, else one element per lane and access, or (over RN_WIDE columns) accesses that start anywhere (RnRow).
 static int rn_threads(int d) { return d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024; }
 // Workgroups: enough to fill the chip (8 waves per SIMD asked for by the forward, 2 by the gradient with its sums in registers), each
 // walking over its rows; the gradient leaves a partial row per workgroup and parameter, wide rows one per slice of rn_sums_kernel.
@@ -442,38 +461,37 @@ static int rn_launch_act(const rn_args &A, bool vec, hipStream_t st) {
   constexpr int VW = 16 / (int)sizeof(T);
   const int nt = rn_threads(A.d);
   const unsigned grid = rn_blocks(A.n, A.d, BWD);
-#define RN_GO(NT, W, NVV)                                                                                         \
+#define RN_GO(NT, W, NVV, LOOSE)                                                                                  \
   do {                                                                                                            \
-    if constexpr (BWD) rn_bwd_kernel<T, NT, W, NVV, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                 \
-    else rn_fwd_kernel<T, NT, W, NVV, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                               \
+    if constexpr (BWD) rn_bwd_kernel<T, NT, W, NVV, LOOSE, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);          \
+    else rn_fwd_kernel<T, NT, W, NVV, LOOSE, ACT><<<grid, NT > 64 ? NT : 256, 0, st>>>(A);                        \
     return pqn_check_launch(BWD ? "pqn_residual_norm_grad" : "pqn_residual_norm");                                \
   } while (0)
   if (vec) {
-    if (A.d <= 128) RN_GO(64, 2, 1);
-    if (A.d <= 256) RN_GO(64, 4, 1);
-    if (nt == 64) RN_GO(64, VW, 8 / VW);
-    if (nt == 128) RN_GO(128, VW, 8 / VW);
-    if (nt == 256) RN_GO(256, VW, 8 / VW);
-    if (nt == 512) RN_GO(512, VW, 8 / VW);
-    RN_GO(1024, VW, 8 / VW);
+    if (A.d <= 128) RN_GO(64, 2, 1, false);
+    if (A.d <= 256) RN_GO(64, 4, 1, false);
+    if (nt == 64) RN_GO(64, VW, 8 / VW, false);
+    if (nt == 128) RN_GO(128, VW, 8 / VW, false);
+    if (nt == 256) RN_GO(256, VW, 8 / VW, false);
+    if (nt == 512) RN_GO(512, VW, 8 / VW, false);
+    RN_GO(1024, VW, 8 / VW, false);
   }
-  if (A.d <= 128) RN_GO(64, 1, 2);
-  if (nt == 64) RN_GO(64, 1, 8);
-  if (nt == 128) RN_GO(128, 1, 8);
-  if (nt == 256) RN_GO(256, 1, 8);
-  if (nt == 512) RN_GO(512, 1, 8);
-  RN_GO(1024, 1, 8);
+  if (A.d <= 128) RN_GO(64, 1, 2, false);
+  if (nt == 64) RN_GO(64, 1, 8, false);
+  if (nt == 128) RN_GO(128, 1, 8, false);
+  if (nt == 256) RN_GO(256, 1, 8, false);
+  if (nt == 512) RN_GO(512, 1, 8, false);
+  RN_GO(1024, VW, 8 / VW, true);
 #undef RN_GO
 }
 template <typename T>
 static int rn_launch_sums(const rn_args &A, bool vec, hipStream_t st) {
   constexpr int VW = 16 / (int)sizeof(T);
-  const int w = vec ? VW : 1;
-  const dim3 grid((A.d + 256 * w - 1) / (256 * w), rn_parts(A.n, A.d));
+  const dim3 grid((A.d + 256 * VW - 1) / (256 * VW), rn_parts(A.n, A.d));
 #define RN_GO(ACT)                                                       \
   if (A.gate_act == ACT) {                                               \
-    if (vec) rn_sums_kernel<T, VW, ACT><<<grid, 256, 0, st>>>(A);        \
-    else rn_sums_kernel<T, 1, ACT><<<grid, 256, 0, st>>>(A);             \
+    if (vec) rn_sums_kernel<T, VW, false, ACT><<<grid, 256, 0, st>>>(A); \
+    else rn_sums_kernel<T, VW, true, ACT><<<grid, 256, 0, st>>>(A);      \
   }
   RN_GO(PQN_GATE_NONE)
   RN_GO(PQN_GATE_SIGMOID)

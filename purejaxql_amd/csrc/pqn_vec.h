@@ -10,11 +10,17 @@ PQN_D float pqn_to_f32(float x) { return x; }
 PQN_D float pqn_to_f32(pqn_bf16 x) { return (float)x; }
 PQN_D float pqn_to_f32(pqn_f16 x) { return (float)x; }
 
-// W consecutive elements in one access (the caller has checked the alignment of W * sizeof(T) bytes)
+// W consecutive elements in one access (the caller has checked the alignment of W * sizeof(T) bytes); pqn_loose: of any element's
+// alignment, which global memory takes in one access too
 template <typename T, int W>
 struct pqn_pack {
   T v[W];
 } __attribute__((aligned(W * sizeof(T) > 16 ? 16 : W * sizeof(T))));
+
+template <typename T, int W>
+struct pqn_loose {
+  T v[W];
+};
 
 template <typename T, int W>
 PQN_D void pqn_load(float *dst, const T *src) {
