@@ -188,7 +188,8 @@ static constexpr int DA_MIN_PART = 64, DA_FILL = 2048;
 
 static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int vec) {
   da_split X = {};
-  const long long waves = rows * passes * da_nw(a, b, vec);
+  const int nw = da_nw(a, b, vec);
+  const long long waves = rows * passes * (nw == 3 ? 4 : nw);     // a CU holds as many workgroups of three waves as of four
   long long want = (DA_FILL + waves - 1) / (waves > 0 ? waves : 1);
   const long long most = t_len / DA_MIN_PART;
   if (want > most) want = most;
@@ -347,13 +348,14 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
   if (!da_by_steps(a, true)) {
     const int vec = da_vec(a, 1);
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
-    // dq and dk have states of [dv][dk], dv of [dk][dv].  One launch of the kernel that holds both where that is the kernel of each, or
-    // where there is little to do in several launches (the time axis is cut) and they are more than the padding.  Measured on both
-    // sides, together / one after the other, us: 300 steps x 6 rows, 32 and 128 columns, f32 48 / 77, bf16 33 / 57; 1001 x 35, 48 and 80,
-    // f32 166 / 148, bf16 79 / 90; 5000 x 8, 64 and 128, bf16 75 / 114; 4000 x 160, 32 and 64, f32 782 / 582, bf16 328 / 281; 32 x 512,
-    // 80 and 48, f32 61 / 52 (not cut).
+    // dq and dk have states of [dv][dk], dv of [dk][dv].  One launch of the kernel that holds both where that is nearly the kernel of
+    // each, or where there is little to do in several launches (the time axis is cut) and they are more than the padding.  Measured on
+    // both sides, together / one after the other, us: 300 steps x 6 rows, 32 and 128 columns, f32 48 / 77, bf16 33 / 57; 1001 x 35, 48
+    // and 80, f32 166 / 148, bf16 79 / 90; 5000 x 8, 64 and 128, bf16 75 / 114; 4000 x 160, 32 and 64, f32 782 / 582, bf16 328 / 281;
+    // 32 x 512, 80 and 48, f32 61 / 52 (not cut); 300 x 480, 128 and 96, bf16 133 / 165.
     const int w = a->dk > a->dv ? a->dk : a->dv, least = a->dk + a->dv - w;
-    const bool alike = da_ap(least, vec) == da_ap(w, vec) && da_nw(least, w, vec) == da_nw(w, w, vec) && da_nw(w, least, vec) == da_nw(w, w, vec);
+    const bool same = da_ap(least, vec) == da_ap(w, vec) && da_nw(least, w, vec) == da_nw(w, w, vec) && da_nw(w, least, vec) == da_nw(w, w, vec);
+    const bool alike = same || least > 64 || (least > 32 && w <= 64);
     const long long rows = (long long)a->m * a->heads;
     if (alike || (a->t_len * rows <= (a->dtype == PQN_DTYPE_F32 ? 1 << 14 : 1 << 16) && da_cut(a->t_len, rows, 3, w, w, vec).parts > 1))
       return da_run_chunks(A, 3, a->dtype, vec, a->workspace, (hipStream_t)stream);

@@ -69,8 +69,8 @@ PQN_D int da_col(int c, int r) { return 2 * r + c; }
 template <typename T, int W>
 struct DaTile {
   static constexpr int EV = 16 / (int)sizeof(T);
-  static constexpr int LD = sizeof(T) == 2 ? W : W + 4;
-  static constexpr int SHIFT = W >= 128 ? 0 : W == 64 ? 1 : 2;   // rows that share the 64 banks: 1, 2, 4
+  static constexpr int LD = sizeof(T) == 2 ? (W == 96 ? 128 : W) : W + 4;   // bf16: a power of two of slots
+  static constexpr int SHIFT = W >= 96 ? 0 : W == 64 ? 1 : 2;   // rows that share the 64 banks: 1, 2, 4
   PQN_D static int at(int row, int col) {
     if constexpr (sizeof(T) == 2) {
       const int swz = (((row & 3) >> SHIFT) << 2) | ((row >> 2) & 3);
@@ -178,14 +178,15 @@ PQN_D void da_mfma2(f32x4_t a0, f32x4_t a1, f32x4_t b0, f32x4_t b1, f32x4_t (&c)
 template <typename T, int W, int L, int NTHR, bool VEC, bool PAIRS>
 struct DaLoad {
   static constexpr int EV = 16 / (int)sizeof(T), VPR = W / EV, STEP = NTHR / VPR, N = (L + STEP - 1) / STEP;
-  static_assert(NTHR % VPR == 0, "whole rows per pass");
+  // threads behind the last whole row of a pass do the next pass's first row as well, the same values to the same place
+  static constexpr bool EVEN = NTHR % VPR == 0 && L % STEP == 0;
   u32x4_t r[N];
   const T *p;                       // this lane's first row and column of the chunk
   long long stride;
   int width;
   PQN_D static int row0() { return threadIdx.x / VPR; }
   PQN_D static int col() { return threadIdx.x % VPR * EV; }
-  PQN_D static bool inside(int row) { return L % STEP == 0 || row < L; }
+  PQN_D static bool inside(int row) { return EVEN || row < L; }
   PQN_D void start(const T *first, long long stride_, int width_) {
     stride = stride_;
     width = width_;
@@ -203,7 +204,7 @@ struct DaLoad {
     }
   }
   PQN_D void load(int n) {          // n >= 1
-    if (n == L && L % STEP == 0) {
+    if (n == L && EVEN) {
 #pragma unroll
       for (int i = 0; i < N; ++i) fetch(i, p + i * STEP * stride);
     } else
@@ -686,11 +687,12 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
   }
 }
 
-// widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave.  Tensors whose rows are not whole 16-byte
-// accesses go element by element, in fewer forms.
-inline int da_ap(int a, int vec) { return a <= 32 && vec ? 32 : a <= 64 ? 64 : 128; }
+// widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave.  96 beside the powers of two: 200 steps x 800
+// rows of 96 x 96, forward / gradient, f32 138 / 331 us, padded to 128 172 / 415, bf16 60 / 134 and 70 / 160.  Tensors whose rows are not
+// whole 16-byte accesses go element by element, in fewer forms.
+inline int da_ap(int a, int vec) { return a <= 32 && vec ? 32 : a <= 64 ? 64 : a <= 96 && vec ? 96 : 128; }
 inline int da_nw(int a, int b, int vec) {
-  const int nw = b <= 32 ? 1 : b <= 64 ? 2 : 4;
+  const int nw = b <= 32 ? 1 : b <= 64 ? 2 : b <= 96 && vec ? 3 : 4;
   return !vec ? a > 64 || nw == 4 ? 4 : 2 : a > 64 && nw < 2 ? 2 : nw;    // a wave alone would hold 128 registers of loads in flight
 }
 // the kernel for passes of unequal widths is the one that holds the widest
@@ -716,11 +718,17 @@ static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool
   }
   DA_GO(32, 1, true)
   DA_GO(32, 2, true)
+  DA_GO(32, 3, true)
   DA_GO(32, 4, true)
   DA_GO(64, 1, true)
   DA_GO(64, 2, true)
+  DA_GO(64, 3, true)
   DA_GO(64, 4, true)
+  DA_GO(96, 2, true)
+  DA_GO(96, 3, true)
+  DA_GO(96, 4, true)
   DA_GO(128, 2, true)
+  DA_GO(128, 3, true)
   DA_GO(128, 4, true)
   DA_GO(64, 2, false)
   DA_GO(64, 4, false)

@@ -95,6 +95,13 @@ def test_decay_attention_and_gradient(gpu, shape, dtype):
     _attn_check(_attn_inputs(gpu, *shape, dtype, seed=sum(shape)), scale=shape[3] ** -0.5)
 
 
+@pytest.mark.parametrize("dk,dv", [(96, 96), (80, 16), (24, 88), (72, 64), (96, 128), (128, 72), (88, 40)])
+@pytest.mark.parametrize("t,m,h", [(20, 3, 2), (33, 40, 3), (300, 2, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_decay_attention_widths_between_powers_of_two(gpu, t, m, h, dk, dv, dtype):
+    _attn_check(_attn_inputs(gpu, t, m, h, dk, dv, dtype, dk + dv, True, 0.02), scale=dk ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("state,resets,spread", [(False, 0.0, False), (True, 0.0, True), (False, 0.5, True), (True, 1.0, False)])
 def test_decay_attention_states_resets_strides(gpu, dtype, state, resets, spread):
