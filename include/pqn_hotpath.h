@@ -652,7 +652,8 @@ int pqn_bigmlp_gemm(int32_t m, int32_t n, int32_t k, const float *a, int64_t lda
  * linear attention with a decay per head (the memory), the norms around a residual block, the log probabilities of taken actions.
  * Tensors are f32, bf16 or f16 as `dtype` says; sums, states, statistics and parameters are f32, and a 16-bit output is rounded once,
  * to nearest even.  Strides count elements; the last index of every tensor is contiguous, outputs are contiguous.  Outputs must not
- * overlap inputs unless an entry says so.  Workspaces are scratch of one call: two calls that may run at the same time need two. */
+ * overlap inputs unless an entry says so.  Workspaces are scratch of one call: two calls that may run at the same time need two.  A
+ * call that one launch of 2^32 threads does not cover (some 2^26 (row, head) pairs, 2^29 rows of a few logits) is refused. */
 enum { PQN_DTYPE_F32 = 0, PQN_DTYPE_BF16 = 1, PQN_DTYPE_F16 = 2 };
 
 /* Linear attention with a decay per head, cut at episode ends (the role of ScannedRNN, pqn_rnn_gymnax.py:26-54: resets come BEFORE

@@ -149,6 +149,7 @@ static int da_launch_recur(const da_args &A, int passes, hipStream_t st) {
     vec = vec && P.s_cs == 1 && P.b % 4 == 0 && (((uintptr_t)P.s_in | (uintptr_t)P.s_out) & 15) == 0;
   }
   const long long units = (long long)A.m * A.heads * cbmax, blocks = (units + 3) / 4;
+  PQN_REQUIRE(pqn_one_launch(blocks, 256), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
   const dim3 grid((unsigned)blocks, passes);
 #define DA_GO(RPT)                                                          \
   do {                                                                      \

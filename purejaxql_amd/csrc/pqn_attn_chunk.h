@@ -45,7 +45,7 @@ struct da_args {
 // (heads of 128, 128 steps x 2048 rows, bf16, gradient: 267 us).  Next chunk's loads are in flight in registers while a chunk is computed.
 // Measured, forward / gradient: bf16, 128 steps x 2048 rows of 128 x 128: 128 / 267 us (floors 106 / 171 by the bytes at 5.08 TB/s); f32,
 // 32 steps x 16384 rows of 32 x 32: 118 / 267 us (79 / 132; the three scans of the gradient read the window nearly twice); one step of
-// 8192 bf16 rows of 128 x 128: 216 us, 5.0 TB/s; f32, 1001 steps x 35 rows of 48 x 80: 52 / 148 us (latency: three launches a scan, each
+// 8192 bf16 rows of 128 x 128: 216 us, 5.0 TB/s; f32, 1001 steps x 35 rows of 48 x 80: 50 / 124 us (latency: three launches a scan, each
 // a few chunks deep).
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef pqn_bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -708,7 +708,7 @@ template <typename T, int L>
 static int da_launch_chunk(const da_args &A, const da_split &X, int passes, bool state, hipStream_t st) {
   const int a = da_widest(A, passes, &da_pass::a), ap = da_ap(a, X.vec), nw = da_nw(a, da_widest(A, passes, &da_pass::b), X.vec);
   const long long units = (long long)A.m * A.heads * (state ? X.parts - 1 : X.parts), grid = (units + 7) / 8 * 8 * passes;
-  PQN_REQUIRE(grid < (1ll << 31), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
+  PQN_REQUIRE(pqn_one_launch(grid, 64 * nw), "pqn_decay_attn: %d x %d rows and heads are more than one launch covers", A.m, A.heads);
 #define DA_GO(AP, NW, VEC)                                                                                                   \
   if (ap == AP && nw == NW && (X.vec != 0) == VEC) {                                                                         \
     if (state) da_chunk_kernel<T, AP, NW, L, VEC, DA_STATE><<<(unsigned)grid, 64 * NW, 0, st>>>(A, X, passes);               \

@@ -10,9 +10,9 @@
 // the order of the work.
 //
 // Bound: HBM for many logits (about 9 vector operations and one v_exp_f32 a logit, below the time its bytes take), latency for few.
-// Measured, forward / gradient: 4096 x 32000 bf16, five alternatives, 85 / 84 us at best (3.1 / 6.2 TB/s: the gradient's reads come from
-// the last-level cache in part); 131072 x 17 f32 with masks and three alternatives 9.0 / 8.6 us (vector work of joining 17 logits over
-// lanes); 8 x 100003 bf16, eight alternatives, 10.7 us and 6.5 us for joining 25 parts a row (latency).
+// Measured, forward / gradient: 4096 x 32000 bf16, five alternatives 61 / 96 us, none 49 (4.3 - 5.4 TB/s; part of the gradient's reads
+// come from the last-level cache); 131072 x 17 f32 with masks and three alternatives 8.8 / 8.3 us (vector work of joining 17 logits over
+// lanes); 8 x 100003 bf16, eight alternatives, 8.3 us and 6.8 us for joining 25 parts a row (latency).
 #include <type_traits>
 
 #include "pqn_vec.h"
@@ -570,9 +570,9 @@ static lp_args lp_fill(const pqn_action_logprobs_t *a) {
   return A;
 }
 
-// Rows of up to LP_ROW_MAX logits live in a wave's registers (lp_rows_kernel or lp_long_kernel), longer ones in a workgroup's, up to 16 accesses a thread (32768 16-bit or
-// 16384 f32 logits); beyond that, or where there are too few rows to fill the chip, a row is cut (a part keeps at least LP_MIN_PART
-// logits, below which the join costs more than it gives).
+// Rows of up to LP_ROW_MAX logits live in a wave's registers (lp_rows_kernel or lp_long_kernel), longer ones in a workgroup's, up to 16
+// accesses a thread (32768 16-bit or 16384 f32 logits); beyond that, or where there are too few rows to fill the chip, a row is cut (a
+// part keeps at least LP_MIN_PART logits, below which the join costs more than it gives).
 static constexpr int LP_ROW_MAX = 1024, LP_NT = 256, LP_MIN_PART = 4096, LP_FILL = 1024, LP_MOST = 16;
 static int lp_splits(int n, int a, int vw) {
   if (a <= LP_ROW_MAX) return 1;
@@ -603,6 +603,8 @@ static int lp_launch(lp_args A, hipStream_t st) {
   if (A.a <= 256 || (A.a <= 512 && A.top <= 3) || (A.a <= LP_ROW_MAX && A.top <= 1)) {
 #define LP_GO(G, E)                                                                           \
   do {                                                                                        \
+    PQN_REQUIRE(pqn_one_launch(((long long)A.n * G + 255) / 256, 256),                        \
+                "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a); \
     lp_rows_kernel<T, G, E><<<(unsigned)(((long long)A.n * G + 255) / 256), 256, 0, st>>>(A); \
     return pqn_check_launch("pqn_action_logprobs");                                           \
   } while (0)
@@ -614,7 +616,7 @@ static int lp_launch(lp_args A, hipStream_t st) {
   A.part = lp_part(A.a, A.splits);
   A.splits = (A.a + A.part - 1) / A.part;
   const long long grid = (long long)A.n * A.splits;
-  PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a);
+  PQN_REQUIRE(pqn_one_launch(grid, LP_NT), "pqn_action_logprobs: %d x %d logits are more than one launch covers", A.n, A.a);
   const int each = (A.part + LP_NT * VW - 1) / (LP_NT * VW);
   // few accesses: a wave or two to a row, with less to join.  16000 x 4000 bf16, 8 alternatives, 128 / 256 threads 52 / 69 us; 60000 x
   // 1100, 64 / 256 threads 88 / 195
@@ -638,6 +640,8 @@ static int lp_launch_grad(lp_grad_args P, hipStream_t st) {
   if (A.a <= LP_ROW_MAX) {
 #define LP_GO(G, E)                                                                                \
   do {                                                                                             \
+    PQN_REQUIRE(pqn_one_launch(((long long)A.n * G + 255) / 256, 256),                             \
+                "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", A.n, A.a); \
     lp_grad_rows_kernel<T, G, E><<<(unsigned)(((long long)A.n * G + 255) / 256), 256, 0, st>>>(P); \
     return pqn_check_launch("pqn_action_logprobs_grad");                                           \
   } while (0)
@@ -650,7 +654,7 @@ static int lp_launch_grad(lp_grad_args P, hipStream_t st) {
   const int span = 256 * LP_SPAN * (vec ? VW : 1);
   P.blocks = (A.a + span - 1) / span;
   const long long grid = (long long)A.n * P.blocks;
-  PQN_REQUIRE(grid < (1ll << 31), "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", A.n, A.a);
+  PQN_REQUIRE(pqn_one_launch(grid, 256), "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", A.n, A.a);
   if (vec) lp_grad_kernel<T, VW><<<(unsigned)grid, 256, 0, st>>>(P);
   else lp_grad_kernel<T, 1><<<(unsigned)grid, 256, 0, st>>>(P);
   return pqn_check_launch("pqn_action_logprobs_grad");

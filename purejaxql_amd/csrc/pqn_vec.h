@@ -81,6 +81,8 @@ PQN_D uint32_t pqn_group_max(uint32_t x) {
   return pqn_group_fold<G>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
+// a launch covers fewer than 2^32 threads along its first axis
+inline bool pqn_one_launch(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
 inline int pqn_dtype_size(int dtype) { return dtype == PQN_DTYPE_F32 ? 4 : 2; }
 inline bool pqn_dtype_known(int dtype) { return dtype == PQN_DTYPE_F32 || dtype == PQN_DTYPE_BF16 || dtype == PQN_DTYPE_F16; }
 // f(T{}) with the element type of `dtype` (checked before)

@@ -50,6 +50,26 @@ def test_attention_refusals(kw, says):
     assert says in lib.pqn_last_error().decode()
 
 
+@pytest.mark.parametrize("kw", [{"t_len": 1, "m": 1 << 27}, {"t_len": 100, "m": 1 << 25, "dk": 128, "dv": 128}, {"t_len": 100, "m": 1 << 26, "dtype": 1}])
+def test_attention_of_more_rows_than_a_launch(kw):
+    from purejaxql_amd import _lib
+    lib = _lib.load()
+    assert lib.pqn_decay_attn(C.byref(_attn(**kw)), None) == -1 and "more than one launch" in lib.pqn_last_error().decode()
+    kw = dict(kw, dout=64, dq=64, dk_out=64, dv_out=64)
+    assert lib.pqn_decay_attn_grad(C.byref(_attn(**kw)), None) == -1 and "more than one launch" in lib.pqn_last_error().decode()
+
+
+@pytest.mark.parametrize("n,a", [((1 << 31) - 1, 7), (1 << 30, 20), (1 << 28, 60), (1 << 26, 900), (1 << 25, 3000), (1 << 21, 1 << 21)])
+def test_log_probabilities_of_more_rows_than_a_launch(n, a):
+    from purejaxql_amd import _lib
+    lib = _lib.load()
+    args = _lib.ActionLogprobsArgs(n=n, a=a, top=0, dtype=1, temperature=1.0, logits=64, logits_stride=a, action=64, logp=64, entropy=64, lse=64,
+                                   dlogp=64, dlogits=64, workspace=64)
+    assert lib.pqn_action_logprobs(C.byref(args), None) == -1 and "more than one launch" in lib.pqn_last_error().decode()
+    if a > 100:
+        assert lib.pqn_action_logprobs_grad(C.byref(args), None) == -1 and "more than one launch" in lib.pqn_last_error().decode()
+
+
 def test_attention_gradient_refusals():
     from purejaxql_amd import _lib
     lib = _lib.load()
