@@ -420,7 +420,7 @@ def make_train(config: Dict[str, Any], device: Optional[str] = None, grad_hook: 
     # Round 6 root cause of the round-5 fault (16 seeds x 4096 envs with evaluations died after ~16 updates): the HIP runtime
     # bundled in the PyTorch wheel (ROCm 7.0.51831 in torch/lib, the one a Python process loads) faults after ~25 replays of a
     # long hipGraph launched on the NULL stream when eager launches are queued behind the replay; on a created stream, or
-    # with /opt/rocm's 7.2 runtime, the same program is clean (tools/repro/update_replay.cpp, profiles/r06_v2_null_stream_fault.txt).
+    # with /opt/rocm's 7.2 runtime, the same program is clean (profiles/r06_v2_null_stream_fault.txt).
     # config _WORK_STREAM=False keeps the caller's current stream (the regression test's negative control).
     work_stream = torch.cuda.Stream(dev) if config.get("_WORK_STREAM", True) else None
     if config.get("SEED_BATCH_BIT_IDENTICAL", False):

@@ -1,5 +1,5 @@
 """Regression for the round-5 GPU memory access fault: 16 seeds x 4096 envs of Breakout with the yaml default
-TEST_DURING_TRAINING=True died after ~16 updates.  Root cause (round 6, tools/repro/update_replay.cpp): the HIP runtime bundled in
+TEST_DURING_TRAINING=True died after ~16 updates.  Root cause (round 6): the HIP runtime bundled in
 the PyTorch wheel faults when a long hipGraph is replayed on the legacy NULL stream with eager launches queued behind the replay;
 make_train now runs everything on a created stream.  Each case runs in a child process: a fault aborts the process, and the suite
 should report a failure instead of dying with it.  Reference behaviour matched: evaluations inside the training loop
