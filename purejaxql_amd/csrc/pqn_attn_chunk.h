@@ -34,13 +34,14 @@ struct da_args {
 // shares V's fragments with it.  The columns of q, k, v are assigned to accumulator rows so that a lane's 8 values of two stacked
 // 16 x 16 tiles are 8 neighbouring columns (da_row, da_col): one 16-byte read of Q, one 16-byte store of O.
 //
-// bf16: v_mfma_f32_16x16x32_bf16 with the state (S^T Q^T) and the weighted products (V^T P^T) rounded to bf16 as operands -- the
-// output is rounded to bf16 anyway -- and w V split in three bf16 pieces, which hold it exactly, because the state is an f32 result
-// that is carried on (two pieces left it 3e-6 off after some hundred steps).  f32: v_mfma_f32_16x16x4_f32 throughout, four of them per
-// 16 values of k.
+// bf16: v_mfma_f32_16x16x32_bf16.  What is f32 and an operand -- the state (S^T Q^T), the weighted products (V^T P^T), w V -- is three bf16
+// pieces, which hold it exactly: sums and states are f32 and an output is rounded once.  With the state and the weights as one bf16 number
+// each (2.5e-3 rms on the outputs instead of 1.7e-3, their own rounding) 128 steps x 2048 rows of 128 x 128 took 123 / 266 us, now 137 / 321:
+// 111 matrix instructions a chunk and wave instead of 71, and some 300 vector instructions.  f32: v_mfma_f32_16x16x4_f32 throughout, four
+// of them per 16 values of k.
 //
 // Bound: HBM where there are rows enough.  A chunk of 32 steps of 128 + 128 bf16 columns moves 32 KB (about 3900 cycles of a CU's share
-// of the bandwidth) and costs a wave 71 matrix instructions of 16 cycles; f32 doubles the bytes and costs four times the instructions at
+// of the bandwidth) and costs a wave 111 matrix instructions of 16 cycles; f32 doubles the bytes and costs four times the instructions at
 // 32 cycles each, about as much as the bytes.  Chunks of 32 steps and not 64: half the registers in flight, no spills, two waves a SIMD
 // (heads of 128, 128 steps x 2048 rows, bf16, gradient: 267 us).  Next chunk's loads are in flight in registers while a chunk is computed.
 // Measured, forward / gradient: bf16, 128 steps x 2048 rows of 128 x 128: 128 / 267 us (floors 106 / 171 by the bytes at 5.08 TB/s); f32,
@@ -140,6 +141,21 @@ PQN_D void da_mfma6(bf16x8_t a, const bf16x8_t (&b)[2][3], f32x4_t (&c)[2]) {
                "v_mfma_f32_16x16x32_bf16 %0, %2, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %2, %8, %1"
                : "+v"(c[0]), "+v"(c[1])
                : "v"(a), "v"(b[0][0]), "v"(b[0][1]), "v"(b[0][2]), "v"(b[1][0]), "v"(b[1][1]), "v"(b[1][2]));
+}
+// the three pieces of a by b, both of a by the three pieces of b
+PQN_D void da_mfma6(const bf16x8_t (&a)[2][3], bf16x8_t b, f32x4_t (&c)[2]) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %8, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %5, %8, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %3, %8, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %6, %8, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %4, %8, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %7, %8, %1"
+               : "+v"(c[0]), "+v"(c[1])
+               : "v"(a[0][0]), "v"(a[0][1]), "v"(a[0][2]), "v"(a[1][0]), "v"(a[1][1]), "v"(a[1][2]), "v"(b));
+}
+PQN_D void da_mfma6(const bf16x8_t (&a)[2], const bf16x8_t (&b)[3], f32x4_t (&c)[2]) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %4, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %4, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %2, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %5, %1\n\t"
+               "v_mfma_f32_16x16x32_bf16 %0, %2, %6, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %6, %1"
+               : "+v"(c[0]), "+v"(c[1])
+               : "v"(a[0]), "v"(a[1]), "v"(b[0]), "v"(b[1]), "v"(b[2]));
 }
 // waits for the products before it and hands on their results: the one wait for all of x
 template <typename F, int N>
@@ -273,6 +289,27 @@ PQN_D uint32_t da_pair(float a, float b) { return __builtin_bit_cast(uint32_t, _
 PQN_D float da_low(uint32_t p) { return __uint_as_float(p << 16); }
 PQN_D float da_high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// f32 numbers as the sum of three bf16 ones, exactly: the leading 8 bits of what is left, three times (cut off, not rounded: the largest
+// floats stay finite).  da_cut3 takes one piece of a pair off it.
+PQN_D uint32_t da_cut3(float &a, float &b) {
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  a -= __uint_as_float(ua & 0xffff0000u);
+  b -= __uint_as_float(ub & 0xffff0000u);
+  return __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+}
+PQN_D void da_pieces(f32x4_t a, f32x4_t b, bf16x8_t (&x)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    u32x4_t u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = da_cut3(v[2 * e], v[2 * e + 1]);
+    x[k] = __builtin_bit_cast(bf16x8_t, u);
+    a = f32x4_t{v[0], v[1], v[2], v[3]};
+    b = f32x4_t{v[4], v[5], v[6], v[7]};
+  }
+}
+
 struct da_split {       // the time axis in `parts` parts of `len` steps, one workgroup each; parts = 1: not cut
   int parts, len;
   int vec;              // every row of every tensor of the launch starts on 16 bytes and is whole 16-byte accesses
@@ -352,6 +389,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
   constexpr bool B16 = sizeof(T) == 2, STATE = MODE == DA_STATE;
   constexpr int NTHR = 64 * NW, BP = 32 * NW, KB = B16 ? 32 : 16, NF = AP / KB, NS = AP / 16, NJ = L / KB, NT = L / 16;
   constexpr int EV = 16 / (int)sizeof(T), PER = KB / 16, OUT = B16 ? 1 : 2;
+  constexpr int PIECES = B16 ? 3 : 1;   // operands that an f32 number is in a product
   // The weights between the steps of a chunk: the waves share the tiles out and exchange them through LDS.  A wave alone keeps them in
   // its registers, where they lie as the next product's operand already.
   constexpr bool SHARE = NW > 1 && !STATE;
@@ -361,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
   typedef DaTile<T, AP> TA;
   typedef DaTile<T, BP> TB;
   typedef DaTile<T, L> TP;
-  __shared__ __attribute__((aligned(16))) T Qs[STATE || ALIAS ? 8 : L * TA::LD], Ks[L * TA::LD], Ps[SHARE ? L * TP::LD : 8];
+  __shared__ __attribute__((aligned(16))) T Qs[STATE || ALIAS ? 8 : L * TA::LD], Ks[L * TA::LD], Ps[SHARE ? PIECES * L * TP::LD : 8];
   __shared__ __attribute__((aligned(16))) T Vs[L * (ALIAS && TA::LD > TB::LD ? TA::LD : TB::LD)];
   T *const Q = ALIAS ? Vs : Qs;
   __shared__ __attribute__((aligned(16))) float pw[L + 4];
@@ -542,34 +580,48 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
             p = weights(tt, jt, qf);
           }
           if constexpr (B16) {                                   // in the order of DaTile::cols
-            uint32_t *dst = (uint32_t *)(Ps + TP::at(16 * tt + ln, 32 * (jt >> 1) + 8 * g + 4 * (jt & 1)));
-            dst[0] = da_pair(p[0], p[1]);
-            dst[1] = da_pair(p[2], p[3]);
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+              uint32_t *dst = (uint32_t *)(Ps + k * L * TP::LD + TP::at(16 * tt + ln, 32 * (jt >> 1) + 8 * g + 4 * (jt & 1)));
+              float v[4] = {p[0], p[1], p[2], p[3]};
+              dst[0] = da_cut3(v[0], v[1]);
+              dst[1] = da_cut3(v[2], v[3]);
+              p = f32x4_t{v[0], v[1], v[2], v[3]};
+            }
           } else *(f32x4_t *)(Ps + TP::at(16 * tt + ln, 16 * jt + 4 * g)) = p;
         }
       }
       __syncthreads();
     }
     if constexpr (!STATE) {
-      F sf[NF][2];
+      f32x4_t os[B16 ? NT : 1][2];                               // bf16: the state is cut in pieces once for all steps
+      if constexpr (B16) {
 #pragma unroll
-      for (int f = 0; f < NF; ++f)
+        for (int tt = 0; tt < NT; ++tt) os[tt][0] = os[tt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if constexpr (B16) {
-            const f32x4_t a = s[2 * f][c], b = s[2 * f + 1][c];
-            sf[f][c] = __builtin_bit_cast(F, (u32x4_t{da_pair(a[0], a[1]), da_pair(a[2], a[3]), da_pair(b[0], b[1]), da_pair(b[2], b[3])}));
-          } else sf[f][c] = s[f][c];
+        for (int f = 0; f < NF; ++f) {
+          F sp[2][PIECES];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) da_pieces(s[2 * f][c], s[2 * f + 1][c], sp[c]);
+#pragma unroll
+          for (int tt = 0; tt < NT; ++tt)
+            if (16 * tt < n) da_mfma6(sp, TA::template rows<F>(Q, 16 * tt, f * KB), os[tt]);
+        }
+        da_drain<F>(os);
+      }
 #pragma unroll
       for (int tt = 0; tt < NT; ++tt) {
         if (16 * tt >= n) continue;
+        f32x4_t (&o)[2] = os[B16 ? tt : 0];
         F qf[NF];
+        if constexpr (!B16 || !SHARE)
 #pragma unroll
-        for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Q, 16 * tt, f * KB);
-        f32x4_t o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          for (int f = 0; f < NF; ++f) qf[f] = TA::template rows<F>(Q, 16 * tt, f * KB);
+        if constexpr (!B16) {
+          o[0] = o[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int f = 0; f < NF; ++f) da_mfma2(sf[f][0], sf[f][1], qf[f], qf[f], o);
-        da_drain<F>(o);
+          for (int f = 0; f < NF; ++f) da_mfma2(s[f][0], s[f][1], qf[f], qf[f], o);
+        }
         const float wc = pw[16 * tt + ln + first] * P.o_scale;
         if (cuts) {                                              // a choice, not a product: the state may be NaN
           const bool carried = (cuts & ((2ull << (16 * tt + ln)) - 1ull)) == 0;
@@ -585,20 +637,22 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if (j * KB >= 16 * (tt + 1)) continue;
-          F pf;
-          if constexpr (SHARE) pf = TP::template rows<F>(Ps, 16 * tt, j * KB);
-          else if constexpr (B16) {
-            u32x4_t u = {0u, 0u, 0u, 0u};
+          F pf[PIECES];
+          if constexpr (SHARE)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (2 * j + half > tt) continue;
-              const f32x4_t p = weights(tt, 2 * j + half, qf);
-              u[2 * half] = da_pair(p[0], p[1]);
-              u[2 * half + 1] = da_pair(p[2], p[3]);
+            for (int k = 0; k < PIECES; ++k) pf[k] = TP::template rows<F>(Ps + k * L * TP::LD, 16 * tt, j * KB);
+          else {
+            f32x4_t p[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              if (PER * j + i > tt) p[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+              else p[i] = weights(tt, PER * j + i, qf);
             }
-            pf = __builtin_bit_cast(F, u);
-          } else pf = weights(tt, j, qf);
-          da_mfma2(vf[j][0], vf[j][1], pf, pf, o);
+            if constexpr (B16) da_pieces(p[0], p[1], pf);
+            else pf[0] = p[0];
+          }
+          if constexpr (B16) da_mfma6(vf[j], pf, o);
+          else da_mfma2(vf[j][0], vf[j][1], pf[0], pf[0], o);
         }
         da_drain<F>(o);
         if constexpr (B16)
@@ -632,7 +686,6 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
     for (int j = 0; j < NJ; ++j) {
       if (j * KB >= n) continue;
       if constexpr (MODE == DA_ONE) weigh_state(j, n, cuts);
-      constexpr int PIECES = B16 ? 3 : 1;
       F x[2][PIECES];                                  // w v is its pieces' sum exactly
 #pragma unroll
       for (int c = 0; c < 2; ++c) {

@@ -25,6 +25,105 @@ def scan(asm_path):
     return hits
 
 
+REG = re.compile(r'\bv(?:\[(\d+):(\d+)\]|(\d+)\b)')
+WAIT = 11      # wait states between v_mfma_f32_16x16x32_bf16 (8 passes) and another instruction's access to its result
+LABEL = re.compile(r'^([.\w$]+):')
+
+
+def _regs(text):
+    out = set()
+    for lo, hi, one in REG.findall(text):
+        out.update(range(int(lo), int(hi) + 1) if lo else (int(one),))
+    return out
+
+
+def _blocks(lines):
+    """[(label, [(line number, mnemonic, operands)], successors)] of one kernel's text"""
+    blocks, cur = [], ["", [], set()]
+    for ln, line in lines:
+        line = line.split(";")[0].strip()
+        m = LABEL.match(line)
+        if m:
+            cur[2].add(m.group(1))
+            blocks.append(cur)
+            cur = [m.group(1), [], set()]
+            continue
+        if not line or line.startswith("."):
+            continue
+        op, _, rest = line.partition(" ")
+        cur[1].append((ln, op, rest))
+        if op.startswith("s_cbranch") or op == "s_branch":
+            cur[2].add(rest.strip())
+            if op == "s_branch":
+                blocks.append(cur)
+                cur = ["after line %d" % ln, [], set()]
+        elif op == "s_endpgm":
+            blocks.append(cur)
+            cur = ["after line %d" % ln, [], set()]
+    return blocks + [cur]
+
+
+def _walk(block, left, hits):
+    """Runs a block from the registers that still wait ({register: wait states}); what waits behind every branch and at its end"""
+    out, left = {}, dict(left)
+
+    def to(label):
+        have = out.setdefault(label, {})
+        for r, n in left.items():
+            have[r] = max(have.get(r, 0), n)
+
+    for ln, op, rest in block[1]:
+        if op == "v_mfma_f32_16x16x32_bf16":
+            d, a, b, c = (_regs(x) for x in re.split(r",\s*(?![^\[]*\])", rest)[:4])
+            if (a | b) & set(left) or (c != d and (c | d) & set(left)):
+                hits.append((ln, op + " " + rest))
+        elif _regs(rest) & set(left):
+            hits.append((ln, op + " " + rest))
+        passed = int(rest) + 1 if op == "s_nop" else 1
+        left = {r: n - passed for r, n in left.items() if n > passed}
+        if op == "v_mfma_f32_16x16x32_bf16":
+            left.update({r: WAIT for r in d})
+        if op.startswith("s_cbranch") or op == "s_branch":
+            to(rest.strip())
+    for label in block[2]:
+        if not any(op.startswith(("s_cbranch", "s_branch")) and rest.strip() == label for _, op, rest in block[1]):
+            to(label)
+    return out
+
+
+def scan_unfinished(asm_path):
+    """The bf16 products are asm, whose results the compiler takes for ready at once: every access to one but the next product of its
+    chain has to lie WAIT wait states behind it, on every path (a copy or a spill that the compiler puts between is found here)."""
+    hits, kernel, cur = [], None, []
+    kernels = []
+    for ln, line in enumerate(open(asm_path), 1):
+        if line.startswith("_Z") and ":" in line:
+            kernel, cur = line.split(":")[0], []
+            kernels.append((kernel, cur))
+        elif line.startswith(".Lfunc_end"):
+            kernel = None
+        elif kernel:
+            cur.append((ln, line))
+    for name, lines in kernels:
+        blocks = _blocks(lines)
+        at = {b[0]: {} for b in blocks}
+        todo, found = [b for b in blocks], set()
+        by = {b[0]: b for b in blocks}
+        while todo:
+            b = todo.pop()
+            mine = []
+            for label, left in _walk(b, at[b[0]], mine).items():
+                if label not in at:
+                    continue
+                more = {r: n for r, n in left.items() if n > at[label].get(r, 0)}
+                if more:
+                    at[label].update(more)
+                    todo.append(by[label])
+            found.update(mine)
+        hits += [(name, ln, text) for ln, text in sorted(found)]
+    return hits
+
+
 M0_OK = re.compile(r'^\s*s_mov_b32 m0, s\d+\s*$')
 
 
@@ -44,7 +143,7 @@ def main():
             extra = ["-fno-slp-vectorize"] if os.path.basename(f) == "pqn_qnet_pos.hip" else []     # as the Makefile builds it
             subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *extra,
                             "--cuda-device-only", "-S", f, "-o", out], check=True, cwd=CSRC, stderr=subprocess.DEVNULL)
-            hits = scan(out)
+            hits, early = scan(out), scan_unfinished(out)
             if os.path.basename(f) == "pqn_qnet_pos.hip":
                 m0 = scan_m0(out)
                 print("%-20s %d uses of M0 other than the LDS-DMA destination writes" % (os.path.basename(f), len(m0)))
@@ -54,7 +153,10 @@ def main():
         print("%-20s %d partially overlapping MFMA D/C" % (os.path.basename(f), len(hits)))
         for k, ln, l in hits[:12]:
             print("    %s:%d  %s" % (k[:50], ln, l))
-        bad += len(hits)
+        print("%-20s %d accesses to the result of a bf16 product within %d wait states" % (os.path.basename(f), len(early), WAIT))
+        for k, ln, l in early[:12]:
+            print("    %s:%d  %s" % (k[:50], ln, l))
+        bad += len(hits) + len(early)
     sys.exit(1 if bad else 0)
 
 
