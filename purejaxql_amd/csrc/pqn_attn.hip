@@ -172,15 +172,16 @@ static bool da_vec(const pqn_decay_attn_t *a, int grad) {
   return vec;
 }
 
-// Windows of up to this many steps go step by step, longer ones by chunks.  Measured on both sides, us forward / gradient: 4096 x 4 heads
-// of 32, f32, 2 steps 30 / 90 against 46 / 113 by chunks, 4 steps 37 / 110 against 45 / 107, 6 steps 46 / 135 against 45 / 107; 1024 x 8
-// heads of 64, f32, 1 step 48 / 137 against 75 / 175; 1024 x 8 heads of 128, 1 step, f32 218 / 585 against 224 / 508, bf16 216 / 657
-// against 196 / 356, 2 steps bf16 257 / 806 against 213 / 366.  Off 16 bytes chunks load element by element: 1000 x 4 heads of 127, 3 steps
-// f32 212 / 396 against 238 / 547, 2 steps bf16 219 / 395 against 216 / 521, 4 steps bf16 275 / 575 against 219 / 528; 4000 x 8 heads of 33
-// and 65, 3 steps bf16 328 / 1170 against 645 / 2429.
+// Windows of up to this many steps go step by step, longer ones by chunks; a single step of the forward always does, so that a row acts
+// alike (to the bit) whatever number of rows acts beside it.  Measured on both sides, us forward / gradient: 4096 x 4 heads of 32, f32, 2
+// steps 30 / 90 against 46 / 113 by chunks, 4 steps 37 / 110 against 45 / 107, 6 steps 46 / 135 against 45 / 107; 1024 x 8 heads of 64, f32,
+// 1 step 48 / 137 against 75 / 175; 1024 x 8 heads of 128, 1 step, f32 218 / 585 against 224 / 508, bf16 218 / 657 against 205 / 441; bf16
+// steps in place of 1024 x 8 heads: 128 x 128 225 against 212, 72 x 128 133 against 198, 128 x 32 54 against 110; 256 x 8 of 96 x 96 32 and
+// 41.  Off 16 bytes chunks load element by element: 1000 x 4 heads of 127, 3 steps f32 212 / 396 against 238 / 547, 2 steps bf16 219 / 395
+// against 216 / 521, 4 steps bf16 275 / 575 against 219 / 528; 4000 x 8 heads of 33 and 65, 3 steps bf16 328 / 1170 against 645 / 2429.
 static bool da_by_steps(const pqn_decay_attn_t *a, bool grad) {
   const int w = a->dk > a->dv ? a->dk : a->dv;
-  return a->t_len <= (w <= 32 ? 4 : !da_vec(a, grad) ? 3 : w <= 64 || (a->dtype == PQN_DTYPE_F32 && !grad) || (long long)a->m * a->heads < 2048 ? 1 : 0);
+  return a->t_len <= (w <= 32 ? 4 : !da_vec(a, grad) ? 3 : w <= 64 || !grad || (long long)a->m * a->heads < 2048 ? 1 : 0);
 }
 // The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
 // reading of k and v and a state written and read), as many as make DA_FILL waves.  Measured, 1001 steps x 35 rows of 48 and 80 columns,

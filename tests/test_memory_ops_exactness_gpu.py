@@ -30,3 +30,16 @@ def test_bf16_outputs_are_rounded_once(gpu, t, m, h, dk, dv):
     for name, g, w, a in zip(("dq", "dk", "dv"), got, want, most):
         _close(g, w, n * a + half * (w.abs() + n * a), name)
     _close(got[3], want[3], n * most[3] + 1e-30, "dstate")
+
+
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 64), (128, 128), (96, 72), (67, 128)])
+def test_a_row_steps_alike_alone_and_among_many(gpu, dk, dv):
+    """An env acts the same whatever runs beside it: a row's step has the same bits in a batch of 5 rows and in one of 700."""
+    from purejaxql_amd import ops
+    for dtype in (BF16, torch.float32):
+        x = _attn_inputs(gpu, 1, 700, 4, dk, dv, dtype, dk + dv, True, 0.3)
+        few, many = x["state"][:5].clone(), x["state"].clone()
+        args = [x[n][0] for n in ("q", "k", "v")]
+        a = ops.decay_attention_step(*(z[:5] for z in args), x["decay"], few, reset=x["reset"][0, :5], scale=0.3)
+        b = ops.decay_attention_step(*args, x["decay"], many, reset=x["reset"][0], scale=0.3)
+        assert torch.equal(a, b[:5]) and torch.equal(few, many[:5]), dtype
