@@ -462,21 +462,34 @@ __global__ __launch_bounds__(64) void lp_join_kernel(lp_args A) {
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
 // d/dx_j = dlogp (1[j = action] - p_j) - dentropy p_j (log p_j + H) + dlse p_j, over the temperature.
+// log p_j = x_j - lse puts every p_j of a row off by e^(the rounding of lse): nothing beside the sum's own rounding where |lse| <= LP_NEAR
+// (2^-24 * 32, a sum over A logits some (64 + A / 64) 2^-24), 28 % for logits / temperature of 4e6.  So rows of larger ones take
+// log p_j = (logit_j - m) / temperature - log_s from the largest logit and the sum of the powers, made again: from registers in narrow
+// rows, by reading a wide row a second time.  us, |lse| <= 32 / above (of the forward's lse alone): 4096 x 32000 bf16
+// 100 / 154 (97), 60000 x 1100 bf16 85 / 215 (76), 512 x 130000 f32 99 / 235 (97), 8 x 100003 bf16 9 / 22 (9), 60000 x 1000 f32 82 / 86 (86).
+static constexpr float LP_NEAR = 32.f;
 struct lp_grad_args {
   lp_args A;
   const float *dlogp, *dentropy, *dlse;
   void *dlogits;                     // [n][a]
-  int blocks;                        // wide rows: workgroups per row
+  int blocks, far;                   // wide rows: workgroups per row; those of them that work on a row beyond LP_NEAR
 };
+// the largest of a set of logits and s = sum 2^((logit - m) log2 e / temperature); empty: -inf and 0
+struct LpPowers {
+  float m, s;
+};
+PQN_D float lp_rescale(float m, float to, float scale) { return m == to ? 1.f : lp_exp2((m - to) * scale); }
 struct LpGrad {                      // a row's scalars
-  float lse, h, dlp, dh, dl, inv_temp;
+  float m, base, h, dlp, dh, dl, inv_temp;      // log p = (logit - m) / temperature - base
   int act;
-  bool none;
+  bool none, near;
   template <typename T>
   PQN_D void open(const lp_grad_args &G, long long row) {
     const lp_args &A = G.A;
-    lse = A.lse[row];
-    none = fabsf(lse) == INFINITY;       // nothing allowed, or beyond the largest float
+    m = 0.f;
+    base = A.lse[row];
+    near = !(fabsf(base) > LP_NEAR);     // NaN: so is every gradient
+    none = fabsf(base) == INFINITY;      // nothing allowed, or beyond the largest float
     h = A.entropy[row];
     act = A.action[row];
     dlp = G.dlogp ? G.dlogp[row] : 0.f;
@@ -486,8 +499,12 @@ struct LpGrad {                      // a row's scalars
     // an id outside the row, or an action that is not allowed, has a constant log probability
     if (act < 0 || act >= A.a || lp_logit<T>(A, row, act) == -INFINITY) dlp = 0.f;
   }
+  PQN_D void sums(LpPowers v) {
+    m = v.m;
+    base = LP_LN2 * log2f(v.s);
+  }
   PQN_D float at(float x, int j) const {               // x: the logit, -inf where not allowed
-    const float lp = fmaf(x, inv_temp, -lse), q = lp_exp2(lp * LP_LOG2E);
+    const float lp = fmaf(x - m, inv_temp, -base), q = lp_exp2(lp * LP_LOG2E);
     const float c = dl - dlp - dh * (fmaxf(lp, -1000.f) + h);          // q is 0 below
     const float g = ((act == j ? dlp : 0.f) + q * c) * inv_temp;
     return x == -INFINITY || none ? 0.f : g;
@@ -498,51 +515,160 @@ template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void lp_grad_rows_kernel(lp_grad_args P) {
   const lp_args &A = P.A;
   const int lane = threadIdx.x & (G - 1);
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
-  if (row >= A.n) return;
+  const long long row0 = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+  const bool live = row0 < A.n;                    // rows behind the last one go along with a copy of it
+  const long long row = live ? row0 : A.n - 1;
   LpGrad R;
   R.open<T>(P, row);
   T *o = (T *)P.dlogits + row * A.a;
   float x[E];
   lp_row_load<T, G, E>(A, row, lane, x);
+  if (__any(!R.near)) {                            // whole waves, for the exchanges
+    LpPowers v = {-INFINITY, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) v.m = fmaxf(v.m, x[e]);
+    v.m = pqn_group_fmax<G>(v.m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v.s += x[e] == -INFINITY ? 0.f : lp_exp2((x[e] - v.m) * A.scale);
+    v.s = pqn_group_sum<G>(v.s);
+    if (!R.near) R.sums(v);
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = e * G + lane;
-    if (j < A.a) o[j] = (T)R.at(x[e], j);
+    if (live && j < A.a) o[j] = (T)R.at(x[e], j);
   }
 }
-// wide rows: `blocks` workgroups to a row, LP_SPAN accesses of VW logits a lane.  Rows whose logits and gradients lie alike on 16
-// bytes take whole accesses, their first and last elements one to a lane.
-static constexpr int LP_SPAN = 4;
-template <typename T, int VW>
+// A wide row's columns: whole accesses of the logits lie on 16 bytes, from `head` to `end`; the first and last elements go one to a thread.
+// The gradients' accesses start anywhere.
+template <typename T>
+struct LpWide {
+  static constexpr int VW = 16 / (int)sizeof(T);
+  const T *x;
+  const uint8_t *mk;
+  T *o;
+  int head, end, jr;
+  bool has_rest;
+  float xr;
+  PQN_D LpWide(const lp_grad_args &P, long long row) {
+    const lp_args &A = P.A;
+    x = (const T *)A.logits + row * A.ls;
+    mk = A.mask ? A.mask + row * A.ms : nullptr;
+    o = (T *)P.dlogits + row * A.a;
+    head = min(A.a, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+    end = head + (A.a - head) / VW * VW;
+    has_rest = (int)threadIdx.x < head + (A.a - end);
+    jr = (int)threadIdx.x < head ? threadIdx.x : end + (threadIdx.x - head);
+    xr = !has_rest || (mk && !mk[jr]) ? -INFINITY : pqn_to_f32(x[jr]);
+  }
+  // the sums of the whole row, the same in every thread; eight accesses requested together
+  PQN_D LpPowers sums(float scale, LpPowers *part) const {
+    constexpr int BATCH = 8;
+    LpPowers v = {fmaxf(xr, -INFINITY), 0.f};        // not a NaN
+    v.s = xr == -INFINITY ? 0.f : lp_exp2((xr - v.m) * scale);
+    for (int j0 = head; j0 < end; j0 += 256 * VW * BATCH) {
+      lp_u32x4 r[BATCH];
+      auto at = [&](int i) { return j0 + (i * 256 + (int)threadIdx.x) * VW; };
+      auto some = [&](int i) { return j0 + i * 256 * VW < end; };
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        r[i] = lp_u32x4{0u, 0u, 0u, 0u};
+        if (some(i)) r[i] = *(const lp_u32x4 *)(x + (at(i) < end ? at(i) : head));
+      }
+      float top = v.m;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (!some(i)) continue;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          if (mk) lp_forbid<T>(r[i], e, mk[min(at(i) + e, end - 1)] == 0);
+          lp_forbid<T>(r[i], e, at(i) >= end);
+          top = fmaxf(top, lp_get<T>(r[i], e));
+        }
+      }
+      v.s *= lp_rescale(v.m, top, scale);
+      v.m = top;
+      const float m = top == -INFINITY ? 0.f : top;  // nothing yet: 2^-inf, or NaN
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (!some(i)) continue;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) v.s += lp_exp2((lp_get<T>(r[i], e) - m) * scale);
+      }
+    }
+    const float m = pqn_group_fmax<64>(v.m), s = pqn_wave_sum(v.s * lp_rescale(v.m, m, scale));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {m, s};
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) v.m = fmaxf(v.m, part[w].m);
+    v.s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v.s += part[w].s * lp_rescale(part[w].m, v.m, scale);
+    return v;
+  }
+  PQN_D void rest(const LpGrad &R) const {
+    if (has_rest) o[jr] = (T)R.at(xr, jr);
+  }
+  // span b, SPAN accesses a thread.  Each is requested where it is used: the four at once measured slower (16000 x 4000 bf16 52 us against 45,
+  // 8192 x 8000 f32 with a mask 149 against 130).
+  static constexpr int SPAN = 4;
+  PQN_D void write(const LpGrad &R, int b) const {
+#pragma unroll
+    for (int i = 0; i < SPAN; ++i) {
+      const int j = head + ((b * SPAN + i) * 256 + (int)threadIdx.x) * VW;
+      if (j >= end) break;
+      float v[VW];
+      pqn_load<T, VW>(v, x + j);
+      pqn_loose<T, VW> g;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) g.v[e] = (T)R.at(mk && !mk[j + e] ? -INFINITY : v[e], j + e);
+      *(pqn_loose<T, VW> *)(o + j) = g;
+    }
+  }
+};
+// `blocks` workgroups to a row, a span each.  Rows beyond LP_NEAR are left to lp_grad_far_kernel, or (ALONE) `far` of the workgroups make the
+// row's sums, each for itself, and take the spans in turn.
+template <typename T, bool ALONE>
 __global__ __launch_bounds__(256) void lp_grad_kernel(lp_grad_args P) {
-  const lp_args &A = P.A;
   const long long row = blockIdx.x / P.blocks;
   const int block = blockIdx.x % P.blocks;
   LpGrad R;
   R.open<T>(P, row);
-  const T *x = (const T *)A.logits + row * A.ls;
-  const uint8_t *mk = A.mask ? A.mask + row * A.ms : nullptr;
-  T *o = (T *)P.dlogits + row * A.a;
-  int head = 0;
-  if constexpr (VW > 1) {
-    head = min(A.a, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
-    const int tail = (A.a - head) % VW;
-    if (block == 0 && (int)threadIdx.x < head + tail) {
-      const int j = (int)threadIdx.x < head ? threadIdx.x : A.a - tail + (threadIdx.x - head);
-      o[j] = (T)R.at(mk && !mk[j] ? -INFINITY : pqn_to_f32(x[j]), j);
+  const bool again = !R.near && !R.none;           // the workgroup's row: the same in every thread
+  if (again && !(ALONE && block < P.far)) return;
+  const LpWide<T> W(P, row);
+  int step = P.blocks;
+  if constexpr (ALONE) {
+    __shared__ LpPowers part[4];
+    if (again) {
+      R.sums(W.sums(P.A.scale, part));
+      step = P.far;
     }
   }
-  const int end = head + (A.a - head) / VW * VW;
-#pragma unroll
-  for (int i = 0; i < LP_SPAN; ++i) {
-    const int j = head + ((block * LP_SPAN + i) * 256 + (int)threadIdx.x) * VW;
-    if (j >= end) break;
-    float v[VW];
-    pqn_load<T, VW>(v, x + j);
-#pragma unroll
-    for (int e = 0; e < VW; ++e) v[e] = R.at(mk && !mk[j + e] ? -INFINITY : v[e], j + e);
-    pqn_store<T, VW>(o + j, v);
+  if (block == 0) W.rest(R);
+  for (int b = block; b < P.blocks; b += step) W.write(R, b);
+}
+// rows beyond LP_NEAR, a workgroup to each: it looks for them among every gridDim.x-th row, 64 at a time
+template <typename T>
+__global__ __launch_bounds__(256) void lp_grad_far_kernel(lp_grad_args P) {
+  __shared__ LpPowers part[4];
+  const int lane = threadIdx.x & 63;
+  for (long long row0 = blockIdx.x; row0 < P.A.n; row0 += 64ll * gridDim.x) {
+    const long long mine = row0 + (long long)lane * gridDim.x;
+    const float lse = mine < P.A.n ? P.A.lse[mine] : 0.f;
+    unsigned long long todo = __ballot(fabsf(lse) > LP_NEAR && fabsf(lse) < INFINITY);      // the same in every wave
+    while (todo) {
+      const long long row = row0 + (long long)(__ffsll(todo) - 1) * gridDim.x;
+      todo &= todo - 1;
+      LpGrad R;
+      R.open<T>(P, row);
+      const LpWide<T> W(P, row);
+      R.sums(W.sums(P.A.scale, part));
+      W.rest(R);
+      for (int b = 0; b < P.blocks; ++b) W.write(R, b);
+      __syncthreads();                             // `part` has been read
+    }
   }
 }
 
@@ -648,15 +774,21 @@ static int lp_launch_grad(lp_grad_args P, hipStream_t st) {
     LP_ROW_SHAPES(LP_GO, A.a)
 #undef LP_GO
   }
-  constexpr int VW = 16 / (int)sizeof(T);
-  // every row's logits and gradients the same way off 16 bytes
-  const bool vec = (((uintptr_t)A.logits - (uintptr_t)P.dlogits) & 15) == 0 && (A.ls - A.a) % VW == 0;
-  const int span = 256 * LP_SPAN * (vec ? VW : 1);
+  constexpr int span = 256 * LpWide<T>::SPAN * (16 / (int)sizeof(T));
   P.blocks = (A.a + span - 1) / span;
   const long long grid = (long long)A.n * P.blocks;
   PQN_REQUIRE(pqn_one_launch(grid, 256), "pqn_action_logprobs_grad: %d x %d logits are more than one launch covers", A.n, A.a);
-  if (vec) lp_grad_kernel<T, VW><<<(unsigned)grid, 256, 0, st>>>(P);
-  else lp_grad_kernel<T, 1><<<(unsigned)grid, 256, 0, st>>>(P);
+  // Few workgroups: rows beyond LP_NEAR in the same launch, several workgroups to each though every one reads all of the row
+  if (grid <= LP_FILL) {
+    const int far = LP_FILL / A.n;
+    P.far = far < 32 ? far : 32;
+    lp_grad_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(P);
+    return pqn_check_launch("pqn_action_logprobs_grad");
+  }
+  lp_grad_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(P);
+  const int rc = pqn_check_launch("pqn_action_logprobs_grad");
+  if (rc != PQN_OK) return rc;
+  lp_grad_far_kernel<T><<<(unsigned)(A.n < 2048 ? A.n : 2048), 256, 0, st>>>(P);
   return pqn_check_launch("pqn_action_logprobs_grad");
 }
 
@@ -684,6 +816,6 @@ extern "C" int pqn_action_logprobs_grad(const pqn_action_logprobs_t *a, void *st
   PQN_REQUIRE(a->dlogits, "pqn_action_logprobs_grad: NULL dlogits");
   PQN_REQUIRE(a->dlogp || a->dentropy || a->dlse, "pqn_action_logprobs_grad: dlogp, dentropy and dlse are all NULL");
   return pqn_with_dtype(a->dtype, [&](auto t) {
-    return lp_launch_grad<decltype(t)>({lp_fill(a), a->dlogp, a->dentropy, a->dlse, a->dlogits, 0}, (hipStream_t)stream);
+    return lp_launch_grad<decltype(t)>({lp_fill(a), a->dlogp, a->dentropy, a->dlse, a->dlogits, 0, 0}, (hipStream_t)stream);
   });
 }

@@ -43,3 +43,78 @@ def test_a_row_steps_alike_alone_and_among_many(gpu, dk, dv):
         a = ops.decay_attention_step(*(z[:5] for z in args), x["decay"], few, reset=x["reset"][0, :5], scale=0.3)
         b = ops.decay_attention_step(*args, x["decay"], many, reset=x["reset"][0], scale=0.3)
         assert torch.equal(a, b[:5]) and torch.equal(few, many[:5]), dtype
+
+
+# ---- log probabilities -----------------------------------------------------------------------------------------------------------
+def _softmax_grad(x, actions, dlogp, dentropy, dlse, temperature):
+    """(gradient, sum of the absolute values of its terms) in 64 bits, from differences to the row's largest logit"""
+    z = x.double() / temperature
+    lp = torch.log_softmax(z - z.amax(-1, keepdim=True), -1)
+    p = lp.exp()
+    h = -(p * lp).sum(-1, keepdim=True)
+    hot = (torch.arange(x.shape[1], device=x.device)[None] == actions[:, None]).double()
+    g, e, s = (d.double()[:, None] for d in (dlogp, dentropy, dlse))
+    return ((g * (hot - p) - e * p * (lp + h) + s * p) / temperature,
+            (g.abs() * (hot + p) + e.abs() * p * (lp.abs() + h + 1) + s.abs() * p) / temperature)
+
+
+def _large_logits(gpu, n, a, dtype, seed):
+    """Rows whose logits are large beside their spread: near 2^20 in two levels, all -1e9 (a penalty), near 2^24, q values near 100."""
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(seed)
+    x = torch.randn(n, a, generator=gen, device=gpu)
+    at = torch.arange(a, device=gpu)
+    x[0::4] = 2.0 ** 20 + at % 2 * 2.0 ** 14
+    x[1::4] = -1e9
+    x[2::4] = 2.0 ** 24 + 2.0 * (at % 3)
+    x[3::4] = 100.0 + 0.03 * x[3::4]
+    r = dict(logits=x.to(dtype), actions=torch.randint(0, a, (n,), generator=gen, device=gpu, dtype=torch.int32))
+    r.update({k: torch.randn(n, generator=gen, device=gpu) for k in ("dlogp", "dentropy", "dlse")})
+    return r
+
+
+@pytest.mark.parametrize("n,a", [(9, 3), (9, 17), (50, 300), (9, 1000), (8, 1100), (5, 2500), (6, 5000), (1300, 5000), (5, 20001), (4, 70000), (1100, 33000),
+                                 (1030, 40000)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("temperature", [1.0, 0.01])
+def test_log_probability_gradient_of_large_logits(gpu, n, a, dtype, temperature):
+    """Nothing grows with |logit| / temperature: differences to the largest logit are exact or rounded once (|z| u with |z| <= 126 log 2
+    where p counts), the scale and the product as much again, the sum of A terms (64 + A / 64) u; log p and H carry as much."""
+    from purejaxql_amd import ops
+    if dtype == torch.float16 and temperature == 0.01:
+        n = min(n, 9)
+    x = _large_logits(gpu, n, a, dtype, n + a)
+    if dtype == torch.float16:      # ends at 65504
+        x["logits"] = (_large_logits(gpu, n, a, torch.float32, n + a)["logits"] % 1024).to(dtype) + 32768
+    logits, act = x["logits"], x["actions"]
+    _, ent, lse, _, _ = ops.action_logprobs(logits, act, temperature=temperature)
+    got = ops.action_logprobs_grad(logits, act, lse, ent, x["dlogp"], x["dentropy"], x["dlse"], temperature=temperature)
+    want, size = _softmax_grad(logits, act, x["dlogp"], x["dentropy"], x["dlse"], temperature)
+    e = (4 * 126 + 2 * (64 + a / 64) + 64) * U
+    floor = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126 * 200 / temperature
+    _close(got, want, HALF[dtype] * want.abs() + (1 + HALF[dtype]) * e * size + floor, "dlogits")
+
+
+@pytest.mark.parametrize("n,a", [(21, 17), (21, 200), (7, 1101), (6, 5003), (2100, 5003), (3, 60001), (1100, 40001)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["f32", "bf16"])
+def test_log_probability_gradient_of_large_and_small_logits_with_masks(gpu, n, a, dtype):
+    """Rows of large logits between ordinary ones, a third not allowed (some NaN there), rows that start anywhere; bound as above."""
+    from purejaxql_amd import ops
+    x = _large_logits(gpu, n, a, dtype, a)
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(a)
+    wide = torch.zeros(n, a + 3, dtype=dtype, device=gpu)
+    wide[:, 1:a + 1] = x["logits"]
+    wide[::2, 1:a + 1] = (torch.randn(n, a, generator=gen, device=gpu)[::2] * 3).to(dtype)
+    logits, act = wide[:, 1:a + 1], x["actions"]
+    mask = (torch.rand(n, a, generator=gen, device=gpu) < 0.67).to(torch.uint8)
+    mask.scatter_(1, act.long()[:, None], 1)
+    clean = logits.double().masked_fill(mask == 0, -1e300)          # p is 0 there in 64 bits too
+    logits[:, ::5] = torch.where(mask[:, ::5] == 0, torch.full_like(logits[:, ::5], float("nan")), logits[:, ::5])
+    _, ent, lse, _, _ = ops.action_logprobs(logits, act, mask=mask, temperature=0.5)
+    assert bool(torch.isfinite(lse).all()) and bool((lse.abs() > 32).any()) and bool((lse.abs() < 32).any())
+    got = ops.action_logprobs_grad(logits, act, lse, ent, x["dlogp"], x["dentropy"], x["dlse"], mask=mask, temperature=0.5)
+    want, size = _softmax_grad(clean, act, x["dlogp"], x["dentropy"], x["dlse"], 0.5)
+    want, size = (torch.where(mask != 0, t, torch.zeros_like(t)) for t in (want, size))
+    e = (4 * 126 + 2 * (64 + a / 64) + 64) * U
+    _close(got, want, HALF[dtype] * want.abs() + (1 + HALF[dtype]) * e * size + 2.0 ** -126 * 400 * (mask != 0), "dlogits")
