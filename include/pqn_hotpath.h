@@ -722,7 +722,8 @@ int pqn_residual_norm_grad(const pqn_residual_norm_t *args /* host */, void *str
  * allowed logits, ties to the lowest index, -1 / -inf where fewer are allowed.  An action outside 0 .. a-1 is none: logp 0, no
  * gradient; one that is not allowed: logp -inf, no gradient.  A row that allows nothing: lse -inf, entropy 0, gradient 0.  NaN or +inf
  * among the allowed logits: lse, logp, entropy NaN.  A probability below 2^-126 counts as 0.  Where logits / temperature is beyond the
- * largest float lse is infinite, logp and entropy still are what they should be, and the row's gradient is 0.
+ * largest float lse is infinite; logp, entropy and their gradients still are what they should be, but a row that is given a gradient of such
+ * an lse (dlse not 0) has gradient 0.
  * pqn_action_logprobs_grad reads logits, action, mask, lse, entropy and the gradients of logp, entropy, lse (NULL = zeros, not all) and
  * writes dlogits, 0 where not allowed. */
 #define PQN_LOGPROB_MAX_TOP 16

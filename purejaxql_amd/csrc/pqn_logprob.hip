@@ -478,23 +478,27 @@ struct lp_grad_args {
 struct LpPowers {
   float m, s;
 };
+// A logsumexp beyond the largest float (or of nothing) has no gradient of its own: a row that is given one has none at all.  logp and entropy
+// are finite there, and so are their gradients.
+PQN_D bool lp_none(float lse, float dl) { return fabsf(lse) == INFINITY && dl != 0.f; }
+PQN_D bool lp_again(float lse, float dl) { return fabsf(lse) > LP_NEAR && !lp_none(lse, dl); }   // false for NaN: so is every gradient
 PQN_D float lp_rescale(float m, float to, float scale) { return m == to ? 1.f : lp_exp2((m - to) * scale); }
 struct LpGrad {                      // a row's scalars
   float m, base, h, dlp, dh, dl, inv_temp;      // log p = (logit - m) / temperature - base
   int act;
-  bool none, near;
+  bool none, again;
   template <typename T>
   PQN_D void open(const lp_grad_args &G, long long row) {
     const lp_args &A = G.A;
     m = 0.f;
     base = A.lse[row];
-    near = !(fabsf(base) > LP_NEAR);     // NaN: so is every gradient
-    none = fabsf(base) == INFINITY;      // nothing allowed, or beyond the largest float
     h = A.entropy[row];
     act = A.action[row];
     dlp = G.dlogp ? G.dlogp[row] : 0.f;
     dh = G.dentropy ? G.dentropy[row] : 0.f;
     dl = G.dlse ? G.dlse[row] : 0.f;
+    none = lp_none(base, dl);
+    again = lp_again(base, dl);
     inv_temp = A.inv_temp;
     // an id outside the row, or an action that is not allowed, has a constant log probability
     if (act < 0 || act >= A.a || lp_logit<T>(A, row, act) == -INFINITY) dlp = 0.f;
@@ -523,7 +527,7 @@ __global__ __launch_bounds__(256) void lp_grad_rows_kernel(lp_grad_args P) {
   T *o = (T *)P.dlogits + row * A.a;
   float x[E];
   lp_row_load<T, G, E>(A, row, lane, x);
-  if (__any(!R.near)) {                            // whole waves, for the exchanges
+  if (__any(R.again)) {                            // whole waves, for the exchanges
     LpPowers v = {-INFINITY, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) v.m = fmaxf(v.m, x[e]);
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(256) void lp_grad_rows_kernel(lp_grad_args P) {
 #pragma unroll
     for (int e = 0; e < E; ++e) v.s += x[e] == -INFINITY ? 0.f : lp_exp2((x[e] - v.m) * A.scale);
     v.s = pqn_group_sum<G>(v.s);
-    if (!R.near) R.sums(v);
+    if (R.again) R.sums(v);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -635,13 +639,12 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(lp_grad_args P) {
   const int block = blockIdx.x % P.blocks;
   LpGrad R;
   R.open<T>(P, row);
-  const bool again = !R.near && !R.none;           // the workgroup's row: the same in every thread
-  if (again && !(ALONE && block < P.far)) return;
+  if (R.again && !(ALONE && block < P.far)) return;           // the workgroup's row: the same in every thread
   const LpWide<T> W(P, row);
   int step = P.blocks;
   if constexpr (ALONE) {
     __shared__ LpPowers part[4];
-    if (again) {
+    if (R.again) {
       R.sums(W.sums(P.A.scale, part));
       step = P.far;
     }
@@ -656,8 +659,8 @@ __global__ __launch_bounds__(256) void lp_grad_far_kernel(lp_grad_args P) {
   const int lane = threadIdx.x & 63;
   for (long long row0 = blockIdx.x; row0 < P.A.n; row0 += 64ll * gridDim.x) {
     const long long mine = row0 + (long long)lane * gridDim.x;
-    const float lse = mine < P.A.n ? P.A.lse[mine] : 0.f;
-    unsigned long long todo = __ballot(fabsf(lse) > LP_NEAR && fabsf(lse) < INFINITY);      // the same in every wave
+    const bool in = mine < P.A.n;
+    unsigned long long todo = __ballot(in && lp_again(P.A.lse[in ? mine : 0], P.dlse ? P.dlse[in ? mine : 0] : 0.f));   // the same in every wave
     while (todo) {
       const long long row = row0 + (long long)(__ffsll(todo) - 1) * gridDim.x;
       todo &= todo - 1;

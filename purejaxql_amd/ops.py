@@ -351,7 +351,7 @@ def action_logprobs(logits: torch.Tensor, actions: torch.Tensor, mask: Optional[
     logits [N, A] in f32, bf16 or f16 (rows may be strided), actions int32 [N] (outside 0 .. A-1: no action, logp 0), mask u8 / bool
     [N, A] (0 = not allowed, never looked at).  Returns (logp [N], entropy [N], lse [N], top_logp [N, top], top_action i32 [N, top]),
     f32; alternatives in falling order, ties to the lowest index, -inf / -1 where fewer are allowed.  A row that allows nothing has
-    lse -inf and entropy 0; one whose logits / temperature overflow has an infinite lse and no gradient."""
+    lse -inf and entropy 0; one whose logits / temperature overflow has an infinite lse, which has no gradient."""
     a = _logprob_args(logits, actions, mask, temperature, top)
     n, dev, f32 = a.n, logits.device, torch.float32
     logp, entropy, lse = torch.empty(3, n, dtype=f32, device=dev).unbind(0)
@@ -371,7 +371,7 @@ def action_logprobs_grad(logits: torch.Tensor, actions: torch.Tensor, lse: torch
                          dlse: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                          temperature: float = 1.0) -> torch.Tensor:
     """Gradient of action_logprobs with respect to the logits from those of logp, entropy and lse (f32 [N], None: zeros, not all);
-    lse and entropy as action_logprobs returned them.  0 where not allowed."""
+    lse and entropy as action_logprobs returned them.  0 where not allowed, and in a row whose lse is infinite and is given a gradient."""
     a = _logprob_args(logits, actions, mask, temperature, 0)
     n, dev = a.n, logits.get_device()
     if dlogp is None and dentropy is None and dlse is None:

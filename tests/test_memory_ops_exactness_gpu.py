@@ -118,3 +118,33 @@ def test_log_probability_gradient_of_large_and_small_logits_with_masks(gpu, n, a
     want, size = (torch.where(mask != 0, t, torch.zeros_like(t)) for t in (want, size))
     e = (4 * 126 + 2 * (64 + a / 64) + 64) * U
     _close(got, want, HALF[dtype] * want.abs() + (1 + HALF[dtype]) * e * size + 2.0 ** -126 * 400 * (mask != 0), "dlogits")
+
+
+@pytest.mark.parametrize("n,a", [(12, 17), (12, 300), (12, 5000), (1100, 5000), (12, 70000)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["f32", "bf16"])
+def test_log_probability_gradient_beyond_the_largest_float(gpu, n, a, dtype):
+    """logits / temperature overflows: lse is infinite, logp and entropy are finite and have their gradients (bound as above); a row
+    that is given a gradient of its infinite lse has none, and a row that allows nothing either."""
+    from purejaxql_amd import ops
+    big = torch.finfo(dtype).max
+    at = torch.arange(a, device=gpu)
+    l = torch.empty(n, a, device=gpu)
+    l[0::4], l[1::4], l[2::4] = -big, big, big * (1 - at % 2 * 0.5)
+    l[3::4] = torch.randn(len(range(3, n, 4)), a, device=gpu, generator=torch.Generator(device=gpu).manual_seed(a))
+    x = l.to(dtype)
+    act = (torch.arange(n, device=gpu) * 2 % a).to(torch.int32)
+    mask = torch.ones(n, a, dtype=torch.uint8, device=gpu)
+    mask[4:6] = 0
+    _, ent, lse, _, _ = ops.action_logprobs(x, act, mask=mask, temperature=0.25)
+    assert torch.equal(torch.isinf(lse), (torch.arange(n, device=gpu) % 4 != 3) | (mask[:, 0] == 0)) and bool(torch.isfinite(ent).all())
+    gen = torch.Generator(device=gpu).manual_seed(n)
+    dlogp, dent = torch.randn(n, generator=gen, device=gpu), torch.randn(n, generator=gen, device=gpu)
+    some = (torch.arange(n, device=gpu) % 3 == 0).float()
+    for dlse in (None, torch.zeros(n, device=gpu), some):
+        got = ops.action_logprobs_grad(x, act, lse, ent, dlogp, dent, dlse, mask=mask, temperature=0.25)
+        want, size = _softmax_grad(x, act, dlogp, dent, torch.zeros(n, device=gpu) if dlse is None else dlse, 0.25)
+        none = (mask == 0) | (torch.isinf(lse) & (dlse != 0) if dlse is not None else torch.zeros(n, dtype=torch.bool, device=gpu))[:, None]
+        assert bool((got[none.expand_as(got)] == 0).all())
+        want, size = (torch.where(none, torch.zeros_like(t), t) for t in (want, size))
+        e = (4 * 126 + 2 * (64 + a / 64) + 64) * U
+        _close(got, want, HALF[dtype] * want.abs() + (1 + HALF[dtype]) * e * size + 2.0 ** -126 * 800, "dlogits")
