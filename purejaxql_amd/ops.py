@@ -112,6 +112,13 @@ def _on_gpu(t: torch.Tensor, name: str, dtypes):
         raise ValueError(f"{name}: need a CUDA tensor of {' / '.join(str(d) for d in dtypes)}, got {t.dtype} on {t.device}")
 
 
+def _int32(value: int, name: str) -> int:
+    """A size for a 32-bit field of an argument block, which would drop its upper bits silently."""
+    if value > 0x7FFFFFFF:
+        raise ValueError(f"{name}: up to 2^31 - 1, got {value}")
+    return value
+
+
 def _flags(t: torch.Tensor) -> torch.Tensor:
     return t.view(torch.uint8) if t.dtype == torch.bool else t
 
@@ -140,6 +147,9 @@ def _attn_args(a, q, k, v, decay, state, reset, scale, step: bool):
     lead, dv = shape[:-1], v.shape[-1]
     if not (0 < dk <= _lib.ATTN_MAX_D and 0 < dv <= _lib.ATTN_MAX_D):
         raise ValueError(f"q, v: head widths of 1 .. {_lib.ATTN_MAX_D}, got {dk} and {dv}")
+    if (shape[0] | m | h) >> 31:
+        for name, size in zip(("steps", "rows", "heads")[-len(shape) + 1:], shape):
+            _int32(size, name)
     _last_contiguous(q, "q", shape, dt, dev)
     _last_contiguous(k, "k", shape, dt, dev)
     _last_contiguous(v, "v", lead + (dv,), dt, dev)
@@ -249,6 +259,8 @@ def _norm_args(x, f, gate, gate_act, params, norm_type, post, pre, eps):
     if (gate is None) != (gate_act == "none"):
         raise ValueError("gate and gate_act go together: a gate tensor with 'sigmoid' or 'silu', neither with 'none'")
     shape, d, dt, dev = x.shape, x.shape[-1], x.dtype, x.get_device()
+    if d >> 31:
+        _int32(d, "D")
     a = _lib.ResidualNormArgs()
     x, a.x_stride = _rows(x, "x", shape, dt, dev)
     f, a.f_stride = _rows(f, "f", shape, dt, dev)
@@ -326,6 +338,8 @@ def _logprob_args(logits, actions, mask, temperature, top):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits: need [N, A] with A >= 1, got {tuple(logits.shape)}")
     n, width = logits.shape
+    if (n | width) >> 31:
+        _int32(n, "N"), _int32(width, "A")
     dev = logits.get_device()
     _last_contiguous(logits, "logits", (n, width), logits.dtype, dev)
     _exactly(actions, "actions", (n,), torch.int32, dev)
