@@ -676,20 +676,22 @@ __global__ __launch_bounds__(256) void lp_grad_far_kernel(lp_grad_args P) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
+static float lp_scale(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }
 static int lp_check(const pqn_action_logprobs_t *a, const char *who) {
   PQN_REQUIRE(a, "%s: NULL argument block", who);
   PQN_REQUIRE(pqn_dtype_known(a->dtype), "%s: unknown dtype %d", who, a->dtype);
   PQN_REQUIRE(a->n >= 0 && a->a > 0, "%s: n must be >= 0 and a > 0 (n=%d a=%d)", who, a->n, a->a);
   PQN_REQUIRE(a->a <= (1 << 30), "%s: up to 2^30 columns (a=%d)", who, a->a);
   PQN_REQUIRE(a->top >= 0 && a->top <= LP_MAX_TOP && a->top <= a->a, "%s: top must be in 0 .. min(a, %d) (top=%d a=%d)", who, LP_MAX_TOP, a->top, a->a);
-  PQN_REQUIRE(a->temperature > 0.f && a->temperature < INFINITY && 1.0f / a->temperature < INFINITY, "%s: temperature must be positive and finite", who);
+  PQN_REQUIRE(a->temperature > 0.f && a->temperature < INFINITY && lp_scale(a->temperature) < INFINITY,
+              "%s: temperature must be positive, finite and at least 4.24e-39 (log2 e over it is a float)", who);
   if (a->n > 0) PQN_REQUIRE(a->logits && a->action && a->lse && a->entropy, "%s: NULL logits, action, lse or entropy", who);
   return PQN_OK;
 }
 static lp_args lp_fill(const pqn_action_logprobs_t *a) {
   lp_args A = {};
   A.n = a->n; A.a = a->a; A.top = a->top; A.inv_temp = 1.0f / a->temperature;
-  A.scale = (float)(1.4426950408889634 / (double)a->temperature);
+  A.scale = lp_scale(a->temperature);
   A.logits = a->logits; A.ls = a->logits_stride; A.mask = a->mask; A.ms = a->mask_stride;
   A.action = a->action; A.logp = a->logp; A.entropy = a->entropy; A.lse = a->lse;
   A.top_logp = a->top_logp; A.top_action = a->top_action;

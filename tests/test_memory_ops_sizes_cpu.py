@@ -66,3 +66,17 @@ def test_the_largest_sizes_reach_the_library():
     n = (1 << 31) - 1
     a = ops._logprob_args(_Shape(n, 3), _Shape(n, dtype=torch.int32), None, 1.0, 0)
     assert a.n == n and a.a == 3
+
+
+@pytest.mark.parametrize("temperature", [3.0e-39, 3.5e-39, 4.2e-39])
+def test_temperatures_whose_scale_is_no_float(temperature):
+    """1 / temperature is a float there, log2 e / temperature is not: the largest logit itself would come out as 0 * infinity."""
+    from purejaxql_amd import _lib
+    lib = _lib.load()
+    a = _lib.ActionLogprobsArgs(n=4, a=8, top=0, dtype=0, temperature=temperature, logits=64, logits_stride=8, action=64, logp=64, entropy=64, lse=64,
+                                dlogp=64, dlogits=64)
+    for fn in (lib.pqn_action_logprobs, lib.pqn_action_logprobs_grad):
+        a.n = 0                        # nothing would be launched, were it let through
+        assert fn(C.byref(a), None) == -1 and "temperature" in lib.pqn_last_error().decode()
+    a.temperature = 4.3e-39
+    assert lib.pqn_action_logprobs(C.byref(a), None) == 0
