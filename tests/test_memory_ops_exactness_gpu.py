@@ -45,6 +45,49 @@ def test_a_row_steps_alike_alone_and_among_many(gpu, dk, dv):
         assert torch.equal(a, b[:5]) and torch.equal(few, many[:5]), dtype
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t,m,h,dk,dv,off", [(3, 2, 2, 32, 32, False), (20, 3, 2, 32, 32, False), (20, 2, 2, 64, 64, False), (20, 2, 2, 96, 96, False), (31, 2, 2, 33, 50, False),
+                                             (32, 2, 3, 128, 128, False), (20, 2, 2, 40, 128, False), (20, 2, 2, 64, 64, True), (150, 2, 2, 32, 32, False),
+                                             (150, 2, 2, 64, 64, True), (150, 2, 2, 96, 96, False), (150, 2, 2, 96, 96, True), (150, 2, 2, 33, 50, False),
+                                             (150, 2, 2, 128, 128, False), (400, 1, 2, 64, 96, False), (300, 1, 2, 67, 40, True)])
+def test_non_finite_steps_stay_where_they_belong_in_every_form(gpu, t, m, h, dk, dv, off, dtype, bad):
+    """NaN or infinity in k, v, q, dout and a dropped state, in windows of one chunk, several and cut ones, at every number of waves, on and off
+    16 bytes: exactly the numbers that the definition makes non-finite are, and the others are right (the sums of their absolute values
+    are taken without what is bad: it is no term of theirs)."""
+    from purejaxql_amd import ops
+    x = _attn_inputs(gpu, t, m, h, dk, dv, dtype, t + dk, True, 0.0)
+    if off:
+        for n in ("q", "k", "v", "dout"):
+            wide = torch.zeros(t, m, h, x[n].shape[-1] + 1, dtype=dtype, device=gpu)
+            wide[..., 1:] = x[n]
+            x[n] = wide[..., 1:]
+    reset = torch.zeros(t, m, dtype=torch.uint8, device=gpu)
+    reset[0, 0] = reset[t // 2, 0] = 1
+    x["state"][0] = float("nan")
+    clean = {n: x[n].clone() for n in ("q", "k", "v", "dout")}
+    for n, at, head, col in (("k", t // 4, 0, 3), ("v", t // 4, 1, 5), ("q", t - 1, 0, 2), ("dout", t // 4, 1, 7)):
+        x[n][at, 0, head, col] = bad
+        clean[n][at, 0, head, col] = 0
+    state0 = x["state"].clone()
+    state0[0] = 0
+    args, kw = [x[n] for n in ("q", "k", "v")], dict(state=x["state"], reset=reset, scale=0.25)
+    out, new = ops.decay_attention(*args, x["decay"], **kw)
+    grads = ops.decay_attention_grad(*args, x["decay"], x["dout"], dstate_out=x["dstate"], **kw)
+    wide = [_d(a) for a in args]
+    want = (*ref.attention(*wide, _d(x["decay"]), _d(x["state"]), reset, 0.25),
+            *ref.attention_grad(*wide, _d(x["decay"]), _d(x["dout"]), _d(x["dstate"]), _d(x["state"]), reset, 0.25))
+    c = [_abs(clean[n]) for n in ("q", "k", "v")]
+    most = (*ref.attention(*c, _d(x["decay"]), _abs(state0), reset, 0.25),
+            *ref.attention_grad(*c, _d(x["decay"]), _abs(clean["dout"]), _abs(x["dstate"]), _abs(state0), reset, 0.25))
+    e = (2 * t + dk + dv + 16) * U
+    for name, g, w, a in zip(("out", "state", "dq", "dk", "dv", "dstate"), (out, new, *grads), want, most):
+        fine = torch.isfinite(w)
+        assert torch.equal(torch.isfinite(g), fine), (name, int((torch.isfinite(g) != fine).sum()))
+        half = HALF[dtype] if g.dtype != torch.float32 else 0.0
+        _close(g[fine], w[fine], (e * a + half * (w.abs() + e * a) + 1e-30)[fine], name)
+
+
 # ---- log probabilities -----------------------------------------------------------------------------------------------------------
 def _softmax_grad(x, actions, dlogp, dentropy, dlse, temperature):
     """(gradient, sum of the absolute values of its terms) in 64 bits, from differences to the row's largest logit"""

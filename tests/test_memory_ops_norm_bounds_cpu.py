@@ -6,8 +6,6 @@ import torch
 from tests import memory_ops_reference as ref
 from tests import norm_bounds as nb
 
-SMALL = [s for s in nb.SHAPES if s[0] * s[1] <= 1 << 21]
-
 
 def _f32(x, kind, act, post=True, pre=True):
     """The same in plain f32 torch, by autograd: rows of f32 whatever the inputs' type."""
@@ -17,7 +15,7 @@ def _f32(x, kind, act, post=True, pre=True):
     return {"y": y, "h": h, **{"d" + k: g for k, g in zip(leaves, grads)}}
 
 
-@pytest.mark.parametrize("n,d,act,params,strided", SMALL)
+@pytest.mark.parametrize("n,d,act,params,strided", nb.SHAPES)
 @pytest.mark.parametrize("kind", ["layer_norm", "rms_norm"])
 def test_f32_is_within_and_a_lost_gradient_is_not(n, d, act, params, strided, kind):
     x = nb.inputs("cpu", n, d, torch.float32, n + d, act, params, strided)
