@@ -3,8 +3,9 @@
 their accumulator input (D != C but sharing registers).  ROCm 7.2 emits these for v_mfma_f32_16x16x32_bf16 builtins;
 on MI355X they produced timing-dependent wrong results in the conv phase of the training kernel (DESIGN.md,
 "compiler hazard").  The bf16x3 path therefore issues that instruction as tied inline asm; this script is the guard
-that no builtin-generated instance is left.  Usage: tools/check_mfma_overlap.py [file.hip ...]   (exit 1 on a hit)"""
+that no builtin-generated instance is left, and that nothing touches the result of such an asm product before it is there.  Usage: tools/check_mfma_overlap.py [file.hip ...]   (exit 1 on a hit)"""
 import os, re, subprocess, sys, tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "purejaxql_amd", "csrc")
@@ -134,29 +135,36 @@ def scan_m0(asm_path):
             if re.search(r'\bm0\b', line.split(";")[0]) and not M0_OK.match(line.split(";")[0])]
 
 
+def assembly(f, out):
+    """The gfx950 assembly of a HIP source, as the Makefile builds it"""
+    extra = ["-fno-slp-vectorize"] if os.path.basename(f) == "pqn_qnet_pos.hip" else []
+    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang",
+                    "-packed-fp32-ops", *extra, "--cuda-device-only", "-S", f, "-o", out], check=True, cwd=CSRC, stderr=subprocess.DEVNULL)
+
+
+def scanned(f):
+    """(partial overlaps, early accesses, uses of M0) of a source"""
+    with tempfile.TemporaryDirectory() as td:
+        out = os.path.join(td, "x.s")
+        assembly(f, out)
+        return scan(out), scan_unfinished(out), scan_m0(out) if os.path.basename(f) == "pqn_qnet_pos.hip" else []
+
+
 def main():
     files = [os.path.abspath(f) for f in sys.argv[1:]] or [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".hip")]
     bad = 0
-    for f in files:
-        with tempfile.TemporaryDirectory() as td:
-            out = os.path.join(td, "x.s")
-            extra = ["-fno-slp-vectorize"] if os.path.basename(f) == "pqn_qnet_pos.hip" else []     # as the Makefile builds it
-            subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *extra,
-                            "--cuda-device-only", "-S", f, "-o", out], check=True, cwd=CSRC, stderr=subprocess.DEVNULL)
-            hits, early = scan(out), scan_unfinished(out)
-            if os.path.basename(f) == "pqn_qnet_pos.hip":
-                m0 = scan_m0(out)
-                print("%-20s %d uses of M0 other than the LDS-DMA destination writes" % (os.path.basename(f), len(m0)))
+    with ThreadPoolExecutor(4) as pool:
+        for f, (hits, early, m0) in zip(files, pool.map(scanned, files)):
+            name = os.path.basename(f)
+            if name == "pqn_qnet_pos.hip":
+                print("%-20s %d uses of M0 other than the LDS-DMA destination writes" % (name, len(m0)))
                 for ln, l in m0[:8]:
                     print("    line %d  %s" % (ln, l))
-                bad += len(m0)
-        print("%-20s %d partially overlapping MFMA D/C" % (os.path.basename(f), len(hits)))
-        for k, ln, l in hits[:12]:
-            print("    %s:%d  %s" % (k[:50], ln, l))
-        print("%-20s %d accesses to the result of a bf16 product within %d wait states" % (os.path.basename(f), len(early), WAIT))
-        for k, ln, l in early[:12]:
-            print("    %s:%d  %s" % (k[:50], ln, l))
-        bad += len(hits) + len(early)
+            print("%-20s %d partially overlapping MFMA D/C" % (name, len(hits)))
+            print("%-20s %d accesses to the result of a bf16 product within %d wait states" % (name, len(early), WAIT))
+            for k, ln, l in hits[:12] + early[:12]:
+                print("    %s:%d  %s" % (k[:50], ln, l))
+            bad += len(hits) + len(early) + len(m0)
     sys.exit(1 if bad else 0)
 
 
