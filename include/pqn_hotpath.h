@@ -653,7 +653,7 @@ int pqn_bigmlp_gemm(int32_t m, int32_t n, int32_t k, const float *a, int64_t lda
  * Tensors are f32, bf16 or f16 as `dtype` says; sums, states, statistics and parameters are f32, and a 16-bit output is rounded once,
  * to nearest even.  Strides count elements; the last index of every tensor is contiguous, outputs are contiguous.  Outputs must not
  * overlap inputs unless an entry says so.  Workspaces are scratch of one call: two calls that may run at the same time need two.  A
- * call that one launch of 2^32 threads does not cover (some 2^26 (row, head) pairs, 2^29 rows of a few logits) is refused. */
+ * call that one launch of 2^32 threads does not cover (some 2^26 (row, head) pairs, 2^29 rows of a few logits, 2^24 of over 256) is refused. */
 enum { PQN_DTYPE_F32 = 0, PQN_DTYPE_BF16 = 1, PQN_DTYPE_F16 = 2 };
 
 /* Linear attention with a decay per head, cut at episode ends (the role of ScannedRNN, pqn_rnn_gymnax.py:26-54: resets come BEFORE
@@ -664,7 +664,8 @@ enum { PQN_DTYPE_F32 = 0, PQN_DTYPE_BF16 = 1, PQN_DTYPE_F16 = 2 };
  * pqn_decay_attn      reads q, k, v, decay, state_in, reset; writes out, state_out
  * pqn_decay_attn_grad reads those but out / state_out, and dout, dstate_out (the gradient of state_out); writes dq, dk, dv and, where
  *                     wanted, dstate_in.
- * Bit-identical in every run.  A NaN or infinity in q, k, v reaches the steps behind it in its episode and no others. */
+ * Bit-identical in every run; a single step of the forward also whatever number of rows there is.  A NaN or infinity in q, k, v reaches the
+ * steps behind it in its episode and no others (an infinity may arrive as a NaN). */
 #define PQN_ATTN_MAX_D 128
 typedef struct {
   int32_t t_len, m, heads, dk, dv; /* dk, dv <= PQN_ATTN_MAX_D */
@@ -723,7 +724,7 @@ int pqn_residual_norm_grad(const pqn_residual_norm_t *args /* host */, void *str
  * gradient; one that is not allowed: logp -inf, no gradient.  A row that allows nothing: lse -inf, entropy 0, gradient 0.  NaN or +inf
  * among the allowed logits: lse, logp, entropy NaN.  A probability below 2^-126 counts as 0.  Where logits / temperature is beyond the
  * largest float lse is infinite; logp, entropy and their gradients still are what they should be, but a row that is given a gradient of such
- * an lse (dlse not 0) has gradient 0.
+ * an lse (dlse not 0) has gradient 0.  Logits of a row that differ by more than the largest float count as infinitely far apart.
  * pqn_action_logprobs_grad reads logits, action, mask, lse, entropy and the gradients of logp, entropy, lse (NULL = zeros, not all) and
  * writes dlogits, 0 where not allowed. */
 #define PQN_LOGPROB_MAX_TOP 16

@@ -174,18 +174,19 @@ static bool da_vec(const pqn_decay_attn_t *a, int grad) {
 
 // Windows of up to this many steps go step by step, longer ones by chunks; a single step of the forward always does, so that a row acts
 // alike (to the bit) whatever number of rows acts beside it.  Measured on both sides, us forward / gradient: 4096 x 4 heads of 32, f32, 2
-// steps 30 / 90 against 46 / 113 by chunks, 4 steps 37 / 110 against 45 / 107, 6 steps 46 / 135 against 45 / 107; 1024 x 8 heads of 64, f32,
-// 1 step 48 / 137 against 75 / 175; 1024 x 8 heads of 128, 1 step, f32 218 / 585 against 224 / 508, bf16 218 / 657 against 205 / 441; bf16
+// steps 32 / 89 against 49 / 111 by chunks, 4 steps 39 / 114 against 47 / 116, 6 steps 50 / 149 against 47 / 124; 1024 x 8 heads of 64, f32,
+// 1 step 51 / 144 against 77 / 190; 1024 x 8 heads of 128, 1 step, f32 218 / 595 against 239 / 539, bf16 218 / 674 against 209 / 440; bf16
 // steps in place of 1024 x 8 heads: 128 x 128 225 against 212, 72 x 128 133 against 198, 128 x 32 54 against 110; 256 x 8 of 96 x 96 32 and
-// 41.  Off 16 bytes chunks load element by element: 1000 x 4 heads of 127, 3 steps f32 212 / 396 against 238 / 547, 2 steps bf16 219 / 395
-// against 216 / 521, 4 steps bf16 275 / 575 against 219 / 528; 4000 x 8 heads of 33 and 65, 3 steps bf16 328 / 1170 against 645 / 2429.
+// 41.  Off 16 bytes chunks load element by element: 1000 x 4 heads of 127, 3 steps f32 213 / 400 against 238 / 560, 2 steps bf16 219 / 408
+// against 229 / 600, 4 steps bf16 277 / 585 against 232 / 607; 4000 x 8 heads of 33 and 65, 3 steps bf16 329 / 1176 against 675 / 2695.
 static bool da_by_steps(const pqn_decay_attn_t *a, bool grad) {
   const int w = a->dk > a->dv ? a->dk : a->dv;
   return a->t_len <= (w <= 32 ? 4 : !da_vec(a, grad) ? 3 : w <= 64 || !grad || (long long)a->m * a->heads < 2048 ? 1 : 0);
 }
 // The time axis is cut where rows x heads alone give the chip too few waves: parts of at least DA_MIN_PART steps (each costs a second
-// reading of k and v and a state written and read), as many as make DA_FILL waves.  Measured, 1001 steps x 35 rows of 48 and 80 columns,
-// f32, forward / gradient: parts of 64 or more 61 / 174 us, 128 63 / 202, 256 97 / 273; 16001 x 16 rows, bf16: 2048 waves 112 us, 4096 121.
+// reading of k and v and a state written and read), as many as make DA_FILL waves, in whole chunks: 1001 steps x 35 rows of 48 and 80 columns
+// go in 11 parts of 96.  Measured there, f32, forward / gradient: parts of at least 64 52 / 126 us, 128 52 / 147, 256 91 / 213; 16001 x 16
+// rows of 64 and 128, bf16: 1024 waves 165 / 451, 2048 109 / 300, 4096 112 / 331; 5000 x 8 of 128 and 128, bf16: 55 / 125, 51 / 88, 51 / 102.
 static constexpr int DA_MIN_PART = 64, DA_FILL = 2048;
 
 static da_split da_cut(int t_len, long long rows, int passes, int a, int b, int vec) {
@@ -352,9 +353,9 @@ extern "C" int pqn_decay_attn_grad(const pqn_decay_attn_t *a, void *stream) {
     PQN_REQUIRE(a->workspace || pqn_decay_attn_workspace_bytes(a, 1) == 0, "pqn_decay_attn_grad: NULL workspace");
     // dq and dk have states of [dv][dk], dv of [dk][dv].  One launch of the kernel that holds both where that is nearly the kernel of
     // each, or where there is little to do in several launches (the time axis is cut) and they are more than the padding.  Measured on
-    // both sides, together / one after the other, us: 300 steps x 6 rows, 32 and 128 columns, f32 48 / 77, bf16 33 / 57; 1001 x 35, 48
-    // and 80, f32 166 / 148, bf16 79 / 90; 5000 x 8, 64 and 128, bf16 75 / 114; 4000 x 160, 32 and 64, f32 782 / 582, bf16 328 / 281;
-    // 32 x 512, 80 and 48, f32 61 / 52 (not cut); 300 x 480, 128 and 96, bf16 133 / 165.
+    // both sides, together / one after the other, us: 300 steps x 6 rows, 32 and 128 columns, f32 49 / 80, bf16 37 / 63; 1001 x 35, 48
+    // and 80, f32 136 / 126, bf16 80 / 88; 5000 x 8, 64 and 128, bf16 88 / 102; 4000 x 160, 32 and 64, f32 813 / 595, bf16 416 / 344;
+    // 32 x 512, 80 and 48, f32 51 / 48 (not cut); 300 x 480, 128 and 96, bf16 177 / 205.
     const int w = a->dk > a->dv ? a->dk : a->dv, least = a->dk + a->dv - w;
     const bool same = da_ap(least, vec) == da_ap(w, vec) && da_nw(least, w, vec) == da_nw(w, w, vec) && da_nw(w, least, vec) == da_nw(w, w, vec);
     const bool alike = same || least > 64 || (least > 32 && w <= 64);

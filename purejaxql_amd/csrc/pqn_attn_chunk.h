@@ -36,18 +36,20 @@ struct da_args {
 //
 // bf16: v_mfma_f32_16x16x32_bf16.  What is f32 and an operand -- the state (S^T Q^T), the weighted products (V^T P^T), w V -- is three bf16
 // pieces, which hold it exactly: sums and states are f32 and an output is rounded once.  With the state and the weights as one bf16 number
-// each (2.5e-3 rms on the outputs instead of 1.7e-3, their own rounding) 128 steps x 2048 rows of 128 x 128 took 123 / 266 us, now 137 / 321:
+// each (2.5e-3 rms on the outputs instead of 1.7e-3, their own rounding) calls of 128 steps x 2048 rows of 128 x 128 took 123 / 266 us, now
+// 137 / 321 (in turn, one session):
 // 111 matrix instructions a chunk and wave instead of 71, and some 300 vector instructions.  f32: v_mfma_f32_16x16x4_f32 throughout, four
 // of them per 16 values of k.
 //
-// Bound: HBM where there are rows enough.  A chunk of 32 steps of 128 + 128 bf16 columns moves 32 KB (about 3900 cycles of a CU's share
-// of the bandwidth) and costs a wave 111 matrix instructions of 16 cycles; f32 doubles the bytes and costs four times the instructions at
-// 32 cycles each, about as much as the bytes.  Chunks of 32 steps and not 64: half the registers in flight, no spills, two waves a SIMD
-// (heads of 128, 128 steps x 2048 rows, bf16, gradient: 267 us).  Next chunk's loads are in flight in registers while a chunk is computed.
-// Measured, forward / gradient: bf16, 128 steps x 2048 rows of 128 x 128: 128 / 267 us (floors 106 / 171 by the bytes at 5.08 TB/s); f32,
-// 32 steps x 16384 rows of 32 x 32: 118 / 267 us (79 / 132; the three scans of the gradient read the window nearly twice); one step of
-// 8192 bf16 rows of 128 x 128: 216 us, 5.0 TB/s; f32, 1001 steps x 35 rows of 48 x 80: 50 / 124 us (latency: three launches a scan, each
-// a few chunks deep).
+// Bound: HBM and the vector and matrix work together where there are rows enough.  A chunk of 32 steps of 128 + 128 bf16 columns moves 32 KB
+// (about 3900 cycles of a CU's share of the bandwidth) and costs a wave 111 matrix instructions of 16 cycles beside its vector work; f32
+// doubles the bytes and costs four times the instructions at 32 cycles each, about as much as the bytes.  Chunks of 32 steps and not 64:
+// half the registers in flight, two waves a SIMD.  Of the 48 kernels of a type six (bf16) and nine (f32) still spill, 8 to 116 bytes a
+// lane -- f32 heads of 32 in one chunk 36 at three waves a SIMD, 128 x 64 and 128 x 96 up to 80 --, bf16 and f32 heads of 128 x 128 on 16
+// bytes do not.  Next chunk's loads are in flight in registers while a chunk is computed.
+// Measured, forward / gradient (the kernels' least under a trace): bf16, 128 steps x 2048 rows of 128 x 128: 140 / 353 us (floors 106 / 171 by
+// the bytes at 5.08 TB/s); f32, 32 steps x 16384 rows of 32 x 32: 117 / 270 us (79 / 132; the three scans of the gradient read the window
+// nearly twice); whole calls of f32, 1001 steps x 35 rows of 48 x 80: 52 / 126 us (latency: three launches a scan, parts three chunks deep).
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef pqn_bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -741,7 +743,7 @@ __global__ __launch_bounds__(64 * NW, MODE == DA_ONE && AP == 32 ? 3 : 2) void d
 }
 
 // widths as the kernel is built for them: rows of the state padded to AP, 32 columns a wave.  96 beside the powers of two: 200 steps x 800
-// rows of 96 x 96, forward / gradient, f32 138 / 331 us, padded to 128 172 / 415, bf16 60 / 134 and 70 / 160.  Tensors whose rows are not
+// rows of 96 x 96, forward / gradient, f32 142 / 334 us, padded to 128 175 / 418, bf16 75 / 173 and 89 / 209.  Tensors whose rows are not
 // whole 16-byte accesses go element by element, in fewer forms.
 inline int da_ap(int a, int vec) { return a <= 32 && vec ? 32 : a <= 64 ? 64 : a <= 96 && vec ? 96 : 128; }
 inline int da_nw(int a, int b, int vec) {

@@ -10,9 +10,10 @@
 // the order of the work.
 //
 // Bound: HBM for many logits (about 9 vector operations and one v_exp_f32 a logit, below the time its bytes take), latency for few.
-// Measured, forward / gradient: 4096 x 32000 bf16, five alternatives 61 / 96 us, none 49 (4.3 - 5.4 TB/s; part of the gradient's reads
-// come from the last-level cache); 131072 x 17 f32 with masks and three alternatives 8.8 / 8.3 us (vector work of joining 17 logits over
-// lanes); 8 x 100003 bf16, eight alternatives, 8.3 us and 6.8 us for joining 25 parts a row (latency).
+// Measured, forward / gradient in turn (the kernels' least under a trace): 4096 x 32000 bf16, five alternatives 74 / 81 + 4 us (52 and 103 by
+// their bytes at 5.08 TB/s: part of the gradient's reads come from the last-level cache); 131072 x 17 f32 with masks and three alternatives
+// 8.5 / 7.7 us (vector work of joining 17 logits over lanes); 8 x 100003 bf16, eight alternatives, 7.6 us and 5.8 us for joining 25 parts a
+// row (latency).
 #include <type_traits>
 
 #include "pqn_vec.h"

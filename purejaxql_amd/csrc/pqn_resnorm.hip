@@ -9,9 +9,10 @@
 // instead of reading a stored y: the same bytes, and no rounding between the two halves.
 //
 // Bound: HBM.  Waves walk over rows with the parameters in registers and the next row's loads in flight; 8 columns per thread keep
-// the gradient's row tensors, parameters and five column sums within the registers of three waves per SIMD.  Measured, forward /
-// gradient: 131072 x 1024 bf16 with a gate and all parameters 275 / 445 + 10 us (column sums), 4.9 / 4.8 TB/s; 4099 x 4095 f32, element by
-// element, 63 / 113 + 14 us, 5.3 / 4.7 TB/s; 128 x 128 f32 3.7 us, latency (12.5 with the call).
+// the gradient's row tensors, parameters and five column sums within the registers of two waves per SIMD (160 to 244 at 512 to 4096 columns;
+// over 4096, 1024 threads with 128 registers, of which silu in 16 bits spills up to 20 bytes a lane and f32 up to 100).  Measured, forward /
+// gradient (the kernels' least under a trace): 131072 x 1024 bf16 with a gate and all parameters 270 / 439 + 9 us (column sums), 5.0 / 4.9
+// TB/s; 4099 x 4095 f32, element by element, 63 / 115 + 13 us, 5.3 / 4.7 TB/s; 128 x 128 f32 3.2 us, latency (12.8 with the call).
 #include <type_traits>
 
 #include "pqn_vec.h"
@@ -66,7 +67,7 @@ PQN_D void rn_row_sum(float (&v)[K], float *lds, int &turn) {
 // Thread `lane` of the NT holds NV accesses of VW columns, the i-th from (i NT + lane) VW on.  LOOSE: the rows start anywhere and their
 // width is no multiple of VW; the access that would end behind the row ends at its last column instead, and what it shares with the one
 // before is that one's.  For rows of more than RN_WIDE columns, whose kernels have no registers for an address and a condition per
-// element: 2799 x 5394 bf16, forward / gradient 67 / 168 us, element by element 101 / 362; 18326 x 1163 60 / 157 and 56 / 145.
+// element: 2799 x 5394 bf16, forward / gradient 65 / 166 us, element by element 101 / 362; 18326 x 1163 60 / 157 and 56 / 145.
 template <typename T, int NT, int VW, int NV, bool LOOSE>
 struct RnRow {
   static constexpr int E = VW * NV;

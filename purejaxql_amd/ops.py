@@ -188,7 +188,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     q, k [T, M, H, Dk], v [T, M, H, Dv] (f32 or bf16, Dk and Dv up to 128, any strides with a contiguous last index), decay f32 [H]
     in [0, 1], state f32 [M, H, Dk, Dv] (None: zeros), reset u8 / bool [T, M] (the flag comes BEFORE its step: done of the step
     before; what it drops may be NaN).  Returns (out [T, M, H, Dv], the state behind the last step or None).  A NaN or infinity in
-    q, k, v reaches the steps behind it in its episode and no others."""
+    q, k, v reaches the steps behind it in its episode and no others.  Autograd records nothing: the gradient is decay_attention_grad."""
     lib = _lib.load()
     a = _lib.DecayAttnArgs()
     lead, st = _attn_args(a, q, k, v, decay, state, reset, scale, False)
@@ -202,8 +202,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
                          reset: Optional[torch.Tensor] = None, scale: float = 1.0) -> torch.Tensor:
-    """One step of decay_attention for acting: q, k [M, H, Dk], v [M, H, Dv], reset [M]; `state` is advanced in place.  Returns
-    out [M, H, Dv]."""
+    """One step of decay_attention for acting: q, k [M, H, Dk], v [M, H, Dv], reset [M]; `state` is advanced in place, with
+    the same bits whatever other rows there are.  Returns out [M, H, Dv]; autograd records nothing."""
     lib = _lib.load()
     if state is None:
         raise ValueError("state: a step advances a state, pass zeros for a new one")
@@ -288,7 +288,7 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, gate: Optional[torch.Tensor]
 
     x the residual stream, f the block's output, gate (act "sigmoid" or "silu") [..., D] in f32, bf16 or f16, D up to 8192; parameters
     f32 [D], None = 1 (scales) or 0 (biases).  norm_type "layer_norm" or "rms_norm"; post=False leaves f as it is, pre=False returns
-    no h.  Returns (y, h or None)."""
+    no h.  Returns (y, h or None).  Autograd records nothing: the gradient is residual_norm_grad."""
     params = dict(zip(_NORM_PARAMS, (res_scale, post_scale, post_bias, pre_scale, pre_bias)))
     a, shape, keep = _norm_args(x, f, gate, gate_act, params, norm_type, post, pre, eps)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -365,7 +365,8 @@ def action_logprobs(logits: torch.Tensor, actions: torch.Tensor, mask: Optional[
     logits [N, A] in f32, bf16 or f16 (rows may be strided), actions int32 [N] (outside 0 .. A-1: no action, logp 0), mask u8 / bool
     [N, A] (0 = not allowed, never looked at).  Returns (logp [N], entropy [N], lse [N], top_logp [N, top], top_action i32 [N, top]),
     f32; alternatives in falling order, ties to the lowest index, -inf / -1 where fewer are allowed.  A row that allows nothing has
-    lse -inf and entropy 0; one whose logits / temperature overflow has an infinite lse, which has no gradient."""
+    lse -inf and entropy 0; one whose logits / temperature overflow has an infinite lse, which has no gradient.
+    Autograd records nothing: the gradient is action_logprobs_grad."""
     a = _logprob_args(logits, actions, mask, temperature, top)
     n, dev, f32 = a.n, logits.device, torch.float32
     logp, entropy, lse = torch.empty(3, n, dtype=f32, device=dev).unbind(0)
