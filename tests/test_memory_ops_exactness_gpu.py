@@ -191,3 +191,67 @@ def test_log_probability_gradient_beyond_the_largest_float(gpu, n, a, dtype):
         want, size = (torch.where(none, torch.zeros_like(t), t) for t in (want, size))
         e = (4 * 126 + 2 * (64 + a / 64) + 64) * U
         _close(got, want, HALF[dtype] * want.abs() + (1 + HALF[dtype]) * e * size + 2.0 ** -126 * 800, "dlogits")
+
+
+# ---- captured and replayed -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,a", [(1100, 5003), (5, 60001), (300, 200)])
+def test_gradients_of_large_and_small_logits_captured(gpu, n, a):
+    """The rows that are read again are found on the device: a graph replayed on rows of other sizes, with eager work between."""
+    from purejaxql_amd import ops
+    x = _large_logits(gpu, n, a, BF16, a)
+    near = torch.randn(n, a, device=gpu, generator=torch.Generator(device=gpu).manual_seed(n)).to(BF16)
+    logits = near.clone()
+
+    def run(z):
+        logp, ent, lse, _, _ = ops.action_logprobs(z, x["actions"])
+        return logp, ops.action_logprobs_grad(z, x["actions"], lse, ent, x["dlogp"], x["dentropy"], x["dlse"])
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        run(logits)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        got = run(logits)
+    for turn in range(4):
+        new = near.clone()
+        new[turn::3 if turn else 1] = x["logits"][turn::3 if turn else 1]
+        logits.copy_(near if turn == 2 else new)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got, run(logits)):
+            assert torch.equal(g, w), turn
+
+
+@pytest.mark.parametrize("t,m,dk,dv", [(900, 1, 64, 128), (20, 40, 128, 128), (130, 3, 33, 50)])
+def test_bf16_attention_captured(gpu, t, m, dk, dv):
+    """A window and its gradient, the time axis cut or not, captured and replayed on other inputs."""
+    from purejaxql_amd import ops
+    x, y = (_attn_inputs(gpu, t, m, 2, dk, dv, BF16, s, True, 0.01) for s in (1, 2))
+
+    def run(z):
+        kw = dict(state=z["state"], reset=z["reset"])
+        out = ops.decay_attention(z["q"], z["k"], z["v"], z["decay"], **kw)
+        return [*out, *ops.decay_attention_grad(z["q"], z["k"], z["v"], z["decay"], z["dout"], dstate_out=z["dstate"], **kw)]
+
+    live = {k: v.clone() for k, v in x.items()}
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        run(live)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        got = run(live)
+    for turn in range(4):
+        for k, v in (x, y)[turn % 2].items():
+            live[k].copy_(v)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got, run((x, y)[turn % 2])):
+            assert torch.equal(g, w), turn
